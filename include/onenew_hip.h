@@ -367,6 +367,92 @@ typedef struct onhip_attention_desc {
 int onhip_attention(const onhip_attention_desc_t *d, const void *q, const void *k, const void *v, void *out,
                     void *stream);
 
+/* ---- a paged key-value cache and the attention around it: what a generating transformer has between its projections ------------
+ * No counterparts in the reference, whose KV_CACHE_INFO_S (common/nn_common.h) has nothing behind it.  Tensors are bf16 or fp16
+ * (`compute`: ONHIP_COMPUTE_BF16 or _F16), the head dimension 64 or 128 and contiguous, everything 16-byte aligned, strides in elements and
+ * multiples of 8.  Indices, lengths, tables and ranges are int32 arrays in device memory that the kernels check themselves: nothing outside
+ * the cache is read or written whatever they hold.  The calls use no shared workspace: calls on different streams may overlap, as long as
+ * they are not handed the same workspace, result or cache rows that one of them writes.
+ *
+ * The cache: `pages` pages of `page_tokens` rows (a power of two up to 1024) for each of `kv_heads` heads; element (page, head, row, channel)
+ * of k at page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + channel, v likewise.  quantised == 0: rows of the 16-bit type.
+ * quantised == 1: int8 rows (strides multiples of 16) and one fp32 scale a row at page * scale_strides[0] + head * scale_strides[1] +
+ * row * scale_strides[2] of k_scale / v_scale; a value is int8 * scale. */
+typedef struct onhip_cache_desc {
+    int32_t pages, page_tokens, kv_heads, head_dim;
+    int32_t compute, quantised;
+    long long k_strides[3], v_strides[3], scale_strides[3];
+    void *k, *v;
+    float *k_scale, *v_scale;   /* quantised only */
+} onhip_cache_desc_t;
+
+/* Rows of q, k and v (e.g. slices of one projection's rows) on their way to attention and into the cache.  For each token and head, in fp32:
+ *   norm       x * 1 / sqrt(mean(x^2) + eps) * weight[channel], on q where q_weight is given, on k where k_weight is
+ *   rotation   of q and k: the first 2 * pairs channels in pairs (a, b) -> (a cos - b sin, b cos + a sin), pair i being the channels i and
+ *              i + pairs, or with `interleaved` 2 i and 2 i + 1, by the angle positions[token] * inv_freq[i] (product and reduction in 64 bits);
+ *              pairs a multiple of 8, 0 for no rotation
+ *   q          rounded to q_out, which may be q itself
+ *   k, v       to row slots[token] % page_tokens of page slots[token] / page_tokens, rounded to the 16-bit type, or as
+ *              rint(x * 127 / max|x|) with the scale max|x| / 127 (0 for a row of zeros, NaN for a row with an infinity or a NaN in it).
+ * A token whose slot is outside the cache (-1 for padding) leaves the cache as it is; a slot belongs to one token of a call (one that is
+ * named twice holds bytes of both).  Strides are (token, head). */
+typedef struct onhip_cache_rows_desc {
+    int32_t tokens, q_heads;
+    long long q_strides[2], k_strides[2], v_strides[2], out_strides[2];
+    int32_t pairs, interleaved;
+    float eps;
+} onhip_cache_rows_desc_t;
+int onhip_cache_append(const onhip_cache_desc_t *c, const onhip_cache_rows_desc_t *r, const void *q, const void *k, const void *v,
+                       const int32_t *positions, const int32_t *slots, const float *inv_freq, const float *q_weight,
+                       const float *k_weight, void *q_out, void *stream);
+
+/* The first `tokens` rows of every sequence in order, k and v as values of the 16-bit type: element (sequence, head, token, channel) at
+ * sequence * strides[0] + head * strides[1] + token * strides[2] + channel of the results.  Sequence b has lengths[b] rows; row t of it is row
+ * t % page_tokens of page table[b * table_stride + t / page_tokens].  Rows behind the last come out as zeros, rows whose page does not exist (a
+ * number outside the cache, or past the table's table_pages entries) as NaN. */
+int onhip_cache_read(const onhip_cache_desc_t *c, const int32_t *table, long long table_stride, int32_t table_pages,
+                     const int32_t *lengths, int32_t batch, int32_t tokens, void *k_out, const long long k_out_strides[3], void *v_out,
+                     const long long v_out_strides[3], void *stream);
+
+/* Attention of one new token a sequence, which is the last of its lengths[b] rows in the cache:
+ *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * (lengths[b] - 1 - j) where slopes are given
+ *   out = Softmax(s) v   over j in [0, lengths[b]), or with window > 0 the last `window` of them.
+ * Query head h reads key-value head h / (q_heads / kv_heads).  Strides are (sequence, head).  A sequence of length 0 or less gives zeros; one
+ * whose table names a page that does not exist, or is longer than its table, NaN.  The keys of a sequence may be shared out among
+ * workgroups whose parts go through `workspace` (16-byte aligned, onhip_attention_paged_workspace bytes; 0: none needed) and are joined in a
+ * fixed order: the same call gives the same bits. */
+typedef struct onhip_paged_attention_desc {
+    int32_t batch, q_heads;
+    int32_t table_pages;        /* entries of a sequence's row of the table, table_stride apart; at most 2^30 tokens */
+    int32_t window;
+    long long table_stride;
+    long long q_strides[2], out_strides[2];
+    float scale, softcap;
+} onhip_paged_attention_desc_t;
+size_t onhip_attention_paged_workspace(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d);
+int onhip_attention_paged(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table,
+                          const int32_t *lengths, const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention of prompts: any number of queries and keys, masks, capped and biased scores.  Query i is at place P = i + q_offset among the keys
+ * and sees key j when all of these hold:
+ *   causal     j <= P                       (where causal != 0)
+ *   window     P - j < window               (where window > 0)
+ *   ranges     begin <= j < end, the pair ranges[(b * q_tokens + i) * 2] (where given: documents of a packed batch, prefixes, padded lengths)
+ *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * |P - j| where slopes are given
+ *   out = Softmax(s) v over the keys seen, zeros where none is.
+ * Keys and values that a row does not see are kept out of it whatever they hold, infinities and NaN included.  Query head h reads key-value
+ * head h / (q_heads / kv_heads).  Strides are (batch, head, token).  workspace as for onhip_attention_paged.  onhip_attention is the form for
+ * at most 256 tokens without a mask, and for fp32. */
+typedef struct onhip_masked_attention_desc {
+    int32_t batch, q_heads, kv_heads, q_tokens, k_tokens, head_dim;
+    long long q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+    float scale, softcap;
+    int32_t causal, window, q_offset, compute;
+} onhip_masked_attention_desc_t;
+size_t onhip_attention_masked_workspace(const onhip_masked_attention_desc_t *d);
+int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q, const void *k, const void *v, const int32_t *ranges,
+                           const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 /* out[m][n] = sum_k a[m][k] * w[n][k] + bias[n].  Replaces gemm.c eval (:9). */
 int onhip_gemm_f32(int32_t m, int32_t k, int32_t n, const float *a, const float *w,
                    const float *bias, float *out, void *stream);

@@ -220,6 +220,37 @@ class AttentionDesc(C.Structure):
                 ("out_strides", C.c_longlong * 3), ("scale", C.c_float), ("compute", C.c_int32)]
 
 
+class CacheDesc(C.Structure):
+    """onhip_cache_desc_t"""
+    _fields_ = [("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("compute", C.c_int32), ("quantised", C.c_int32),
+                ("k_strides", C.c_longlong * 3), ("v_strides", C.c_longlong * 3), ("scale_strides", C.c_longlong * 3),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class CacheRowsDesc(C.Structure):
+    """onhip_cache_rows_desc_t"""
+    _fields_ = [("tokens", C.c_int32), ("q_heads", C.c_int32),
+                ("q_strides", C.c_longlong * 2), ("k_strides", C.c_longlong * 2), ("v_strides", C.c_longlong * 2),
+                ("out_strides", C.c_longlong * 2), ("pairs", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
+
+
+class PagedAttentionDesc(C.Structure):
+    """onhip_paged_attention_desc_t"""
+    _fields_ = [("batch", C.c_int32), ("q_heads", C.c_int32), ("table_pages", C.c_int32), ("window", C.c_int32),
+                ("table_stride", C.c_longlong), ("q_strides", C.c_longlong * 2), ("out_strides", C.c_longlong * 2),
+                ("scale", C.c_float), ("softcap", C.c_float)]
+
+
+class MaskedAttentionDesc(C.Structure):
+    """onhip_masked_attention_desc_t"""
+    _fields_ = [("batch", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("q_tokens", C.c_int32),
+                ("k_tokens", C.c_int32), ("head_dim", C.c_int32),
+                ("q_strides", C.c_longlong * 3), ("k_strides", C.c_longlong * 3), ("v_strides", C.c_longlong * 3),
+                ("out_strides", C.c_longlong * 3), ("scale", C.c_float), ("softcap", C.c_float),
+                ("causal", C.c_int32), ("window", C.c_int32), ("q_offset", C.c_int32), ("compute", C.c_int32)]
+
+
 def check_layout():
     assert C.sizeof(BUFFER_INFO_S) == 16
     assert C.sizeof(OPERAND_S) == 312 and OPERAND_S.shapes.offset == 276 and OPERAND_S.data_type.offset == 308

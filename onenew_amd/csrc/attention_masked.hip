@@ -1,0 +1,487 @@
+// Attention of prompts:  s_ij = cap tanh(scale q_i.k_j / cap) - slope |P_i - j|,  out_i = Softmax(s_i) v  over the keys that row i sees, in one
+// pass over the keys with the running maximum and sum of a softmax; P_i = i + q_offset is the query's place among the keys.
+//
+// What a row sees is an interval of keys, whatever the mask: causal (j <= P), a window (P - j < window) and the row's own pair
+// [begin, end) (documents of a packed batch, prefixes, lengths) are intersected once.  Tiles outside the union of a workgroup's intervals
+// are not touched, tiles inside the intersection of a wavefront's are computed without a mask.
+//
+// Rows: a workgroup has 128 rows of one key-value head, (token, head of the group) with the head running fastest, so that heads that share
+// keys share the tiles that are staged.  A wavefront has 32 of them and computes the transposed scores S^T = k q^T with
+// v_mfma_f32_32x32x16, so a lane owns one row and, per 32 keys, the 16 keys 8 (r / 4) + 4 (lane / 32) + r % 4; its softmax is the lane's own, and the
+// probabilities feed out^T = v^T P^T from the registers they are in.  Tiles of 64 keys of k and v go through LDS in two buffers, v
+// transposed on its way out by the transposing read.
+//
+// Rounded to the 16-bit type before the second product: 2^(s - m) times a constant, at most 2^8 of it (the reference point m follows the maximum when that is 2^8
+// above it, so that most tiles leave the sums alone).  Scores, maxima, sums and products' sums are fp32.
+#include "attention_join.hpp"
+
+namespace onhip {
+
+struct MaskedParams {
+    const unsigned short *q, *k, *v;
+    unsigned short *out;
+    long long qs[3], ks[3], vs[3], os[3];   // elements: (batch, head, token)
+    const int *ranges;
+    const float *slopes;
+    int batch, q_heads, kv_heads, group, q_tokens, k_tokens, q_offset, causal, window;
+    int blocks, splits;                     // row blocks of a key-value head; parts of the keys
+    int spread;                             // the (batch, key-value head) pairs divide evenly among the XCDs
+    float scale2, cap2, to_cap;             // |scale| * log2(e); cap * log2(e); scale / cap * 2 log2(e)
+    unsigned flip;                          // sign of the scale on q
+    float *part_o, *part_ml;
+};
+
+// halves of a packed pair that are +inf (0), -inf (1) or NaN (2), as 1.0 of the type; and the pair with all of those zeroed
+template <int DT> __device__ __forceinline__ unsigned special_of(unsigned w, int what) {
+    constexpr unsigned INF = DT == DT_BF16 ? 0x7f80u : 0x7c00u, ONE = DT == DT_BF16 ? 0x3f80u : 0x3c00u;
+    unsigned y = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned x = w >> (16 * h) & 0xffffu;
+        const bool is = what == 0 ? x == INF : what == 1 ? x == (INF | 0x8000u) : (x & 0x7fffu) > INF;
+        y |= (is ? ONE : 0u) << (16 * h);
+    }
+    return y;
+}
+template <int DT> __device__ __forceinline__ unsigned finite_of(unsigned w) {
+    constexpr unsigned INF = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+    return ((w & INF) == INF ? 0u : w & 0xffffu) | ((w >> 16 & INF) == INF ? 0u : w & 0xffff0000u);
+}
+
+// GENERAL: scores are capped or biased, or the scale is zero (else one fused product takes them into the exponential)
+template <int DT, int HD, bool GENERAL>
+__global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedParams p) {
+    constexpr int KT = 64, NT = KT / 32, STEPS = HD / 16, DTILES = HD / 32;
+    // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
+    constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
+    constexpr int UNITS = HD / 8, ROWS = 64 / UNITS;           // 16-byte units of a row; rows that a wavefront's load covers
+    constexpr int LOADS = KT / ROWS / 4;                       // loads of a wavefront for its share of a tile of k (or v)
+    __shared__ uint4 Ks[2][KT * UNITS];
+    __shared__ __attribute__((aligned(16))) unsigned short Vs[2][KT * HD];
+    __shared__ int s_lo[4], s_hi[4];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 31, lh = lane >> 5;
+    // item -> (batch, key-value head, row block, part).  Workgroups go to the XCDs in turn; where the heads divide among them, an XCD has whole
+    // heads, so that its L2 holds their keys.  The last row blocks, which see most keys under a causal mask, start first.
+    unsigned id = blockIdx.x;
+    int bh, block, split;
+    {
+        const unsigned pairs = (unsigned) (p.batch * p.kv_heads);
+        unsigned local = id, heads = pairs, first = 0;
+        if (p.spread) {
+            heads = pairs / 8u;
+            first = (id & 7u) * heads;
+            local = id >> 3;
+        }
+        split = (int) (local % (unsigned) p.splits);
+        local /= (unsigned) p.splits;
+        bh = (int) (first + local % heads);
+        block = p.blocks - 1 - (int) (local / heads);
+    }
+    const int b = bh / p.kv_heads, kvh = bh - b * p.kv_heads;
+
+    // this lane's row
+    const long long rows = (long long) p.q_tokens * p.group;
+    const long long r0 = (long long) block * 128 + wave * 32 + li;
+    const bool live = r0 < rows;
+    const int token = (int) ((live ? r0 : rows - 1) / p.group), head = kvh * p.group + (int) ((live ? r0 : rows - 1) - (long long) token * p.group);
+    const int place = token + p.q_offset;
+    int lo = 0, hi = p.k_tokens;
+    if (p.causal) hi = min(hi, place + 1);
+    if (p.window > 0) lo = max(lo, place - p.window + 1);
+    if (p.ranges) {
+        const int2 rg = reinterpret_cast<const int2 *>(p.ranges)[(long long) b * p.q_tokens + token];
+        lo = max(lo, rg.x);
+        hi = min(hi, rg.y);
+    }
+    if (lo >= hi) lo = hi = 0;   // sees nothing
+    // of the wavefront: the union and the intersection of its rows' intervals (a row past the last one repeats it)
+    int any_lo = lo < hi ? lo : 0x7fffffff, any_hi = hi, all_lo = lo, all_hi = hi;
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2) {
+        any_lo = min(any_lo, __shfl_xor(any_lo, x, 64));
+        any_hi = max(any_hi, __shfl_xor(any_hi, x, 64));
+        all_lo = max(all_lo, __shfl_xor(all_lo, x, 64));
+        all_hi = min(all_hi, __shfl_xor(all_hi, x, 64));
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    if (lane == 0) {
+        s_lo[wave] = any_lo;
+        s_hi[wave] = any_hi;
+    }
+    // q: the channels 16 s + 8 (lane / 32) .. + 7 of step s
+    uint4 qf[STEPS];
+    {
+        const unsigned short *src = p.q + b * p.qs[0] + head * p.qs[1] + token * p.qs[2] + lh * 8;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(src + st * 16);
+            qf[st] = make_uint4(x.x ^ p.flip, x.y ^ p.flip, x.z ^ p.flip, x.w ^ p.flip);
+        }
+    }
+    __syncthreads();
+    const int wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+    int t_begin = __builtin_amdgcn_readfirstlane(wg_lo / KT), t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
+    if (wg_hi <= 0) t_begin = t_end = 0;
+    if (p.splits > 1) {
+        const int per = (t_end - t_begin + p.splits - 1) / p.splits;
+        t_begin = min(t_end, t_begin + split * per);
+        t_end = min(t_end, t_begin + per);
+    }
+
+    // staging: load i of a wavefront takes the rows (wave LOADS + i) ROWS + lane / UNITS of a tile, 16 bytes a lane
+    const char *kb = reinterpret_cast<const char *>(p.k + b * p.ks[0] + kvh * p.ks[1]), *vb = reinterpret_cast<const char *>(p.v + b * p.vs[0] + kvh * p.vs[1]);
+    const unsigned k_step = (unsigned) p.ks[2] * 2u, v_step = (unsigned) p.vs[2] * 2u;
+    const int s_row = wave * LOADS * ROWS + lane / UNITS, s_unit = lane % UNITS;
+    u32x4 k_reg[LOADS], v_reg[LOADS];
+    auto fetch = [&](int t) __attribute__((always_inline)) {   // rows past the last key come as zeros
+        const int left = min(p.k_tokens - t * KT, KT);
+        const rsrc_t rk = make_rsrc(kb + (long long) t * KT * k_step, (unsigned) (left - 1) * k_step + HD * 2u);
+        const rsrc_t rv = make_rsrc(vb + (long long) t * KT * v_step, (unsigned) (left - 1) * v_step + HD * 2u);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const unsigned row = (unsigned) (s_row + i * ROWS);
+            k_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, row * k_step + s_unit * 16, 0, 0);
+            v_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, row * v_step + s_unit * 16, 0, 0);
+        }
+    };
+    // Where unit u of a row lies.  k: 16 lanes that take one unit of 16 rows meet every bank once.  v: the transposing read takes 64 bytes of four
+    // rows: those four segments are spread over the banks too.
+    auto k_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 15) : u ^ (row >> 1 & 7)); };
+    auto v_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 3) * 4 : u ^ (row >> 1 & 1) * 4); };
+    auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = s_row + i * ROWS;
+            Ks[buf][k_unit(row, s_unit)] = __builtin_bit_cast(uint4, k_reg[i]);
+            reinterpret_cast<uint4 *>(Vs[buf])[v_unit(row, s_unit)] = __builtin_bit_cast(uint4, v_reg[i]);
+        }
+    };
+    auto mfma = [](const uint4 &x, const uint4 &y, f32x16 c) __attribute__((always_inline)) {
+        if constexpr (DT == DT_BF16)
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+    };
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_t;
+    // of 16 lanes, four read the 32 bytes of 16 channels of one key, and each gets four keys of one channel
+    const int j16 = lane & 15;
+    int v_at[DTILES];   // shorts
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d) {
+        const int row = 4 * lh + j16 / 4;
+        v_at[d] = v_unit(row, 4 * d) * 8 + li / 16 * 16 + j16 % 4 * 4;
+    }
+    auto v_frag = [&](int buf, int t, int g, int d) __attribute__((always_inline)) {   // keys 32 t + 16 g + 4 lh + .. and 8 + .. of channel tile d
+        const unsigned short *at = Vs[buf] + v_at[d] + (32 * t + 16 * g) * HD;
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t) at));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t) (at + 8 * HD)));
+        return make_uint4(x.x, x.y, y.x, y.y);
+    };
+
+    f32x16 o[DTILES];
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const float slope2 = GENERAL && p.slopes ? p.slopes[head] * 1.44269504088896340736f : 0.0f;
+
+    auto tile = [&](int t, int buf) __attribute__((always_inline)) {
+        const int key0 = t * KT;
+        if (key0 >= any_hi || key0 + KT <= any_lo) return;   // uniform: none of the wavefront's rows sees the tile
+        const bool whole = key0 >= all_lo && key0 + KT <= all_hi;
+        f32x16 s[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) s[n] = mfma(Ks[buf][k_unit(32 * n + li, 2 * st + lh)], qf[st], s[n]);
+        }
+        if constexpr (GENERAL) {
+            if (p.cap2 > 0.0f) {   // uniform
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {   // tanh(x) = 1 - 2 / (e^2x + 1)
+                        const float e = __builtin_amdgcn_exp2f(s[n][r] * p.to_cap);
+                        s[n][r] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(e + 1.0f);
+                    }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] *= p.scale2;
+            }
+            if (p.slopes) {   // uniform
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        s[n][r] = __builtin_fmaf(-slope2, fabsf((float) (place - (key0 + 32 * n + 8 * (r / 4) + 4 * lh + r % 4))), s[n][r]);
+            }
+        }
+        if (!whole) {
+            const unsigned span = (unsigned) (hi - lo);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((unsigned) (key0 + 32 * n + 8 * (r / 4) + 4 * lh + r % 4 - lo) >= span) s[n][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if constexpr (!GENERAL) top *= p.scale2;
+        const bool far = top > m + 8.0f;   // each row by itself: its bits do not depend on the rows beside it
+        if (__any(far)) {
+            const float next = far ? top : m, fade = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+            m = next;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+        }
+        const float shift = m == -INFINITY ? 0.0f : SHIFT - m;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[n][r] = __builtin_amdgcn_exp2f(GENERAL ? s[n][r] + shift : __builtin_fmaf(s[n][r], p.scale2, shift));
+                l += s[n][r];
+            }
+        bool odd = false;   // a value among a masked tile's is no number: 0 of it, for the rows that do not see it, is not 0
+        if (!whole) {
+            f32x16 z;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) z = mfma(v_frag(buf, n, g, d), make_uint4(0u, 0u, 0u, 0u), z);
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += z[r];
+            odd = __any(sum != sum);
+        }
+        uint4 pf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                pf[n][g] = make_uint4(pack_h16<DT>(s[n][8 * g], s[n][8 * g + 1]), pack_h16<DT>(s[n][8 * g + 2], s[n][8 * g + 3]),
+                                      pack_h16<DT>(s[n][8 * g + 4], s[n][8 * g + 5]), pack_h16<DT>(s[n][8 * g + 6], s[n][8 * g + 7]));
+        if (!odd) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) o[d] = mfma(v_frag(buf, n, g, d), pf[n][g], o[d]);
+        } else {
+            // finite values as ever; then, for infinities of either sign and NaN, how many of them a row sees
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) {
+                        const uint4 x = v_frag(buf, n, g, d);
+                        o[d] = mfma(make_uint4(finite_of<DT>(x.x), finite_of<DT>(x.y), finite_of<DT>(x.z), finite_of<DT>(x.w)), pf[n][g], o[d]);
+                    }
+            constexpr unsigned ONE = DT == DT_BF16 ? 0x3f80u : 0x3c00u;
+            const unsigned span = (unsigned) (hi - lo);
+#pragma unroll 1
+            for (int what = 0; what < 3; ++what) {
+                const float value = what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN;
+#pragma unroll
+                for (int d = 0; d < DTILES; ++d) {
+                    f32x16 z;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll 1
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll 1
+                        for (int g = 0; g < 2; ++g) {
+                            unsigned seen[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int key = key0 + 32 * n + 16 * g + 8 * (j / 2) + 4 * lh + j % 2 * 2;
+                                seen[j] = ((unsigned) (key - lo) < span ? ONE : 0u) | ((unsigned) (key + 1 - lo) < span ? ONE << 16 : 0u);
+                            }
+                            const uint4 x = v_frag(buf, n, g, d);
+                            z = mfma(make_uint4(special_of<DT>(x.x, what), special_of<DT>(x.y, what), special_of<DT>(x.z, what), special_of<DT>(x.w, what)),
+                                     make_uint4(seen[0], seen[1], seen[2], seen[3]), z);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] += z[r] > 0.0f ? value : 0.0f;
+                }
+            }
+        }
+    };
+
+    if (t_begin < t_end) {
+        fetch(t_begin);
+        put(0);
+        if (t_begin + 1 < t_end) fetch(t_begin + 1);
+        for (int t = t_begin; t < t_end; ++t) {
+            const int buf = (t - t_begin) & 1;
+            __syncthreads();   // tile t is in LDS, tile t - 1 has been read
+            if (t + 1 < t_end) put(buf ^ 1);
+            if (t + 2 < t_end) fetch(t + 2);
+            tile(t, buf);
+        }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    if (!live) return;
+    if (p.splits > 1) {
+        const long long row = ((long long) b * p.q_heads + head) * p.q_tokens + token;
+        if (lh == 0) *reinterpret_cast<float2 *>(p.part_ml + (row * p.splits + split) * 2) = make_float2(m, l);
+        if (t_begin >= t_end) return;
+        float *po = p.part_o + (row * p.splits + split) * HD;
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4 *>(po + 32 * d + 8 * g + 4 * lh) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    unsigned short *dst = p.out + b * p.os[0] + head * p.os[1] + token * p.os[2];
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2 *>(dst + 32 * d + 8 * g + 4 * lh) =
+                make_uint2(pack_h16<DT>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), pack_h16<DT>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+}
+
+// Parts of the keys: where row blocks alone leave compute units without work, 512 keys a part at least.
+static int masked_splits(const onhip_masked_attention_desc_t *d, long long blocks) {
+    const long long all = blocks * d->batch * d->kv_heads;
+    const long long want = (512 + all - 1) / all;
+    long long keys = d->k_tokens;
+    if (d->window > 0 && d->window + 128LL < keys) keys = d->window + 128LL;
+    const long long most = (keys + 511) / 512;
+    const long long s = all >= 256 ? 1 : want < most ? want : most;
+    return s < 1 ? 1 : s > 256 ? 256 : (int) s;
+}
+
+static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *blocks, int *splits) {
+    constexpr int MOST = 1 << 29;
+    if (!d || d->batch < 1 || d->q_heads < 1 || d->kv_heads < 1 || d->q_tokens < 1 || d->k_tokens < 1) return set_error(ONHIP_ERR_ARG, "masked attention: bad shape");
+    if (d->compute == ONHIP_COMPUTE_BF16) *dt = DT_BF16;
+    else if (d->compute == ONHIP_COMPUTE_F16) *dt = DT_F16;
+    else return set_error(ONHIP_ERR_ARG, "masked attention: compute type %d is neither bf16 nor fp16", d->compute);
+    if (d->head_dim != 64 && d->head_dim != 128) return set_error(ONHIP_ERR_ARG, "masked attention: head dimension %d (64 and 128 are available)", d->head_dim);
+    if (d->q_heads % d->kv_heads) return set_error(ONHIP_ERR_ARG, "masked attention: %d query heads for %d key-value heads", d->q_heads, d->kv_heads);
+    if (d->k_tokens > MOST || d->q_tokens > MOST || d->q_offset > MOST || d->q_offset < -MOST) return set_error(ONHIP_ERR_ARG, "masked attention: lengths and places are at most 2^29");
+    if (d->window < 0 || d->window > MOST) return set_error(ONHIP_ERR_ARG, "masked attention: a window of %d", d->window);
+    if (!(d->softcap >= 0.0f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.0f)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be finite, the cap not negative");
+    const long long n = ((long long) d->q_tokens * (d->q_heads / d->kv_heads) + 127) / 128;
+    if (n * d->batch * d->kv_heads >= (1LL << 22) || (long long) d->batch * d->q_heads * d->q_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
+    *blocks = (int) n;
+    *splits = masked_splits(d, n);
+    return ONHIP_OK;
+}
+
+template <int DT, int HD>
+static int masked_launch(const MaskedParams &p, bool general, hipStream_t stream) {
+    const dim3 grid((unsigned) p.batch * p.kv_heads * p.blocks * p.splits);
+    if (general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false>), grid, dim3(256), 0, stream, p);
+    ONHIP_CHECK_HIP(hipGetLastError());
+    return ONHIP_OK;
+}
+
+}  // namespace onhip
+
+using namespace onhip;
+
+extern "C" {
+
+size_t onhip_attention_masked_workspace(const onhip_masked_attention_desc_t *d) {
+    int dt, blocks, splits;
+    if (masked_check(d, &dt, &blocks, &splits)) return 0;
+    return join_bytes((long long) d->batch * d->q_heads * d->q_tokens, splits, d->head_dim);
+}
+
+int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q, const void *k, const void *v, const int32_t *ranges,
+                           const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+    MaskedParams p;
+    int dt;
+    const int rc = masked_check(d, &dt, &p.blocks, &p.splits);
+    if (rc) return rc;
+    if (!q || !k || !v || !out) return set_error(ONHIP_ERR_ARG, "masked attention: null tensor pointer");
+    if (reinterpret_cast<uintptr_t>(ranges) % 8) return set_error(ONHIP_ERR_ARG, "masked attention: ranges must be 8-byte aligned");
+    const long long *strides[4] = {d->q_strides, d->k_strides, d->v_strides, d->out_strides};
+    const void *ptrs[4] = {q, k, v, out};
+    for (int t = 0; t < 4; ++t) {
+        if (reinterpret_cast<uintptr_t>(ptrs[t]) % 16) return set_error(ONHIP_ERR_ARG, "masked attention: tensors must be 16-byte aligned");
+        for (int i = 0; i < 3; ++i)
+            if (strides[t][i] < 0 || strides[t][i] % 8) return set_error(ONHIP_ERR_ARG, "masked attention: strides must be non-negative multiples of 8");
+    }
+    const int extent[3] = {d->batch, d->q_heads, d->q_tokens};
+    for (int i = 0; i < 3; ++i)
+        if (extent[i] > 1 && d->out_strides[i] < d->head_dim) return set_error(ONHIP_ERR_ARG, "masked attention: rows of the result overlap");
+    if (d->k_strides[2] >= (1LL << 23) || d->v_strides[2] >= (1LL << 23)) return set_error(ONHIP_ERR_ARG, "masked attention: token strides of k and v must be below 2^23");
+    const long long rows = (long long) d->batch * d->q_heads * d->q_tokens;
+    const size_t need = join_bytes(rows, p.splits, d->head_dim);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return set_error(ONHIP_ERR_WORKSPACE, "masked attention: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t) 0);
+    p.q = reinterpret_cast<const unsigned short *>(q);
+    p.k = reinterpret_cast<const unsigned short *>(k);
+    p.v = reinterpret_cast<const unsigned short *>(v);
+    p.out = reinterpret_cast<unsigned short *>(out);
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = d->q_strides[i]; p.ks[i] = d->k_strides[i]; p.vs[i] = d->v_strides[i]; p.os[i] = d->out_strides[i];
+    }
+    p.ranges = ranges;
+    p.slopes = slopes;
+    p.batch = d->batch;
+    p.q_heads = d->q_heads;
+    p.kv_heads = d->kv_heads;
+    p.group = d->q_heads / d->kv_heads;
+    p.q_tokens = d->q_tokens;
+    p.k_tokens = d->k_tokens;
+    p.q_offset = d->q_offset;
+    p.causal = d->causal;
+    p.window = d->window;
+    p.spread = (long long) d->batch * d->kv_heads % 8 == 0;
+    p.flip = d->scale < 0.0f ? 0x80008000u : 0u;
+    p.scale2 = fabsf(d->scale) * 1.44269504088896340736f;
+    p.cap2 = d->softcap * 1.44269504088896340736f;
+    p.to_cap = d->softcap > 0.0f ? fabsf(d->scale) / d->softcap * 2.0f * 1.44269504088896340736f : 0.0f;
+    p.part_o = reinterpret_cast<float *>(workspace);
+    p.part_ml = p.part_o + rows * p.splits * d->head_dim;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const bool general = d->softcap > 0.0f || slopes || p.scale2 == 0.0f;
+    auto by_size = [&]<int DT>() { return d->head_dim == 64 ? masked_launch<DT, 64>(p, general, st) : masked_launch<DT, 128>(p, general, st); };
+    const int done = dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
+    if (done || p.splits == 1) return done;
+    JoinParams j;
+    j.o = p.part_o;
+    j.ml = p.part_ml;
+    j.out = p.out;
+    for (int i = 0; i < 3; ++i) j.os[i] = p.os[i];
+    j.heads = p.q_heads;
+    j.tokens = p.q_tokens;
+    j.splits = p.splits;
+    j.rows = rows;
+    return attention_join_launch(dt, d->head_dim, j, st);
+}
+
+}  // extern "C"

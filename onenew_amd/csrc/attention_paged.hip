@@ -1,0 +1,471 @@
+// Attention of one new token a sequence over a paged key-value cache:  s_j = cap tanh(scale q.k_j / cap) - slope (len - 1 - j),  out = Softmax(s) v
+// over the keys j of [max(0, len - window), len), in one pass over the cache with the running maximum and sum of a softmax.
+//
+// Up to 16 query heads that share a key-value head are the columns of the matrix instructions (v_mfma_f32_16x16x32), so the cache is read
+// once for all of them.  A wavefront takes tiles of 32 keys by itself, with no barrier until its end: S^T = K q^T, whose result leaves a
+// lane with 8 scores of one head; and out^T = V^T P^T, whose second operand is those scores' exponentials where they are.  Both operands of
+// the cache come straight from memory into registers.  K: a lane reads 16 bytes of the row of its key.  V: 16 lanes read a whole row, a
+// lane the channels 8 li .. + 7 (HD 128) of 8 keys, and channel 8 li + t of them is its operand for channel tile t, put together from the
+// halves (or bytes) of those registers, so nothing passes through LDS before the end.
+//
+// The rows are bound by memory: a byte of the cache takes part in 2 to 16 operations.  A sequence's tiles are shared out among
+// `splits` workgroups of four wavefronts, whose parts a second launch joins, where (sequence, head) pairs alone would leave compute units idle.
+//
+// int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
+// probability.  What is rounded to the 16-bit type before the second product is exp(s - max) (times a constant, and the scale), half a step each; scores, maximum,
+// sum and products' sums are fp32.
+#include "attention_join.hpp"
+#include "kv_common.hpp"
+
+namespace onhip {
+
+struct PagedParams {
+    CacheView c;
+    const unsigned short *q;
+    unsigned short *out;
+    long long qs[2], os[2];      // elements: (sequence, head)
+    const int *table, *lengths;
+    const float *slopes;
+    long long table_stride;
+    int table_pages, batch, q_heads, kv_heads, group, head_blocks, splits, window;
+    float scale2, cap2, to_cap;  // scale * log2(e); cap * log2(e); scale / cap * 2 log2(e)
+    float *part_o, *part_ml;
+};
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// cap tanh(s scale / cap) log2(e): tanh(x) = 1 - 2 / (e^2x + 1), which is off by 2^-23 of the cap at most, a hundred-thousandth of a score of 50
+__device__ __forceinline__ float capped(float s, float to_cap, float cap2) {
+    const float e = __builtin_amdgcn_exp2f(s * to_cap);
+    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+
+// SMALL: pages of fewer than 16 tokens (a tile then has a page a lane; else two pages, the same for all lanes)
+template <int DT, int HD, bool I8, bool SMALL>
+__global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel(const PagedParams p) {
+    constexpr int TILES = HD / 16, STEPS = HD / 32, NW = 4;
+    constexpr int KW = I8 ? HD / 64 : HD / 32;       // 16-byte loads of a lane's part of a key
+    constexpr int VB = (I8 ? 1 : 2) * HD / 16;        // bytes of a lane's part of a value: 4, 8 or 16
+    constexpr int VW = VB / 4;
+    // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
+    constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 15.0f;
+    __shared__ float s_o[NW][16][HD + 4];
+    __shared__ float s_m[NW][16], s_l[NW][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    unsigned id = blockIdx.x;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int hb = id % p.head_blocks;
+    id /= p.head_blocks;
+    const int kvh = id % p.kv_heads, b = id / p.kv_heads;
+
+    const int reach = p.lengths[b];
+    const long long room = (long long) p.table_pages << p.c.page_shift;
+    const bool too_long = reach > room;   // more tokens than the table has pages for: the result is NaN
+    const int len = too_long ? (int) room : reach;
+    const int begin = p.window > 0 && len > p.window ? len - p.window : 0;
+    const int tile0 = begin >> 5, tiles = len > 0 ? ((len + 31) >> 5) - tile0 : 0;
+    // as many parts as there are, each of 128 keys at least
+    const int parts = min(p.splits, (tiles + 3) / 4), per = parts > 0 ? (tiles + parts - 1) / parts : 0;
+    const int t_begin = tile0 + split * per, t_end = min(t_begin + per, tile0 + tiles);
+
+    const int head = hb * 16 + li;
+    const bool live = head < p.group;
+    const int qh = kvh * p.group + head;
+    uint4 qf[STEPS];
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+        qf[st] = make_uint4(0u, 0u, 0u, 0u);
+        // the channels that this lane's part of a key has in step st
+        const int d = I8 ? st / 2 * 64 + lg * 16 + st % 2 * 8 : st * 32 + lg * 8;
+        if (live) qf[st] = *reinterpret_cast<const uint4 *>(p.q + b * p.qs[0] + qh * p.qs[1] + d);
+    }
+    const float slope2 = p.slopes && live ? p.slopes[qh] * LOG2E : 0.0f;
+
+    auto mfma = [](const uint4 &x, const uint4 &y, f32x4 c) __attribute__((always_inline)) {
+        if constexpr (DT == DT_BF16)
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+    };
+
+    f32x4 o[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    int unit = -1000;   // int8 and fp16: o is in units of 2^unit
+    bool bad = false;
+    const int *table = p.table + b * p.table_stride;
+    const char *kb = p.c.k + kvh * p.c.ks[1], *vb = p.c.v + kvh * p.c.vs[1];
+
+    for (int t = t_begin + wave; t < t_end; t += NW) {
+        const int key0 = t * 32;
+        const bool whole = key0 >= begin && key0 + 32 <= len;   // uniform
+        // the pages of the tile's two halves, or of key `lane`
+        int pg[2];
+        if constexpr (SMALL) {
+            const int key = key0 + (lane & 31);
+            int x = key >= begin && key < len ? table[key >> p.c.page_shift] : 0;
+            if ((unsigned) x >= (unsigned) p.c.pages) { bad = true; x = 0; }
+            pg[0] = x;
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int key = key0 + 16 * a;
+                int x = key + 16 > begin && key < len ? table[key >> p.c.page_shift] : 0;
+                if ((unsigned) x >= (unsigned) p.c.pages) { bad = true; x = 0; }
+                pg[a] = __builtin_amdgcn_readfirstlane(x);
+            }
+        }
+        auto page_of = [&](int in_tile) __attribute__((always_inline)) {   // of key key0 + in_tile
+            if constexpr (SMALL) return __shfl(pg[0], in_tile, 64);
+            else return in_tile < 16 ? pg[0] : pg[1];
+        };
+        // what lies outside [begin, len) is read as well, from rows of pages that exist, and left out below
+        uint4 kf[2][KW];
+        unsigned vf[8][VW];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const int key = key0 + 16 * a + li;
+            const char *src = kb + (long long) (SMALL ? page_of(16 * a + li) : pg[a]) * p.c.ks[0] + ((key & p.c.page_mask) * (int) p.c.ks[2] + lg * 16);
+#pragma unroll
+            for (int i = 0; i < KW; ++i) kf[a][i] = *reinterpret_cast<const uint4 *>(src + i * 64);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = 16 * (j / 4) + 4 * lg + j % 4, key = key0 + at;
+            const char *src = vb + (long long) (SMALL ? page_of(at) : pg[j / 4]) * p.c.vs[0] + ((key & p.c.page_mask) * (int) p.c.vs[2] + li * VB);
+            if constexpr (VB == 16) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                vf[j][0] = x.x; vf[j][1] = x.y; vf[j][2] = x.z; vf[j][3] = x.w;
+            } else if constexpr (VB == 8) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                vf[j][0] = x.x; vf[j][1] = x.y;
+            } else {
+                vf[j][0] = *reinterpret_cast<const unsigned *>(src);
+            }
+        }
+        float ksc[8], vsc[8];
+        if constexpr (I8) {   // lanes 0 to 31 fetch the scales of the keys, 32 to 63 those of the values
+            const int at = lane & 31, key = key0 + at;
+            const float *from = lane < 32 ? p.c.k_scale : p.c.v_scale;
+            float x = 0.0f;
+            const int page = SMALL ? pg[0] : at < 16 ? pg[0] : pg[1];
+            x = from[page * p.c.ss[0] + kvh * p.c.ss[1] + (key & p.c.page_mask) * p.c.ss[2]];
+            if (key < begin || key >= len) x = 0.0f;
+            if constexpr (DT == DT_F16) {   // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
+                float y = lane < 32 ? 0.0f : x;
+#pragma unroll
+                for (int i = 1; i < 64; i *= 2) y = fmaxf(y, __shfl_xor(y, i, 64));
+                const int e = y > 0.0f && y < INFINITY ? __builtin_amdgcn_frexp_expf(y) : -1000;
+                if (e > unit) {   // uniform
+#pragma unroll
+                    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit - e);
+                    unit = e;
+                }
+                x = lane < 32 ? x : ldexpf(x, -unit);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int from_lane = 16 * (j / 4) + 4 * lg + j % 4;
+                ksc[j] = __shfl(x, from_lane, 64);
+                vsc[j] = __shfl(x, 32 + from_lane, 64);
+            }
+        }
+
+        if (!whole) {   // a value that is not seen may be an infinity, and 0 of it is not 0
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = key0 + 16 * (j / 4) + 4 * lg + j % 4;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) vf[j][i] = key >= begin && key < len ? vf[j][i] : 0u;
+            }
+        }
+
+        // S^T: this lane's 8 scores are of head li and the keys 16 (j / 4) + 4 lg + j % 4
+        float s[8];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (I8) {
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) {
+                    const uint4 &x = kf[a][st / 2];
+                    const unsigned two[2] = {st % 2 ? x.z : x.x, st % 2 ? x.w : x.y};
+                    unsigned y[4];
+                    s8_to_h16<DT, 2>(two, y);
+                    acc = mfma(make_uint4(y[0], y[1], y[2], y[3]), qf[st], acc);
+                }
+            } else {
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) acc = mfma(kf[a][st], qf[st], acc);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * a + r] = I8 ? acc[r] * ksc[4 * a + r] : acc[r];
+        }
+        if (p.cap2 > 0.0f) {   // uniform
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] = capped(s[j], p.to_cap, p.cap2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] *= p.scale2;
+        }
+        if (p.slopes) {   // uniform
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] = __builtin_fmaf(slope2, (float) (key0 + 16 * (j / 4) + 4 * lg + j % 4 - (len - 1)), s[j]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = key0 + 16 * (j / 4) + 4 * lg + j % 4;
+                if (key < begin || key >= len) s[j] = -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float next = fmaxf(m, top), shift = next == -INFINITY ? 0.0f : next;
+        const float fade = __builtin_amdgcn_exp2f(m - shift);
+        m = next;
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(s[j] - shift + SHIFT);
+        l *= fade;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l += e[j];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][r] *= fade;
+        if constexpr (I8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] *= vsc[j];
+        const uint4 pf = make_uint4(pack_h16<DT>(e[0], e[1]), pack_h16<DT>(e[2], e[3]), pack_h16<DT>(e[4], e[5]), pack_h16<DT>(e[6], e[7]));
+        // out^T += V^T P^T: row i of channel tile n is the channel TILES i + n
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            unsigned a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (I8) {
+                    const int x = (int) (vf[2 * j][n / 4] >> (n % 4 * 8)), y = (int) (vf[2 * j + 1][n / 4] >> (n % 4 * 8));
+                    a[j] = pack_h16<DT>((float) (signed char) x, (float) (signed char) y);
+                } else {
+                    a[j] = __builtin_amdgcn_perm(vf[2 * j + 1][n / 2], vf[2 * j][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
+                }
+            }
+            o[n] = mfma(make_uint4(a[0], a[1], a[2], a[3]), pf, o[n]);
+        }
+    }
+
+    if constexpr (I8 && DT == DT_F16)
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit);
+    // the four wavefronts' parts
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (__any(bad) || too_long) l = NAN;
+    if (lg == 0) {
+        s_m[wave][li] = m;
+        s_l[wave][li] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < TILES; n += 4)
+            *reinterpret_cast<float4 *>(&s_o[wave][li][(4 * lg + r) * TILES + n]) = make_float4(o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]);
+    __syncthreads();
+    constexpr int PER = HD / 16;   // channels of a thread: 16 threads a head
+    const int oh = threadIdx.x / 16, d0 = threadIdx.x % 16 * PER;
+    if (hb * 16 + oh >= p.group) return;
+    float mm = s_m[0][oh];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, s_m[w][oh]);
+    const float shift = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(s_m[w][oh] - shift);
+        ll += s_l[w][oh] * f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = __builtin_fmaf(s_o[w][oh][d0 + i], f, acc[i]);
+        if (s_l[w][oh] != s_l[w][oh]) ll = NAN;   // a page that does not exist
+    }
+    const int row = b * p.q_heads + kvh * p.group + hb * 16 + oh;
+    if (p.splits > 1) {
+        float *po = p.part_o + ((long long) row * p.splits + split) * HD + d0;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4 *>(po + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        if (d0 == 0) *reinterpret_cast<float2 *>(p.part_ml + ((long long) row * p.splits + split) * 2) = make_float2(mm, ll);
+        return;
+    }
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    unsigned short *dst = p.out + b * p.os[0] + (kvh * p.group + hb * 16 + oh) * p.os[1] + d0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2)
+        reinterpret_cast<unsigned *>(dst)[i / 2] = pack_h16<DT>(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// ---- the parts of a row joined: four wavefronts a row, a lane HD / 64 channels -------------------------------------------------
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void attention_join_kernel(const JoinParams p) {
+    constexpr int PER = HD / 64, NW = 4;
+    __shared__ float s_acc[NW][HD], s_l[NW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long row = blockIdx.x;
+    const float *ml = p.ml + row * p.splits * 2, *o = p.o + row * p.splits * HD;
+    float mm = -INFINITY;
+    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[2 * s]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
+    const float shift = mm == -INFINITY ? 0.0f : mm;
+    float acc[PER], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+    for (int s = wave; s < p.splits; s += NW) {
+        const float ls = ml[2 * s + 1], f = __builtin_amdgcn_exp2f(ml[2 * s] - shift);
+        if (ls == 0.0f && f == 0.0f) continue;   // a part without keys (uniform in the wavefront); a NaN stays
+        l = __builtin_fmaf(ls, f, l);
+        if (ls != ls) l = NAN;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = __builtin_fmaf(o[(long long) s * HD + lane * PER + i], f, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s_acc[wave][lane * PER + i] = acc[i];
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    if (threadIdx.x >= HD / 2) return;
+    l = 0.0f;
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        l += s_l[w];
+        x += s_acc[w][2 * threadIdx.x];
+        y += s_acc[w][2 * threadIdx.x + 1];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const long long token = row % p.tokens, bh = row / p.tokens, h = bh % p.heads, b = bh / p.heads;
+    reinterpret_cast<unsigned *>(p.out + b * p.os[0] + h * p.os[1] + token * p.os[2])[threadIdx.x] = pack_h16<DT>(x * inv, y * inv);
+}
+
+int attention_join_launch(int dt, int hd, const JoinParams &p, hipStream_t stream) {
+    const dim3 grid((unsigned) p.rows);
+    if (dt == DT_BF16 && hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 64>), grid, dim3(256), 0, stream, p);
+    else if (dt == DT_BF16) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 128>), grid, dim3(256), 0, stream, p);
+    else if (hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_F16, 64>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attention_join_kernel<DT_F16, 128>), grid, dim3(256), 0, stream, p);
+    ONHIP_CHECK_HIP(hipGetLastError());
+    return ONHIP_OK;
+}
+
+// Workgroups that a sequence's head is cut into: enough for four a compute unit, 256 keys of the longest possible sequence each at least.
+static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d) {
+    const long long group = d->q_heads / c->kv_heads, rows = (long long) d->batch * c->kv_heads * ((group + 15) / 16);
+    long long longest = (long long) d->table_pages * c->page_tokens;
+    if (d->window > 0 && d->window < longest) longest = d->window;
+    const long long want = (1024 + rows - 1) / rows, most = (longest + 255) / 256;
+    const long long s = want < most ? want : most;
+    return s < 1 ? 1 : s > 256 ? 256 : (int) s;
+}
+
+static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, CacheView *view, int *dt) {
+    const int rc = cache_view("paged attention", c, view, dt);
+    if (rc) return rc;
+    if (!d || d->batch < 1 || d->q_heads < 1 || d->table_pages < 1 || d->table_stride < 0) return set_error(ONHIP_ERR_ARG, "paged attention: bad shape");
+    if (d->q_heads % c->kv_heads) return set_error(ONHIP_ERR_ARG, "paged attention: %d query heads for %d key-value heads", d->q_heads, c->kv_heads);
+    if ((long long) d->batch * d->q_heads >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "paged attention: %d sequences of %d heads", d->batch, d->q_heads);
+    if ((long long) d->table_pages * c->page_tokens > (1LL << 30)) return set_error(ONHIP_ERR_ARG, "paged attention: a table of %d pages", d->table_pages);
+    if (d->window < 0) return set_error(ONHIP_ERR_ARG, "paged attention: a window of %d", d->window);
+    if (!(d->softcap >= 0.0f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.0f)) return set_error(ONHIP_ERR_ARG, "paged attention: scale and cap must be finite, the cap not negative");
+    return ONHIP_OK;
+}
+
+template <int DT, int HD, bool I8>
+static int paged_launch(const PagedParams &p, unsigned blocks, hipStream_t stream) {
+    if (p.c.page_shift < 4) hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, false>), dim3(blocks), dim3(256), 0, stream, p);
+    ONHIP_CHECK_HIP(hipGetLastError());
+    return ONHIP_OK;
+}
+
+}  // namespace onhip
+
+using namespace onhip;
+
+extern "C" {
+
+size_t onhip_attention_paged_workspace(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d) {
+    CacheView view;
+    int dt;
+    if (paged_check(c, d, &view, &dt)) return 0;
+    return join_bytes((long long) d->batch * d->q_heads, paged_splits(c, d), c->head_dim);
+}
+
+int onhip_attention_paged(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table,
+                          const int32_t *lengths, const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+    PagedParams p;
+    int dt;
+    const int rc = paged_check(c, d, &p.c, &dt);
+    if (rc) return rc;
+    if (!q || !out || !table || !lengths) return set_error(ONHIP_ERR_ARG, "paged attention: null pointer");
+    if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16) return set_error(ONHIP_ERR_ARG, "paged attention: tensors must be 16-byte aligned");
+    for (int i = 0; i < 2; ++i) {
+        if (d->q_strides[i] < 0 || d->q_strides[i] % 8 || d->out_strides[i] < 0 || d->out_strides[i] % 8)
+            return set_error(ONHIP_ERR_ARG, "paged attention: strides must be non-negative multiples of 8");
+        if ((i == 0 ? d->batch : d->q_heads) > 1 && d->out_strides[i] < c->head_dim) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
+        p.qs[i] = d->q_strides[i];
+        p.os[i] = d->out_strides[i];
+    }
+    const long long rows = (long long) d->batch * d->q_heads;
+    p.splits = paged_splits(c, d);
+    const size_t need = join_bytes(rows, p.splits, c->head_dim);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return set_error(ONHIP_ERR_WORKSPACE, "paged attention: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t) 0);
+    p.q = reinterpret_cast<const unsigned short *>(q);
+    p.out = reinterpret_cast<unsigned short *>(out);
+    p.table = table;
+    p.lengths = lengths;
+    p.slopes = slopes;
+    p.table_stride = d->table_stride;
+    p.table_pages = d->table_pages;
+    p.batch = d->batch;
+    p.q_heads = d->q_heads;
+    p.kv_heads = c->kv_heads;
+    p.group = d->q_heads / c->kv_heads;
+    p.head_blocks = (p.group + 15) / 16;
+    p.window = d->window;
+    p.scale2 = d->scale * LOG2E;
+    p.cap2 = d->softcap * LOG2E;
+    p.to_cap = d->softcap > 0.0f ? d->scale / d->softcap * 2.0f * LOG2E : 0.0f;
+    p.part_o = reinterpret_cast<float *>(workspace);
+    p.part_ml = p.part_o + rows * p.splits * c->head_dim;
+    const unsigned blocks = (unsigned) (d->batch * c->kv_heads * p.head_blocks * p.splits);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    auto by_size = [&]<int DT>() {
+        if (c->head_dim == 64) return c->quantised ? paged_launch<DT, 64, true>(p, blocks, st) : paged_launch<DT, 64, false>(p, blocks, st);
+        return c->quantised ? paged_launch<DT, 128, true>(p, blocks, st) : paged_launch<DT, 128, false>(p, blocks, st);
+    };
+    const int done = dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
+    if (done || p.splits == 1) return done;
+    JoinParams j;
+    j.o = p.part_o;
+    j.ml = p.part_ml;
+    j.out = p.out;
+    j.os[0] = p.os[0]; j.os[1] = p.os[1]; j.os[2] = 0;
+    j.heads = p.q_heads;
+    j.tokens = 1;
+    j.splits = p.splits;
+    j.rows = rows;
+    return attention_join_launch(dt, c->head_dim, j, st);
+}
+
+}  // extern "C"

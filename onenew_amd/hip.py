@@ -39,7 +39,8 @@ EXPORTS = ["onhip_init", "onhip_last_error", "onhip_set_tuning", "onhip_split_ta
            "onhip_matmul", "onhip_matmul_add", "onhip_gemm_f32", "onhip_copy_f32",
            "onhip_h16_pitch", "onhip_h16_packed_weight_bytes", "onhip_h16_pack_conv_weights", "onhip_h16_pack_matmul_weights",
            "onhip_h16_from_nchw_f32", "onhip_h16_to_nchw_f32", "onhip_h16_from_rows_f32", "onhip_h16_to_rows_f32",
-           "onhip_conv2d_h16", "onhip_h16_first_width", "onhip_h16_first_channels", "onhip_h16_first_input_bytes", "onhip_h16_first_weight_bytes", "onhip_h16_first_from_nchw_f32", "onhip_h16_first_pack_weights", "onhip_conv2d_h16_first", "onhip_linear_h16", "onhip_attention", 
+           "onhip_conv2d_h16", "onhip_h16_first_width", "onhip_h16_first_channels", "onhip_h16_first_input_bytes", "onhip_h16_first_weight_bytes", "onhip_h16_first_from_nchw_f32", "onhip_h16_first_pack_weights", "onhip_conv2d_h16_first", "onhip_linear_h16", "onhip_attention",
+           "onhip_cache_append", "onhip_cache_read", "onhip_attention_paged_workspace", "onhip_attention_paged", "onhip_attention_masked_workspace", "onhip_attention_masked",
            "onhip_ir_block_supported", "onhip_ir_block_packed_weight_bytes", "onhip_ir_block_pack_weights", "onhip_ir_block_f32",
            "onhip_conv2d_pw_supported", "onhip_conv2d_pw_packed_weight_bytes", "onhip_conv2d_pw_pack_weights", "onhip_conv2d_pw_f32",
            "onhip_add_f32", "onhip_relu_f32", "onhip_maxpool_out_shape", "onhip_maxpool_f32", "onhip_maxpool_s8_nhwc", "onhip_maxpool_s8_eval", "onhip_global_avgpool_f32",
@@ -127,6 +128,15 @@ def load():
     L.onhip_h16_first_pack_weights.argtypes = [C.POINTER(ConvDesc), vp, vp, vp]
     L.onhip_conv2d_h16_first.argtypes = [C.POINTER(ConvDesc), vp, vp, vp, vp, vp, i32, vp]
     L.onhip_attention.argtypes = [C.POINTER(abi.AttentionDesc), vp, vp, vp, vp, vp]
+    cache = C.POINTER(abi.CacheDesc)
+    L.onhip_cache_append.argtypes = [cache, C.POINTER(abi.CacheRowsDesc)] + [vp] * 10
+    L.onhip_cache_read.argtypes = [cache, vp, C.c_longlong, i32, vp, i32, i32, vp, C.POINTER(C.c_longlong), vp, C.POINTER(C.c_longlong), vp]
+    L.onhip_attention_paged_workspace.argtypes = [cache, C.POINTER(abi.PagedAttentionDesc)]
+    L.onhip_attention_paged_workspace.restype = C.c_size_t
+    L.onhip_attention_paged.argtypes = [cache, C.POINTER(abi.PagedAttentionDesc)] + [vp] * 6 + [C.c_size_t, vp]
+    L.onhip_attention_masked_workspace.argtypes = [C.POINTER(abi.MaskedAttentionDesc)]
+    L.onhip_attention_masked_workspace.restype = C.c_size_t
+    L.onhip_attention_masked.argtypes = [C.POINTER(abi.MaskedAttentionDesc)] + [vp] * 7 + [C.c_size_t, vp]
     L.onhip_ir_block_supported.argtypes = [C.POINTER(ConvDesc)] * 3
     L.onhip_ir_block_packed_weight_bytes.argtypes = [i32, i32, i32]
     L.onhip_ir_block_packed_weight_bytes.restype = C.c_size_t
@@ -688,6 +698,204 @@ def attention(q, k, v, scale=1.0, out=None, merged_out=True):
     else:
         d.out_strides = (C.c_longlong * 3)(h * t * hd, t * hd, hd)
     _check(load().onhip_attention(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _stream()), "onhip_attention")
+    return out
+
+
+# ---- a paged key-value cache and the attention around it: bf16 / fp16 tensors, int8 caches with fp32 scales ----
+
+def _here(what, dtype, shape=None, **tensors):
+    """checks what the C entry points cannot see: the type, the device and (given one) the shape of tensors, None left out"""
+    import torch
+    device = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise OnhipError(f"{what}: {name} is {t.dtype}, not {dtype}")
+        if t.device.type != "cuda" or t.device.index != device:
+            raise OnhipError(f"{what}: {name} is on {t.device}, the current device is cuda:{device}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise OnhipError(f"{what}: {name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
+
+
+def _h16_compute(what, dtype):
+    import torch
+    if dtype == torch.bfloat16:
+        return abi.COMPUTE_BF16
+    if dtype == torch.float16:
+        return abi.COMPUTE_F16
+    raise OnhipError(f"{what}: {dtype} is neither bfloat16 nor float16")
+
+
+def _flat(what, **tensors):
+    for name, t in tensors.items():
+        if t is not None and not t.is_contiguous():
+            raise OnhipError(f"{what}: {name} must be contiguous")
+
+
+def _last(what, **tensors):
+    for name, t in tensors.items():
+        if t.stride(-1) != 1:
+            raise OnhipError(f"{what}: the head dimension of {name} must be contiguous")
+
+
+def _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype):
+    """k_cache, v_cache [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with scales [pages, kv_heads, page_tokens]"""
+    import torch
+    quantised = k_cache.dtype == torch.int8
+    compute = _h16_compute(what, dtype)
+    if k_cache.dim() != 4:
+        raise OnhipError(f"{what}: a cache is [pages, kv_heads, page_tokens, head_dim]")
+    _here(what, torch.int8 if quantised else dtype, k_cache.shape, k_cache=k_cache, v_cache=v_cache)
+    _last(what, k_cache=k_cache, v_cache=v_cache)
+    d = abi.CacheDesc(*k_cache.shape[:1], k_cache.shape[2], k_cache.shape[1], k_cache.shape[3], compute, int(quantised))
+    d.k_strides[:], d.v_strides[:] = k_cache.stride()[:3], v_cache.stride()[:3]
+    d.k, d.v = k_cache.data_ptr(), v_cache.data_ptr()
+    if (k_scale is None) != (not quantised) or (v_scale is None) != (not quantised):
+        raise OnhipError(f"{what}: scales go with an int8 cache, and an int8 cache with scales")
+    if quantised:
+        _here(what, torch.float32, k_cache.shape[:3], k_scale=k_scale, v_scale=v_scale)
+        if k_scale.stride() != v_scale.stride():
+            raise OnhipError(f"{what}: k_scale and v_scale must have the same strides")
+        d.scale_strides[:] = k_scale.stride()
+        d.k_scale, d.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    return d
+
+
+def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                 k_scale=None, v_scale=None, q_out=None):
+    """q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim] (any token and head strides, e.g. slices of one projection's rows):
+    norm of q's and k's heads where there are weights [head_dim] (fp32), rotation by positions [tokens] (int32) times inv_freq [pairs] (fp32)
+    where there are frequencies, q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
+    [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with fp32 scales [pages, kv_heads, page_tokens]"""
+    import torch
+    what = "cache_append"
+    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
+    tokens, q_heads, hd = q.shape
+    if hd != d.head_dim:
+        raise OnhipError(f"{what}: heads of {hd} channels for a cache of {d.head_dim}")
+    _here(what, q.dtype, None, q=q)
+    _here(what, q.dtype, (tokens, d.kv_heads, hd), k=k, v=v)
+    if q_out is None:
+        q_out = torch.empty((tokens, q_heads, hd), dtype=q.dtype, device=q.device)
+    else:
+        _here(what, q.dtype, q.shape, q_out=q_out)
+    _last(what, q=q, k=k, v=v, q_out=q_out)
+    _here(what, torch.int32, (tokens,), positions=positions, slots=slots)
+    _here(what, torch.float32, (hd,), q_weight=q_weight, k_weight=k_weight)
+    _here(what, torch.float32, None, inv_freq=inv_freq)
+    _flat(what, positions=positions, slots=slots, q_weight=q_weight, k_weight=k_weight, inv_freq=inv_freq)
+    if tokens == 0:
+        return q_out
+    r = abi.CacheRowsDesc(tokens=tokens, q_heads=q_heads, pairs=0 if inv_freq is None else inv_freq.numel(), interleaved=int(interleaved), eps=eps)
+    for name, t in (("q_strides", q), ("k_strides", k), ("v_strides", v), ("out_strides", q_out)):
+        getattr(r, name)[:] = t.stride()[:2]
+    _check(load().onhip_cache_append(C.byref(d), C.byref(r), _ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(slots), _ptr(inv_freq), _ptr(q_weight),
+                                     _ptr(k_weight), _ptr(q_out), _stream()), "onhip_cache_append")
+    return q_out
+
+
+def _table(what, table, lengths, batch):
+    import torch
+    _here(what, torch.int32, None, table=table)
+    _here(what, torch.int32, (batch,), lengths=lengths)
+    _flat(what, lengths=lengths)
+    if table.dim() != 2 or table.shape[0] != batch or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise OnhipError(f"{what}: the table is [sequences, pages] with contiguous rows")
+
+
+def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
+    """rows 0 .. tokens - 1 of every sequence (pages table [sequences, pages], lengths [sequences], int32), zeros behind its length: k and v
+    [sequences, kv_heads, tokens, head_dim] in the cache's 16-bit type, or `dtype` for an int8 cache"""
+    import torch
+    what = "cache_read"
+    dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
+    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype)
+    batch = table.shape[0]
+    _table(what, table, lengths, batch)
+    shape = (batch, d.kv_heads, tokens, d.head_dim)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+    _here(what, dtype, shape, k_out=k_out, v_out=v_out)
+    _last(what, k_out=k_out, v_out=v_out)
+    if batch == 0 or tokens == 0:
+        return k_out, v_out
+    three = C.c_longlong * 3
+    _check(load().onhip_cache_read(C.byref(d), _ptr(table), table.stride(0), table.shape[1], _ptr(lengths), batch, tokens, _ptr(k_out), three(*k_out.stride()[:3]),
+                                   _ptr(v_out), three(*v_out.stride()[:3]), _stream()), "onhip_cache_read")
+    return k_out, v_out
+
+
+def _workspace(nbytes, device):
+    """of this call alone, from torch's allocator: ordered on the stream, private to a graph that is being captured"""
+    import torch
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, softcap=0.0, slopes=None, k_scale=None, v_scale=None, out=None):
+    """attention of one new token a sequence, q [sequences, q_heads, head_dim], over the cache's rows table [sequences, pages] / lengths
+    [sequences] (int32; the new token's row is the last): scores capped to softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the
+    distance, the last `window` rows alone where it is above zero; returns [sequences, q_heads, head_dim]"""
+    import torch
+    what = "attention_paged"
+    c = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
+    batch, q_heads, hd = q.shape
+    _here(what, q.dtype, (batch, q_heads, c.head_dim), q=q)
+    _table(what, table, lengths, batch)
+    _here(what, torch.float32, (q_heads,), slopes=slopes)
+    _flat(what, slopes=slopes)
+    if out is None:
+        out = torch.empty((batch, q_heads, hd), dtype=q.dtype, device=q.device)
+    else:
+        _here(what, q.dtype, q.shape, out=out)
+    _last(what, q=q, out=out)
+    if batch == 0:
+        return out
+    d = abi.PagedAttentionDesc(batch, q_heads, table.shape[1], window, table.stride(0), q.stride()[:2], out.stride()[:2], scale, softcap)
+    lib = load()
+    nbytes = lib.onhip_attention_paged_workspace(C.byref(c), C.byref(d))
+    ws = _workspace(nbytes, q.device)
+    _check(lib.onhip_attention_paged(C.byref(c), C.byref(d), _ptr(q), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(out), _ptr(ws), nbytes, _stream()),
+           "onhip_attention_paged")
+    return out
+
+
+def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, slopes=None, ranges=None, q_offset=None, out=None, merged_out=True):
+    """attention of prompts: q [batch, q_heads, q_tokens, head_dim], k and v [batch, kv_heads, k_tokens, head_dim], bfloat16 or float16 views in
+    any (batch, head, token) stride order.  Query i at place i + q_offset (k_tokens - q_tokens unless given) sees the keys up to its
+    place (causal), no more than window - 1 behind it (window > 0), and begin <= j < end of ranges [batch, q_tokens, 2] (int32); scores are capped to
+    softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the distance.  Returns [batch, q_tokens, q_heads * head_dim] (heads merged) or,
+    with merged_out=False, [batch, q_heads, q_tokens, head_dim]; `out` may be such a tensor (merged: with a pitch above q_heads * head_dim).  Rows
+    that see nothing are zeros"""
+    import torch
+    what = "attention_masked"
+    compute = _h16_compute(what, q.dtype)
+    b, hq, tq, hd = q.shape
+    hkv, tk = k.shape[1], k.shape[2]
+    _here(what, q.dtype, None, q=q)
+    _here(what, q.dtype, (b, hkv, tk, hd), k=k, v=v)
+    _here(what, torch.float32, (hq,), slopes=slopes)
+    _here(what, torch.int32, (b, tq, 2), ranges=ranges)
+    _flat(what, slopes=slopes, ranges=ranges)
+    if out is None:
+        out = torch.empty((b, tq, hq * hd) if merged_out else (b, hq, tq, hd), dtype=q.dtype, device=q.device)
+    else:
+        _here(what, q.dtype, None, out=out)
+        if tuple(out.shape[:2]) != (b, tq) or out.dim() != 3 or out.shape[2] < hq * hd if merged_out else tuple(out.shape) != (b, hq, tq, hd):
+            raise OnhipError(f"{what}: a result of the shape {tuple(out.shape)}")
+    _last(what, q=q, k=k, v=v, out=out)
+    if b == 0 or tq == 0:
+        return out
+    o_strides = (out.stride(0), hd, out.stride(1)) if merged_out else out.stride()[:3]
+    d = abi.MaskedAttentionDesc(b, hq, hkv, tq, tk, hd, q.stride()[:3], k.stride()[:3], v.stride()[:3], o_strides, scale, softcap, int(causal), window,
+                                tk - tq if q_offset is None else q_offset, compute)
+    lib = load()
+    nbytes = lib.onhip_attention_masked_workspace(C.byref(d))
+    ws = _workspace(nbytes, q.device)
+    _check(lib.onhip_attention_masked(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(ranges), _ptr(slopes), _ptr(out), _ptr(ws), nbytes, _stream()),
+           "onhip_attention_masked")
     return out
 
 

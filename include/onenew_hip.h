@@ -377,13 +377,11 @@ int onhip_attention(const onhip_attention_desc_t *d, const void *q, const void *
  * The cache: `pages` pages of `page_tokens` rows (a power of two up to 1024) for each of `kv_heads` heads; element (page, head, row, channel)
  * of k at page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + channel, v likewise.  quantised == 0: rows of the 16-bit type.
  * quantised == 1: int8 rows (strides multiples of 16) and one fp32 scale a row at page * scale_strides[0] + head * scale_strides[1] +
- * row * scale_strides[2] of k_scale / v_scale; a value is int8 * scale. */
+ * row * scale_strides[2] of k_scale / v_scale (else ignored); a value is int8 * scale. */
 typedef struct onhip_cache_desc {
     int32_t pages, page_tokens, kv_heads, head_dim;
     int32_t compute, quantised;
     long long k_strides[3], v_strides[3], scale_strides[3];
-    void *k, *v;
-    float *k_scale, *v_scale;   /* quantised only */
 } onhip_cache_desc_t;
 
 /* Rows of q, k and v (e.g. slices of one projection's rows) on their way to attention and into the cache.  For each token and head, in fp32:
@@ -402,16 +400,16 @@ typedef struct onhip_cache_rows_desc {
     int32_t pairs, interleaved;
     float eps;
 } onhip_cache_rows_desc_t;
-int onhip_cache_append(const onhip_cache_desc_t *c, const onhip_cache_rows_desc_t *r, const void *q, const void *k, const void *v,
-                       const int32_t *positions, const int32_t *slots, const float *inv_freq, const float *q_weight,
-                       const float *k_weight, void *q_out, void *stream);
+int onhip_cache_append(const onhip_cache_desc_t *c, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                       const onhip_cache_rows_desc_t *r, const void *q, const void *k, const void *v, const int32_t *positions,
+                       const int32_t *slots, const float *inv_freq, const float *q_weight, const float *k_weight, void *q_out, void *stream);
 
 /* The first `tokens` rows of every sequence in order, k and v as values of the 16-bit type: element (sequence, head, token, channel) at
  * sequence * strides[0] + head * strides[1] + token * strides[2] + channel of the results.  Sequence b has lengths[b] rows; row t of it is row
  * t % page_tokens of page table[b * table_stride + t / page_tokens].  Rows behind the last come out as zeros, rows whose page does not exist (a
  * number outside the cache, or past the table's table_pages entries) as NaN. */
-int onhip_cache_read(const onhip_cache_desc_t *c, const int32_t *table, long long table_stride, int32_t table_pages,
-                     const int32_t *lengths, int32_t batch, int32_t tokens, void *k_out, const long long k_out_strides[3], void *v_out,
+int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                     const int32_t *table, long long table_stride, int32_t table_pages, const int32_t *lengths, int32_t batch, int32_t tokens, void *k_out, const long long k_out_strides[3], void *v_out,
                      const long long v_out_strides[3], void *stream);
 
 /* Attention of one new token a sequence, which is the last of its lengths[b] rows in the cache:
@@ -430,8 +428,8 @@ typedef struct onhip_paged_attention_desc {
     float scale, softcap;
 } onhip_paged_attention_desc_t;
 size_t onhip_attention_paged_workspace(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d);
-int onhip_attention_paged(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table,
-                          const int32_t *lengths, const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream);
+int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                          const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table, const int32_t *lengths, const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Attention of prompts: any number of queries and keys, masks, capped and biased scores.  Query i is at place P = i + q_offset among the keys
  * and sees key j when all of these hold:

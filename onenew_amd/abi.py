@@ -224,8 +224,7 @@ class CacheDesc(C.Structure):
     """onhip_cache_desc_t"""
     _fields_ = [("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
                 ("compute", C.c_int32), ("quantised", C.c_int32),
-                ("k_strides", C.c_longlong * 3), ("v_strides", C.c_longlong * 3), ("scale_strides", C.c_longlong * 3),
-                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+                ("k_strides", C.c_longlong * 3), ("v_strides", C.c_longlong * 3), ("scale_strides", C.c_longlong * 3)]
 
 
 class CacheRowsDesc(C.Structure):

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
     constexpr int LOADS = KT / ROWS / 4;                       // loads of a wavefront for its share of a tile of k (or v)
     __shared__ uint4 Ks[2][KT * UNITS];
     __shared__ __attribute__((aligned(16))) unsigned short Vs[2][KT * HD];
-    __shared__ int s_lo[4], s_hi[4];
+    __shared__ int s_lo[4], s_hi[4], s_all_lo[4], s_all_hi[4], s_odd;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
@@ -112,7 +112,10 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
     if (lane == 0) {
         s_lo[wave] = any_lo;
         s_hi[wave] = any_hi;
+        s_all_lo[wave] = all_lo;
+        s_all_hi[wave] = all_hi;
     }
+    if (tid == 0) s_odd = 0;
     // q: the channels 16 s + 8 (lane / 32) .. + 7 of step s
     uint4 qf[STEPS];
     {
@@ -125,6 +128,8 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
     }
     __syncthreads();
     const int wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+    const int wg_all_lo = __builtin_amdgcn_readfirstlane(max(max(s_all_lo[0], s_all_lo[1]), max(s_all_lo[2], s_all_lo[3])));
+    const int wg_all_hi = __builtin_amdgcn_readfirstlane(min(min(s_all_hi[0], s_all_hi[1]), min(s_all_hi[2], s_all_hi[3])));
     int t_begin = __builtin_amdgcn_readfirstlane(wg_lo / KT), t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
     if (wg_hi <= 0) t_begin = t_end = 0;
     if (p.splits > 1) {
@@ -153,7 +158,21 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
     // rows: those four segments are spread over the banks too.
     auto k_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 15) : u ^ (row >> 1 & 7)); };
     auto v_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 3) * 4 : u ^ (row >> 1 & 1) * 4); };
-    auto put = [&](int buf) __attribute__((always_inline)) {
+    // Where some row does not see all of a tile, an infinity or a NaN in v times its probability of zero is not zero: those values go into LDS as
+    // zeros, and are added to the rows that see them behind the loop.
+    unsigned odd = 0u;
+    auto mixed = [&](int t) __attribute__((always_inline)) { return t * KT < wg_all_lo || t * KT + KT > wg_all_hi; };
+    auto put = [&](int buf, bool clean) __attribute__((always_inline)) {
+        if (clean) {   // uniform
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned x = v_reg[i][j], y = finite_of<DT>(x);
+                    odd |= x ^ y;
+                    v_reg[i][j] = y;
+                }
+        }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int row = s_row + i * ROWS;
@@ -260,22 +279,6 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
                 s[n][r] = __builtin_amdgcn_exp2f(GENERAL ? s[n][r] + shift : __builtin_fmaf(s[n][r], p.scale2, shift));
                 l += s[n][r];
             }
-        bool odd = false;   // a value among a masked tile's is no number: 0 of it, for the rows that do not see it, is not 0
-        if (!whole) {
-            f32x16 z;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int d = 0; d < DTILES; ++d) z = mfma(v_frag(buf, n, g, d), make_uint4(0u, 0u, 0u, 0u), z);
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sum += z[r];
-            odd = __any(sum != sum);
-        }
         uint4 pf[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -283,66 +286,63 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
             for (int g = 0; g < 2; ++g)
                 pf[n][g] = make_uint4(pack_h16<DT>(s[n][8 * g], s[n][8 * g + 1]), pack_h16<DT>(s[n][8 * g + 2], s[n][8 * g + 3]),
                                       pack_h16<DT>(s[n][8 * g + 4], s[n][8 * g + 5]), pack_h16<DT>(s[n][8 * g + 6], s[n][8 * g + 7]));
-        if (!odd) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int d = 0; d < DTILES; ++d) o[d] = mfma(v_frag(buf, n, g, d), pf[n][g], o[d]);
-        } else {
-            // finite values as ever; then, for infinities of either sign and NaN, how many of them a row sees
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int d = 0; d < DTILES; ++d) {
-                        const uint4 x = v_frag(buf, n, g, d);
-                        o[d] = mfma(make_uint4(finite_of<DT>(x.x), finite_of<DT>(x.y), finite_of<DT>(x.z), finite_of<DT>(x.w)), pf[n][g], o[d]);
-                    }
-            constexpr unsigned ONE = DT == DT_BF16 ? 0x3f80u : 0x3c00u;
-            const unsigned span = (unsigned) (hi - lo);
-#pragma unroll 1
-            for (int what = 0; what < 3; ++what) {
-                const float value = what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN;
-#pragma unroll
-                for (int d = 0; d < DTILES; ++d) {
-                    f32x16 z;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
-#pragma unroll 1
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll 1
-                        for (int g = 0; g < 2; ++g) {
-                            unsigned seen[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int key = key0 + 32 * n + 16 * g + 8 * (j / 2) + 4 * lh + j % 2 * 2;
-                                seen[j] = ((unsigned) (key - lo) < span ? ONE : 0u) | ((unsigned) (key + 1 - lo) < span ? ONE << 16 : 0u);
-                            }
-                            const uint4 x = v_frag(buf, n, g, d);
-                            z = mfma(make_uint4(special_of<DT>(x.x, what), special_of<DT>(x.y, what), special_of<DT>(x.z, what), special_of<DT>(x.w, what)),
-                                     make_uint4(seen[0], seen[1], seen[2], seen[3]), z);
-                        }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] += z[r] > 0.0f ? value : 0.0f;
-                }
-            }
-        }
+                for (int d = 0; d < DTILES; ++d) o[d] = mfma(v_frag(buf, n, g, d), pf[n][g], o[d]);
     };
 
     if (t_begin < t_end) {
         fetch(t_begin);
-        put(0);
+        put(0, mixed(t_begin));
         if (t_begin + 1 < t_end) fetch(t_begin + 1);
         for (int t = t_begin; t < t_end; ++t) {
             const int buf = (t - t_begin) & 1;
             __syncthreads();   // tile t is in LDS, tile t - 1 has been read
-            if (t + 1 < t_end) put(buf ^ 1);
+            if (t + 1 < t_end) put(buf ^ 1, mixed(t + 1));
             if (t + 2 < t_end) fetch(t + 2);
             tile(t, buf);
         }
+    }
+
+    if (__any(odd != 0u) && lane == 0) s_odd = 1;
+    __syncthreads();
+    if (s_odd) {   // uniform and rare: for infinities of either sign and NaN, how many of a channel a row sees
+        constexpr unsigned ONE = DT == DT_BF16 ? 0x3f80u : 0x3c00u;
+        const unsigned span = (unsigned) (hi - lo);
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll 1
+            for (int what = 0; what < 3; ++what) {
+                f32x16 z;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll 1
+                for (int t = t_begin; t < t_end; ++t) {
+                    if (!mixed(t)) continue;   // uniform in the workgroup
+                    __syncthreads();
+                    fetch(t);
+                    put(0, false);
+                    __syncthreads();
+#pragma unroll 1
+                    for (int i = 0; i < 2 * NT; ++i) {
+                        unsigned seen[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = t * KT + 16 * i + 8 * (j / 2) + 4 * lh + j % 2 * 2;
+                            seen[j] = ((unsigned) (key - lo) < span ? ONE : 0u) | ((unsigned) (key + 1 - lo) < span ? ONE << 16 : 0u);
+                        }
+                        const uint4 x = v_frag(0, 0, i, d);
+                        z = mfma(make_uint4(special_of<DT>(x.x, what), special_of<DT>(x.y, what), special_of<DT>(x.z, what), special_of<DT>(x.w, what)),
+                                 make_uint4(seen[0], seen[1], seen[2], seen[3]), z);
+                    }
+                }
+                const float value = what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] += z[r] > 0.0f ? value : 0.0f;
+            }
     }
 
     l += __shfl_xor(l, 32, 64);

@@ -378,7 +378,7 @@ static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention
 }
 
 static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, CacheView *view, int *dt) {
-    const int rc = cache_view("paged attention", c, view, dt);
+    const int rc = cache_shape("paged attention", c, view, dt);
     if (rc) return rc;
     if (!d || d->batch < 1 || d->q_heads < 1 || d->table_pages < 1 || d->table_stride < 0) return set_error(ONHIP_ERR_ARG, "paged attention: bad shape");
     if (d->q_heads % c->kv_heads) return set_error(ONHIP_ERR_ARG, "paged attention: %d query heads for %d key-value heads", d->q_heads, c->kv_heads);
@@ -410,11 +410,12 @@ size_t onhip_attention_paged_workspace(const onhip_cache_desc_t *c, const onhip_
     return join_bytes((long long) d->batch * d->q_heads, paged_splits(c, d), c->head_dim);
 }
 
-int onhip_attention_paged(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table,
-                          const int32_t *lengths, const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                          const onhip_paged_attention_desc_t *d, const void *q, const int32_t *table, const int32_t *lengths,
+                          const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream) {
     PagedParams p;
-    int dt;
-    const int rc = paged_check(c, d, &p.c, &dt);
+    int dt, rc = paged_check(c, d, &p.c, &dt);
+    if (!rc) rc = cache_memory("paged attention", c, k_cache, v_cache, k_scale, v_scale, &p.c);
     if (rc) return rc;
     if (!q || !out || !table || !lengths) return set_error(ONHIP_ERR_ARG, "paged attention: null pointer");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16) return set_error(ONHIP_ERR_ARG, "paged attention: tensors must be 16-byte aligned");

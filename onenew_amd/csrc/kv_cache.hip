@@ -13,7 +13,7 @@
 
 namespace onhip {
 
-int cache_view(const char *what, const onhip_cache_desc_t *c, CacheView *view, int *dt) {
+int cache_shape(const char *what, const onhip_cache_desc_t *c, CacheView *view, int *dt) {
     if (!c) return set_error(ONHIP_ERR_ARG, "%s: null cache description", what);
     if (c->compute == ONHIP_COMPUTE_BF16) *dt = DT_BF16;
     else if (c->compute == ONHIP_COMPUTE_F16) *dt = DT_F16;
@@ -24,11 +24,6 @@ int cache_view(const char *what, const onhip_cache_desc_t *c, CacheView *view, i
         return set_error(ONHIP_ERR_ARG, "%s: pages of %d tokens (a power of two up to 1024)", what, c->page_tokens);
     if ((long long) c->pages * c->page_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "%s: a cache of 2^31 tokens or more", what);
     if (c->quantised != 0 && c->quantised != 1) return set_error(ONHIP_ERR_ARG, "%s: quantised = %d", what, c->quantised);
-    if (!c->k || !c->v) return set_error(ONHIP_ERR_ARG, "%s: null cache pointer", what);
-    if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16) return set_error(ONHIP_ERR_ARG, "%s: the cache must be 16-byte aligned", what);
-    if (c->quantised && (!c->k_scale || !c->v_scale)) return set_error(ONHIP_ERR_ARG, "%s: an int8 cache needs its scales", what);
-    if (c->quantised && (reinterpret_cast<uintptr_t>(c->k_scale) % 4 || reinterpret_cast<uintptr_t>(c->v_scale) % 4))
-        return set_error(ONHIP_ERR_ARG, "%s: misaligned scales", what);
     const int vec = c->quantised ? 16 : 8, extent[3] = {c->pages, c->kv_heads, c->page_tokens};
     const long long *strides[2] = {c->k_strides, c->v_strides};
     for (int t = 0; t < 2; ++t)
@@ -44,10 +39,6 @@ int cache_view(const char *what, const onhip_cache_desc_t *c, CacheView *view, i
             if (extent[i] > 1 && (c->scale_strides[i] < 1 || (i == 2 && c->scale_strides[i] >= (1LL << 30) / c->page_tokens)))
                 return set_error(ONHIP_ERR_ARG, "%s: bad scale strides", what);
     const int size = c->quantised ? 1 : 2;
-    view->k = reinterpret_cast<char *>(c->k);
-    view->v = reinterpret_cast<char *>(c->v);
-    view->k_scale = c->k_scale;
-    view->v_scale = c->v_scale;
     for (int i = 0; i < 3; ++i) {
         view->ks[i] = extent[i] == 1 ? 0 : c->k_strides[i] * size;
         view->vs[i] = extent[i] == 1 ? 0 : c->v_strides[i] * size;
@@ -56,6 +47,19 @@ int cache_view(const char *what, const onhip_cache_desc_t *c, CacheView *view, i
     view->pages = c->pages;
     view->page_shift = __builtin_ctz((unsigned) c->page_tokens);
     view->page_mask = c->page_tokens - 1;
+    return ONHIP_OK;
+}
+
+int cache_memory(const char *what, const onhip_cache_desc_t *c, const void *k, const void *v, const float *k_scale, const float *v_scale, CacheView *view) {
+    if (!k || !v) return set_error(ONHIP_ERR_ARG, "%s: null cache pointer", what);
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16) return set_error(ONHIP_ERR_ARG, "%s: the cache must be 16-byte aligned", what);
+    if (c->quantised && (!k_scale || !v_scale)) return set_error(ONHIP_ERR_ARG, "%s: an int8 cache needs its scales", what);
+    if (c->quantised && (reinterpret_cast<uintptr_t>(k_scale) % 4 || reinterpret_cast<uintptr_t>(v_scale) % 4))
+        return set_error(ONHIP_ERR_ARG, "%s: misaligned scales", what);
+    view->k = const_cast<char *>(reinterpret_cast<const char *>(k));   // cache_append alone writes through them
+    view->v = const_cast<char *>(reinterpret_cast<const char *>(v));
+    view->k_scale = const_cast<float *>(k_scale);
+    view->v_scale = const_cast<float *>(v_scale);
     return ONHIP_OK;
 }
 
@@ -304,12 +308,12 @@ using namespace onhip;
 
 extern "C" {
 
-int onhip_cache_append(const onhip_cache_desc_t *c, const onhip_cache_rows_desc_t *r, const void *q, const void *k, const void *v,
-                       const int32_t *positions, const int32_t *slots, const float *inv_freq, const float *q_weight,
-                       const float *k_weight, void *q_out, void *stream) {
+int onhip_cache_append(const onhip_cache_desc_t *c, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                       const onhip_cache_rows_desc_t *r, const void *q, const void *k, const void *v, const int32_t *positions,
+                       const int32_t *slots, const float *inv_freq, const float *q_weight, const float *k_weight, void *q_out, void *stream) {
     AppendParams p;
-    int dt;
-    const int rc = cache_view("cache append", c, &p.c, &dt);
+    int dt, rc = cache_shape("cache append", c, &p.c, &dt);
+    if (!rc) rc = cache_memory("cache append", c, k_cache, v_cache, k_scale, v_scale, &p.c);
     if (rc) return rc;
     if (!r || r->tokens < 1 || r->q_heads < 1) return set_error(ONHIP_ERR_ARG, "cache append: bad shape");
     if (r->q_heads > (1 << 20) || c->kv_heads > (1 << 20)) return set_error(ONHIP_ERR_ARG, "cache append: %d and %d heads", r->q_heads, c->kv_heads);
@@ -354,12 +358,13 @@ int onhip_cache_append(const onhip_cache_desc_t *c, const onhip_cache_rows_desc_
     return dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
 }
 
-int onhip_cache_read(const onhip_cache_desc_t *c, const int32_t *table, long long table_stride, int32_t table_pages, const int32_t *lengths,
+int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                     const int32_t *table, long long table_stride, int32_t table_pages, const int32_t *lengths,
                      int32_t batch, int32_t tokens, void *k_out, const long long k_out_strides[3], void *v_out, const long long v_out_strides[3],
                      void *stream) {
     ReadParams p;
-    int dt;
-    const int rc = cache_view("cache read", c, &p.c, &dt);
+    int dt, rc = cache_shape("cache read", c, &p.c, &dt);
+    if (!rc) rc = cache_memory("cache read", c, k_cache, v_cache, k_scale, v_scale, &p.c);
     if (rc) return rc;
     if (batch < 1 || tokens < 1 || table_pages < 1 || table_stride < 0) return set_error(ONHIP_ERR_ARG, "cache read: bad shape");
     if (batch > 32767 || c->kv_heads > 65535) return set_error(ONHIP_ERR_ARG, "cache read: %d sequences of %d heads", batch, c->kv_heads);

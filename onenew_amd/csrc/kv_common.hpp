@@ -13,8 +13,10 @@ struct CacheView {
     int pages, page_shift, page_mask;
 };
 
-// fills the view after checking the description; `what` names the entry point in the message
-int cache_view(const char *what, const onhip_cache_desc_t *c, CacheView *view, int *dt);
+// checks the description and fills the view's sizes and strides; `what` names the entry point in the message
+int cache_shape(const char *what, const onhip_cache_desc_t *c, CacheView *view, int *dt);
+// checks the addresses and fills them in
+int cache_memory(const char *what, const onhip_cache_desc_t *c, const void *k, const void *v, const float *k_scale, const float *v_scale, CacheView *view);
 
 // eight (NV = 2) or four (NV = 1) signed bytes as pairs of the 16-bit type: every int8 is a bf16 and an fp16
 template <int DT, int NV> __device__ __forceinline__ void s8_to_h16(const unsigned (&x)[NV], unsigned (&y)[2 * NV]) {

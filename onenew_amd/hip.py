@@ -129,11 +129,11 @@ def load():
     L.onhip_conv2d_h16_first.argtypes = [C.POINTER(ConvDesc), vp, vp, vp, vp, vp, i32, vp]
     L.onhip_attention.argtypes = [C.POINTER(abi.AttentionDesc), vp, vp, vp, vp, vp]
     cache = C.POINTER(abi.CacheDesc)
-    L.onhip_cache_append.argtypes = [cache, C.POINTER(abi.CacheRowsDesc)] + [vp] * 10
-    L.onhip_cache_read.argtypes = [cache, vp, C.c_longlong, i32, vp, i32, i32, vp, C.POINTER(C.c_longlong), vp, C.POINTER(C.c_longlong), vp]
+    L.onhip_cache_append.argtypes = [cache] + [vp] * 4 + [C.POINTER(abi.CacheRowsDesc)] + [vp] * 10
+    L.onhip_cache_read.argtypes = [cache] + [vp] * 5 + [C.c_longlong, i32, vp, i32, i32, vp, C.POINTER(C.c_longlong), vp, C.POINTER(C.c_longlong), vp]
     L.onhip_attention_paged_workspace.argtypes = [cache, C.POINTER(abi.PagedAttentionDesc)]
     L.onhip_attention_paged_workspace.restype = C.c_size_t
-    L.onhip_attention_paged.argtypes = [cache, C.POINTER(abi.PagedAttentionDesc)] + [vp] * 6 + [C.c_size_t, vp]
+    L.onhip_attention_paged.argtypes = [cache] + [vp] * 4 + [C.POINTER(abi.PagedAttentionDesc)] + [vp] * 6 + [C.c_size_t, vp]
     L.onhip_attention_masked_workspace.argtypes = [C.POINTER(abi.MaskedAttentionDesc)]
     L.onhip_attention_masked_workspace.restype = C.c_size_t
     L.onhip_attention_masked.argtypes = [C.POINTER(abi.MaskedAttentionDesc)] + [vp] * 7 + [C.c_size_t, vp]
@@ -702,20 +702,46 @@ def attention(q, k, v, scale=1.0, out=None, merged_out=True):
 
 
 # ---- a paged key-value cache and the attention around it: bf16 / fp16 tensors, int8 caches with fp32 scales ----
+#
+# What a call has to check and to describe depends on types, devices, shapes and strides alone, and a step's calls repeat them: the checked
+# descriptions are kept by those (a call that finds its own takes 8 us of host time, with the checks 15 to 24).  Addresses are passed on each call.
+_plans = {}
 
-def _here(what, dtype, shape=None, **tensors):
-    """checks what the C entry points cannot see: the type, the device and (given one) the shape of tensors, None left out"""
+
+def _plan(key, make):
+    if len(_plans) >= 4096:
+        _plans.clear()
+    plan = _plans[key] = make()
+    return plan
+
+
+def _meta(t):
+    return t if t is None else (t.dtype, t.get_device(), t.shape, t.stride())
+
+
+def _device():
+    """torch's current device, without the checks around it that a tensor on a device has passed"""
     import torch
-    device = torch.cuda.current_device()
+    return torch._C._cuda_getDevice()
+
+
+def _need(what, dtype, shape=None, flat=False, last=False, **tensors):
+    """checks the type, the device (the current one), and where given the shape of tensors, None left out; flat: contiguous, last: the last
+    dimension is"""
+    device = _device()
     for name, t in tensors.items():
         if t is None:
             continue
         if t.dtype != dtype:
             raise OnhipError(f"{what}: {name} is {t.dtype}, not {dtype}")
-        if t.device.type != "cuda" or t.device.index != device:
+        if t.get_device() != device:
             raise OnhipError(f"{what}: {name} is on {t.device}, the current device is cuda:{device}")
         if shape is not None and tuple(t.shape) != tuple(shape):
             raise OnhipError(f"{what}: {name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
+        if flat and not t.is_contiguous():
+            raise OnhipError(f"{what}: {name} must be contiguous")
+        if last and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise OnhipError(f"{what}: the head dimension of {name} must be contiguous")
 
 
 def _h16_compute(what, dtype):
@@ -727,16 +753,10 @@ def _h16_compute(what, dtype):
     raise OnhipError(f"{what}: {dtype} is neither bfloat16 nor float16")
 
 
-def _flat(what, **tensors):
+def _dims(what, n, **tensors):
     for name, t in tensors.items():
-        if t is not None and not t.is_contiguous():
-            raise OnhipError(f"{what}: {name} must be contiguous")
-
-
-def _last(what, **tensors):
-    for name, t in tensors.items():
-        if t.stride(-1) != 1:
-            raise OnhipError(f"{what}: the head dimension of {name} must be contiguous")
+        if t.dim() != n:
+            raise OnhipError(f"{what}: {name} has {t.dim()} dimensions, not {n}")
 
 
 def _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype):
@@ -744,22 +764,36 @@ def _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype):
     import torch
     quantised = k_cache.dtype == torch.int8
     compute = _h16_compute(what, dtype)
-    if k_cache.dim() != 4:
-        raise OnhipError(f"{what}: a cache is [pages, kv_heads, page_tokens, head_dim]")
-    _here(what, torch.int8 if quantised else dtype, k_cache.shape, k_cache=k_cache, v_cache=v_cache)
-    _last(what, k_cache=k_cache, v_cache=v_cache)
-    d = abi.CacheDesc(*k_cache.shape[:1], k_cache.shape[2], k_cache.shape[1], k_cache.shape[3], compute, int(quantised))
-    d.k_strides[:], d.v_strides[:] = k_cache.stride()[:3], v_cache.stride()[:3]
-    d.k, d.v = k_cache.data_ptr(), v_cache.data_ptr()
+    _dims(what, 4, k_cache=k_cache)
+    _need(what, torch.int8 if quantised else dtype, k_cache.shape, last=True, k_cache=k_cache, v_cache=v_cache)
+    pages, heads, rows, hd = k_cache.shape
+    d = abi.CacheDesc(pages, rows, heads, hd, compute, int(quantised), k_cache.stride()[:3], v_cache.stride()[:3])
     if (k_scale is None) != (not quantised) or (v_scale is None) != (not quantised):
         raise OnhipError(f"{what}: scales go with an int8 cache, and an int8 cache with scales")
     if quantised:
-        _here(what, torch.float32, k_cache.shape[:3], k_scale=k_scale, v_scale=v_scale)
+        _need(what, torch.float32, k_cache.shape[:3], k_scale=k_scale, v_scale=v_scale)
         if k_scale.stride() != v_scale.stride():
             raise OnhipError(f"{what}: k_scale and v_scale must have the same strides")
         d.scale_strides[:] = k_scale.stride()
-        d.k_scale, d.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
     return d
+
+
+def _append_plan(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_weight, k_weight, eps, interleaved, k_scale, v_scale, q_out):
+    import torch
+    what = "cache_append"
+    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
+    _dims(what, 3, q=q)
+    tokens, q_heads, hd = q.shape
+    if hd != d.head_dim:
+        raise OnhipError(f"{what}: heads of {hd} channels for a cache of {d.head_dim}")
+    _need(what, q.dtype, q.shape, last=True, q=q, q_out=q_out)
+    _need(what, q.dtype, (tokens, d.kv_heads, hd), last=True, k=k, v=v)
+    _need(what, torch.int32, (tokens,), flat=True, positions=positions, slots=slots)
+    _need(what, torch.float32, (hd,), flat=True, q_weight=q_weight, k_weight=k_weight)
+    _need(what, torch.float32, flat=True, inv_freq=inv_freq)
+    r = abi.CacheRowsDesc(tokens, q_heads, q.stride()[:2], k.stride()[:2], v.stride()[:2], (q_heads * hd, hd) if q_out is None else q_out.stride()[:2],
+                          0 if inv_freq is None else inv_freq.numel(), int(interleaved), eps)
+    return C.byref(d), C.byref(r), q.shape, tokens == 0
 
 
 def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
@@ -769,69 +803,75 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
     where there are frequencies, q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
     [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with fp32 scales [pages, kv_heads, page_tokens]"""
     import torch
-    what = "cache_append"
-    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
-    tokens, q_heads, hd = q.shape
-    if hd != d.head_dim:
-        raise OnhipError(f"{what}: heads of {hd} channels for a cache of {d.head_dim}")
-    _here(what, q.dtype, None, q=q)
-    _here(what, q.dtype, (tokens, d.kv_heads, hd), k=k, v=v)
+    key = ("append", _device(), _meta(q), _meta(k), _meta(v), _meta(positions), _meta(slots), _meta(k_cache), _meta(v_cache), _meta(inv_freq),
+           _meta(q_weight), _meta(k_weight), eps, interleaved, _meta(k_scale), _meta(v_scale), _meta(q_out))
+    d, r, shape, empty = _plans.get(key) or _plan(key, lambda: _append_plan(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_weight, k_weight, eps,
+                                                                            interleaved, k_scale, v_scale, q_out))
     if q_out is None:
-        q_out = torch.empty((tokens, q_heads, hd), dtype=q.dtype, device=q.device)
-    else:
-        _here(what, q.dtype, q.shape, q_out=q_out)
-    _last(what, q=q, k=k, v=v, q_out=q_out)
-    _here(what, torch.int32, (tokens,), positions=positions, slots=slots)
-    _here(what, torch.float32, (hd,), q_weight=q_weight, k_weight=k_weight)
-    _here(what, torch.float32, None, inv_freq=inv_freq)
-    _flat(what, positions=positions, slots=slots, q_weight=q_weight, k_weight=k_weight, inv_freq=inv_freq)
-    if tokens == 0:
-        return q_out
-    r = abi.CacheRowsDesc(tokens=tokens, q_heads=q_heads, pairs=0 if inv_freq is None else inv_freq.numel(), interleaved=int(interleaved), eps=eps)
-    for name, t in (("q_strides", q), ("k_strides", k), ("v_strides", v), ("out_strides", q_out)):
-        getattr(r, name)[:] = t.stride()[:2]
-    _check(load().onhip_cache_append(C.byref(d), C.byref(r), _ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(slots), _ptr(inv_freq), _ptr(q_weight),
-                                     _ptr(k_weight), _ptr(q_out), _stream()), "onhip_cache_append")
+        q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    if not empty:
+        _check(load().onhip_cache_append(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), r, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                         positions.data_ptr(), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream()),
+               "onhip_cache_append")
     return q_out
 
 
-def _table(what, table, lengths, batch):
+def _table(what, table, lengths):
     import torch
-    _here(what, torch.int32, None, table=table)
-    _here(what, torch.int32, (batch,), lengths=lengths)
-    _flat(what, lengths=lengths)
-    if table.dim() != 2 or table.shape[0] != batch or (table.shape[1] > 1 and table.stride(1) != 1):
+    _dims(what, 2, table=table)
+    _need(what, torch.int32, table=table)
+    _need(what, torch.int32, table.shape[:1], flat=True, lengths=lengths)
+    if table.shape[1] > 1 and table.stride(1) != 1:
         raise OnhipError(f"{what}: the table is [sequences, pages] with contiguous rows")
+
+
+def _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype, k_out, v_out):
+    what = "cache_read"
+    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype)
+    _table(what, table, lengths)
+    shape = (table.shape[0], d.kv_heads, tokens, d.head_dim)
+    _need(what, dtype, shape, last=True, k_out=k_out, v_out=v_out)
+    flat = (d.kv_heads * tokens * d.head_dim, tokens * d.head_dim, d.head_dim)
+    strides = [(C.c_longlong * 3)(*(flat if t is None else t.stride()[:3])) for t in (k_out, v_out)]
+    return C.byref(d), shape, table.stride(0), table.shape[1], strides[0], strides[1], shape[0] == 0 or tokens == 0
 
 
 def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
     """rows 0 .. tokens - 1 of every sequence (pages table [sequences, pages], lengths [sequences], int32), zeros behind its length: k and v
     [sequences, kv_heads, tokens, head_dim] in the cache's 16-bit type, or `dtype` for an int8 cache"""
     import torch
-    what = "cache_read"
     dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
-    d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype)
-    batch = table.shape[0]
-    _table(what, table, lengths, batch)
-    shape = (batch, d.kv_heads, tokens, d.head_dim)
+    key = ("read", _device(), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), tokens, _meta(k_scale), _meta(v_scale), dtype, _meta(k_out), _meta(v_out))
+    d, shape, step, pages, ks, vs, empty = _plans.get(key) or _plan(key, lambda: _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype, k_out, v_out))
     if k_out is None:
         k_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
     if v_out is None:
         v_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
-    _here(what, dtype, shape, k_out=k_out, v_out=v_out)
-    _last(what, k_out=k_out, v_out=v_out)
-    if batch == 0 or tokens == 0:
-        return k_out, v_out
-    three = C.c_longlong * 3
-    _check(load().onhip_cache_read(C.byref(d), _ptr(table), table.stride(0), table.shape[1], _ptr(lengths), batch, tokens, _ptr(k_out), three(*k_out.stride()[:3]),
-                                   _ptr(v_out), three(*v_out.stride()[:3]), _stream()), "onhip_cache_read")
+    if not empty:
+        _check(load().onhip_cache_read(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), step, pages, lengths.data_ptr(),
+                                       shape[0], tokens, k_out.data_ptr(), ks, v_out.data_ptr(), vs, _stream()), "onhip_cache_read")
     return k_out, v_out
 
 
 def _workspace(nbytes, device):
-    """of this call alone, from torch's allocator: ordered on the stream, private to a graph that is being captured"""
+    """of one call alone, from torch's allocator: ordered on the stream, private to a graph that is being captured"""
     import torch
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _paged_plan(q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale, v_scale, out):
+    import torch
+    what = "attention_paged"
+    c = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
+    _table(what, table, lengths)
+    _dims(what, 3, q=q)
+    batch, q_heads, hd = q.shape
+    _need(what, q.dtype, (table.shape[0], q_heads, c.head_dim), last=True, q=q)
+    _need(what, q.dtype, q.shape, last=True, out=out)
+    _need(what, torch.float32, (q_heads,), flat=True, slopes=slopes)
+    d = abi.PagedAttentionDesc(batch, q_heads, table.shape[1], window, table.stride(0), q.stride()[:2], (q_heads * hd, hd) if out is None else out.stride()[:2],
+                               scale, softcap)
+    return C.byref(c), C.byref(d), q.shape, load().onhip_attention_paged_workspace(C.byref(c), C.byref(d)), batch == 0
 
 
 def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, softcap=0.0, slopes=None, k_scale=None, v_scale=None, out=None):
@@ -839,27 +879,40 @@ def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, so
     [sequences] (int32; the new token's row is the last): scores capped to softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the
     distance, the last `window` rows alone where it is above zero; returns [sequences, q_heads, head_dim]"""
     import torch
-    what = "attention_paged"
-    c = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
-    batch, q_heads, hd = q.shape
-    _here(what, q.dtype, (batch, q_heads, c.head_dim), q=q)
-    _table(what, table, lengths, batch)
-    _here(what, torch.float32, (q_heads,), slopes=slopes)
-    _flat(what, slopes=slopes)
+    key = ("paged", _device(), _meta(q), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), scale, window, softcap, _meta(slopes), _meta(k_scale),
+           _meta(v_scale), _meta(out))
+    c, d, shape, nbytes, empty = _plans.get(key) or _plan(key, lambda: _paged_plan(q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale,
+                                                                                   v_scale, out))
     if out is None:
-        out = torch.empty((batch, q_heads, hd), dtype=q.dtype, device=q.device)
-    else:
-        _here(what, q.dtype, q.shape, out=out)
-    _last(what, q=q, out=out)
-    if batch == 0:
-        return out
-    d = abi.PagedAttentionDesc(batch, q_heads, table.shape[1], window, table.stride(0), q.stride()[:2], out.stride()[:2], scale, softcap)
-    lib = load()
-    nbytes = lib.onhip_attention_paged_workspace(C.byref(c), C.byref(d))
-    ws = _workspace(nbytes, q.device)
-    _check(lib.onhip_attention_paged(C.byref(c), C.byref(d), _ptr(q), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(out), _ptr(ws), nbytes, _stream()),
-           "onhip_attention_paged")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    if not empty:
+        ws = _workspace(nbytes, q.device) if nbytes else None
+        _check(load().onhip_attention_paged(c, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), d, q.data_ptr(), table.data_ptr(),
+                                            lengths.data_ptr(), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()), "onhip_attention_paged")
     return out
+
+
+def _masked_plan(q, k, v, scale, causal, window, softcap, slopes, ranges, q_offset, out, merged_out):
+    import torch
+    what = "attention_masked"
+    compute = _h16_compute(what, q.dtype)
+    _dims(what, 4, q=q, k=k)
+    b, hq, tq, hd = q.shape
+    hkv, tk = k.shape[1], k.shape[2]
+    _need(what, q.dtype, last=True, q=q, out=out)
+    _need(what, q.dtype, (b, hkv, tk, hd), last=True, k=k, v=v)
+    _need(what, torch.float32, (hq,), flat=True, slopes=slopes)
+    _need(what, torch.int32, (b, tq, 2), flat=True, ranges=ranges)
+    shape = (b, tq, hq * hd) if merged_out else (b, hq, tq, hd)
+    if out is None:
+        o_strides = (tq * hq * hd, hd, hq * hd) if merged_out else (hq * tq * hd, tq * hd, hd)
+    else:
+        if tuple(out.shape[:-1]) != shape[:-1] or out.shape[-1] < shape[-1] or (not merged_out and out.shape[-1] != hd):
+            raise OnhipError(f"{what}: a result of the shape {tuple(out.shape)}, not {shape}")
+        o_strides = (out.stride(0), hd, out.stride(1)) if merged_out else out.stride()[:3]
+    d = abi.MaskedAttentionDesc(b, hq, hkv, tq, tk, hd, q.stride()[:3], k.stride()[:3], v.stride()[:3], o_strides, scale, softcap, int(causal), window,
+                                tk - tq if q_offset is None else q_offset, compute)
+    return C.byref(d), shape, load().onhip_attention_masked_workspace(C.byref(d)), b == 0 or tq == 0
 
 
 def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, slopes=None, ranges=None, q_offset=None, out=None, merged_out=True):
@@ -870,32 +923,14 @@ def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, sl
     with merged_out=False, [batch, q_heads, q_tokens, head_dim]; `out` may be such a tensor (merged: with a pitch above q_heads * head_dim).  Rows
     that see nothing are zeros"""
     import torch
-    what = "attention_masked"
-    compute = _h16_compute(what, q.dtype)
-    b, hq, tq, hd = q.shape
-    hkv, tk = k.shape[1], k.shape[2]
-    _here(what, q.dtype, None, q=q)
-    _here(what, q.dtype, (b, hkv, tk, hd), k=k, v=v)
-    _here(what, torch.float32, (hq,), slopes=slopes)
-    _here(what, torch.int32, (b, tq, 2), ranges=ranges)
-    _flat(what, slopes=slopes, ranges=ranges)
+    key = ("masked", _device(), _meta(q), _meta(k), _meta(v), scale, causal, window, softcap, _meta(slopes), _meta(ranges), q_offset, _meta(out), merged_out)
+    d, shape, nbytes, empty = _plans.get(key) or _plan(key, lambda: _masked_plan(q, k, v, scale, causal, window, softcap, slopes, ranges, q_offset, out, merged_out))
     if out is None:
-        out = torch.empty((b, tq, hq * hd) if merged_out else (b, hq, tq, hd), dtype=q.dtype, device=q.device)
-    else:
-        _here(what, q.dtype, None, out=out)
-        if tuple(out.shape[:2]) != (b, tq) or out.dim() != 3 or out.shape[2] < hq * hd if merged_out else tuple(out.shape) != (b, hq, tq, hd):
-            raise OnhipError(f"{what}: a result of the shape {tuple(out.shape)}")
-    _last(what, q=q, k=k, v=v, out=out)
-    if b == 0 or tq == 0:
-        return out
-    o_strides = (out.stride(0), hd, out.stride(1)) if merged_out else out.stride()[:3]
-    d = abi.MaskedAttentionDesc(b, hq, hkv, tq, tk, hd, q.stride()[:3], k.stride()[:3], v.stride()[:3], o_strides, scale, softcap, int(causal), window,
-                                tk - tq if q_offset is None else q_offset, compute)
-    lib = load()
-    nbytes = lib.onhip_attention_masked_workspace(C.byref(d))
-    ws = _workspace(nbytes, q.device)
-    _check(lib.onhip_attention_masked(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(ranges), _ptr(slopes), _ptr(out), _ptr(ws), nbytes, _stream()),
-           "onhip_attention_masked")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    if not empty:
+        ws = _workspace(nbytes, q.device) if nbytes else None
+        _check(load().onhip_attention_masked(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()),
+               "onhip_attention_masked")
     return out
 
 

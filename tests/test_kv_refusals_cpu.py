@@ -9,8 +9,8 @@ A = 1 << 20   # an address that is never used
 
 
 def _cache(**more):
-    f = dict(pages=8, page_tokens=16, kv_heads=2, head_dim=64, compute=abi.COMPUTE_BF16, quantised=0, k=A, v=A)
-    f.update(more)
+    f = dict(pages=8, page_tokens=16, kv_heads=2, head_dim=64, compute=abi.COMPUTE_BF16, quantised=0)
+    f.update({n: x for n, x in more.items() if n not in ("k", "v", "k_scale", "v_scale")})
     d = abi.CacheDesc(**{n: x for n, x in f.items() if not n.endswith("strides")})
     rows = f["page_tokens"] * f["head_dim"]
     d.k_strides[:] = f.get("k_strides", (2 * rows, rows, f["head_dim"]))
@@ -31,8 +31,12 @@ def _refused(rc, word, code=-1):
     assert word in hip.load().onhip_last_error().decode()
 
 
-def _append(c, r, q=A, k=A, v=A, positions=A, slots=A, inv_freq=A, qw=None, kw=None, out=A):
-    return hip.load().onhip_cache_append(None if c is None else C.byref(c), None if r is None else C.byref(r), q, k, v, positions, slots, inv_freq, qw, kw, out, None)
+def _memory(more):
+    return [more.get(n, at) for n, at in (("k", A), ("v", A), ("k_scale", None), ("v_scale", None))]
+
+
+def _append(c, r, q=A, k=A, v=A, positions=A, slots=A, inv_freq=A, qw=None, kw=None, out=A, memory=(A, A, None, None)):
+    return hip.load().onhip_cache_append(None if c is None else C.byref(c), *memory, None if r is None else C.byref(r), q, k, v, positions, slots, inv_freq, qw, kw, out, None)
 
 
 def _rows(**more):
@@ -46,13 +50,14 @@ def _rows(**more):
 
 @pytest.mark.parametrize("i", range(len(BAD_CACHES)))
 def test_caches(i):
-    c = _cache(**BAD_CACHES[i])
-    _refused(_append(c, _rows()), "cache append")
+    c, memory = _cache(**BAD_CACHES[i]), _memory(BAD_CACHES[i])
+    _refused(_append(c, _rows(), memory=memory), "cache append")
     three = (C.c_longlong * 3)(4096, 1024, 64)
-    _refused(hip.load().onhip_cache_read(C.byref(c), A, 4, 4, A, 1, 5, A, three, A, three, None), "cache read")
+    _refused(hip.load().onhip_cache_read(C.byref(c), *memory, A, 4, 4, A, 1, 5, A, three, A, three, None), "cache read")
     d = abi.PagedAttentionDesc(1, 4, 4, 0, 4, (256, 64), (256, 64), 1.0, 0.0)
-    _refused(hip.load().onhip_attention_paged(C.byref(c), C.byref(d), A, A, A, None, A, None, 0, None), "paged attention")
-    assert hip.load().onhip_attention_paged_workspace(C.byref(c), C.byref(d)) == 0
+    _refused(hip.load().onhip_attention_paged(C.byref(c), *memory, C.byref(d), A, A, A, None, A, None, 0, None), "paged attention")
+    if not set(BAD_CACHES[i]) & {"k", "v", "k_scale"}:
+        assert hip.load().onhip_attention_paged_workspace(C.byref(c), C.byref(d)) == 0
 
 
 def test_append():
@@ -82,7 +87,7 @@ def test_read():
     three = lambda *x: (C.c_longlong * 3)(*x)  # noqa: E731
 
     def read(table=A, stride=4, pages=4, lengths=A, batch=2, tokens=5, k=A, ks=three(4096, 1024, 64), v=A, vs=three(4096, 1024, 64)):
-        return lib.onhip_cache_read(C.byref(c), table, stride, pages, lengths, batch, tokens, k, ks, v, vs, None)
+        return lib.onhip_cache_read(C.byref(c), A, A, None, None, table, stride, pages, lengths, batch, tokens, k, ks, v, vs, None)
 
     for more in (dict(table=None), dict(lengths=None), dict(k=None), dict(v=None), dict(ks=None), dict(vs=None)):
         _refused(read(**more), "null")
@@ -102,7 +107,7 @@ def test_paged():
         f = dict(batch=1, q_heads=4, table_pages=4, window=0, table_stride=4, q_strides=(256, 64), out_strides=(256, 64), scale=1.0, softcap=0.0)
         f.update(more)
         d = abi.PagedAttentionDesc(*f.values())
-        return lib.onhip_attention_paged(C.byref(c), C.byref(d), q, table, lengths, None, out, ws, nbytes, None)
+        return lib.onhip_attention_paged(C.byref(c), A, A, None, None, C.byref(d), q, table, lengths, None, out, ws, nbytes, None)
 
     for more in (dict(q=None), dict(table=None), dict(lengths=None), dict(out=None)):
         _refused(paged(**more), "null")

@@ -2,17 +2,19 @@
 // over the keys j of [max(0, len - window), len), in one pass over the cache with the running maximum and sum of a softmax.
 //
 // Up to 16 query heads that share a key-value head are the columns of the matrix instructions (v_mfma_f32_16x16x32), so the cache is read
-// once for all of them.  A wavefront takes tiles of 32 keys by itself, with no barrier until its end: S^T = K q^T, whose result leaves a
-// lane with 8 scores of one head; and out^T = V^T P^T, whose second operand is those scores' exponentials where they are.  Both operands of
-// the cache come straight from memory into registers.  K: a lane reads 16 bytes of the row of its key.  V: 16 lanes read a whole row, a
-// lane the channels 8 li .. + 7 (HD 128) of 8 keys, and channel 8 li + t of them is its operand for channel tile t, put together from the
-// halves (or bytes) of those registers, so nothing passes through LDS before the end.
+// once for all of them.  A wavefront takes tiles of 32 or 64 keys by itself, with no barrier until its end: S^T = K q^T, whose result leaves a
+// lane with a quarter of the scores of one head; and out^T = V^T P^T, whose second operand is those scores' exponentials where they are.  Both operands of
+// the cache are read whole rows at a time, 4 to 16 lanes a row.  K turns into operands through the wavefront's own part of LDS (straight into them,
+// a row a lane, cost 64 cycles of a compute unit's address path a load: 2.1 us for 128 KB, and 0.9 now).  V needs no such turn: a lane has the channels 8 li .. + 7
+// (HD 128) of 8 keys, and channel 8 li + t of them is its operand for channel tile t, put together from the halves (or bytes) of those registers.
 //
-// The rows are bound by memory: a byte of the cache takes part in 2 to 16 operations.  A sequence's tiles are shared out among
-// `splits` workgroups of four wavefronts, whose parts a second launch joins, where (sequence, head) pairs alone would leave compute units idle.
+// Bound by memory: a byte of the cache takes part in 2 to 16 operations.  Measured against a large copy's 5.1 TB/s: 32 sequences of 2048 to 4096 keys, 8
+// key-value heads of 128 in bf16, 407 MB in 79 us; 4 of up to 65536 in int8 450 MB in 90 us; one of 65536 in bf16 268 MB in 55 us; one of 777 9.6 us, its chain of
+// trips to memory.  A sequence's tiles are shared out among `splits` workgroups of eight wavefronts, whose parts a second launch joins, where
+// (sequence, head) pairs alone would leave compute units idle.
 //
 // int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
-// probability.  What is rounded to the 16-bit type before the second product is exp(s - max) (times a constant, and the scale), half a step each; scores, maximum,
+// probability.  What is rounded to the 16-bit type before the second product is 2^(s - m) (times a constant, and the scale), half a step each; scores, maximum,
 // sum and products' sums are fp32.
 #include "attention_join.hpp"
 #include "kv_common.hpp"
@@ -42,15 +44,20 @@ __device__ __forceinline__ float capped(float s, float to_cap, float cap2) {
 
 // SMALL: pages of fewer than 16 tokens (a tile then has a page a lane; else two pages, the same for all lanes)
 template <int DT, int HD, bool I8, bool SMALL>
-__global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel(const PagedParams p) {
-    constexpr int TILES = HD / 16, STEPS = HD / 32, NW = 4;
-    constexpr int KW = I8 ? HD / 64 : HD / 32;       // 16-byte loads of a lane's part of a key
+__global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedParams p) {
+    constexpr int TILES = HD / 16, STEPS = HD / 32, NW = 8;
+    constexpr int UNITS = (I8 ? 1 : 2) * HD / 16;     // 16-byte units of a key: 4, 8 or 16 lanes take one
+    constexpr int KT = 32, NS = 8;                    // keys of a tile, scores of a lane
+    constexpr int ROWS = 64 / UNITS, KW = KT / ROWS;  // keys of a load, loads of a tile
     constexpr int VB = (I8 ? 1 : 2) * HD / 16;        // bytes of a lane's part of a value: 4, 8 or 16
     constexpr int VW = VB / 4;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
-    constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 15.0f;
-    __shared__ float s_o[NW][16][HD + 4];
+    constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
+    // a wavefront's tile of keys on its way into operands, in the end the wavefronts' results
+    constexpr int KEY_BYTES = NW * KT * UNITS * 16, OUT_BYTES = NW * 16 * (HD + 4) * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char s_mem[KEY_BYTES > OUT_BYTES ? KEY_BYTES : OUT_BYTES];
     __shared__ float s_m[NW][16], s_l[NW][16];
+    float(*s_o)[16][HD + 4] = reinterpret_cast<float(*)[16][HD + 4]>(s_mem);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
     unsigned id = blockIdx.x;
@@ -65,9 +72,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
     const bool too_long = reach > room;   // more tokens than the table has pages for: the result is NaN
     const int len = too_long ? (int) room : reach;
     const int begin = p.window > 0 && len > p.window ? len - p.window : 0;
-    const int tile0 = begin >> 5, tiles = len > 0 ? ((len + 31) >> 5) - tile0 : 0;
-    // as many parts as there are, each of 128 keys at least
-    const int parts = min(p.splits, (tiles + 3) / 4), per = parts > 0 ? (tiles + parts - 1) / parts : 0;
+    const int tile0 = begin / KT, tiles = len > 0 ? (len + KT - 1) / KT - tile0 : 0;
+    // as many parts as there are, each with a tile for every wavefront
+    const int parts = min(p.splits, (tiles + NW - 1) / NW), per = parts > 0 ? (tiles + parts - 1) / parts : 0;
     const int t_begin = tile0 + split * per, t_end = min(t_begin + per, tile0 + tiles);
 
     const int head = hb * 16 + li;
@@ -99,66 +106,111 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
     const int *table = p.table + b * p.table_stride;
     const char *kb = p.c.k + kvh * p.c.ks[1], *vb = p.c.v + kvh * p.c.vs[1];
 
-    for (int t = t_begin + wave; t < t_end; t += NW) {
-        const int key0 = t * 32;
-        const bool whole = key0 >= begin && key0 + 32 <= len;   // uniform
-        // the pages of the tile's two halves, or of key `lane`
-        int pg[2];
+    const unsigned k_lane = (unsigned) (lane / UNITS) * (unsigned) p.c.ks[2] + lane % UNITS * 16, v_lane = 4u * lg * (unsigned) p.c.vs[2] + li * VB;
+    u32x4 *const mine = reinterpret_cast<u32x4 *>(s_mem) + wave * KT * UNITS;
+    auto unit_at = [](int row, int u) { return row * UNITS + (u ^ (row / (16 / UNITS) & (UNITS - 1))); };   // 16 lanes that take one unit of 16 keys meet every bank once
+
+    // A tile as it is in flight: while one is worked on, the wavefront's next one is on its way, and the pages of the one behind that.
+    struct Tile {
+        u32x4 kr[KW];
+        unsigned vf[NS][VW];
+        float k_scale, v_scale;   // of key `lane` of the tile
+    };
+    struct Pages {   // of the tile's sixteens of keys, or of key `lane`
+        int at[SMALL ? 1 : 2];
+    };
+    auto find = [&](int t, Pages &g) __attribute__((always_inline)) {
+        const int key0 = t * KT;
         if constexpr (SMALL) {
-            const int key = key0 + (lane & 31);
-            int x = key >= begin && key < len ? table[key >> p.c.page_shift] : 0;
-            if ((unsigned) x >= (unsigned) p.c.pages) { bad = true; x = 0; }
-            pg[0] = x;
+            const int key = key0 + (lane & (KT - 1));
+            g.at[0] = key >= begin && key < len ? table[key >> p.c.page_shift] : 0;
         } else {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const int key = key0 + 16 * a;
-                int x = key + 16 > begin && key < len ? table[key >> p.c.page_shift] : 0;
-                if ((unsigned) x >= (unsigned) p.c.pages) { bad = true; x = 0; }
-                pg[a] = __builtin_amdgcn_readfirstlane(x);
+                g.at[a] = key + 16 > begin && key < len ? table[key >> p.c.page_shift] : 0;
             }
         }
-        auto page_of = [&](int in_tile) __attribute__((always_inline)) {   // of key key0 + in_tile
-            if constexpr (SMALL) return __shfl(pg[0], in_tile, 64);
-            else return in_tile < 16 ? pg[0] : pg[1];
-        };
-        // what lies outside [begin, len) is read as well, from rows of pages that exist, and left out below
-        uint4 kf[2][KW];
-        unsigned vf[8][VW];
+    };
+    auto load = [&](int t, const Pages &g, Tile &x) __attribute__((always_inline)) {
+        const int key0 = t * KT;
+        int pg[2];
+        if constexpr (SMALL) {
+            const bool none = (unsigned) g.at[0] >= (unsigned) p.c.pages;
+            bad |= none;
+            pg[0] = none ? 0 : g.at[0];
+        } else {
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const int key = key0 + 16 * a + li;
-            const char *src = kb + (long long) (SMALL ? page_of(16 * a + li) : pg[a]) * p.c.ks[0] + ((key & p.c.page_mask) * (int) p.c.ks[2] + lg * 16);
-#pragma unroll
-            for (int i = 0; i < KW; ++i) kf[a][i] = *reinterpret_cast<const uint4 *>(src + i * 64);
+            for (int a = 0; a < 2; ++a) {
+                const bool none = (unsigned) g.at[a] >= (unsigned) p.c.pages;
+                bad |= none;
+                pg[a] = __builtin_amdgcn_readfirstlane(none ? 0 : g.at[a]);
+            }
         }
+        auto page_of = [&](int in_tile) __attribute__((always_inline)) { return __shfl(pg[0], in_tile, 64); };   // of key key0 + in_tile
+        // what lies outside [begin, len) is read as well, from rows of pages that exist, and left out of the work.  Sixteen keys of a page: a
+        // uniform address and the lane's own offset.
+        const char *half_k[2], *half_v[2];
+        if constexpr (!SMALL)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int at = 16 * (j / 4) + 4 * lg + j % 4, key = key0 + at;
-            const char *src = vb + (long long) (SMALL ? page_of(at) : pg[j / 4]) * p.c.vs[0] + ((key & p.c.page_mask) * (int) p.c.vs[2] + li * VB);
-            if constexpr (VB == 16) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src);
-                vf[j][0] = x.x; vf[j][1] = x.y; vf[j][2] = x.z; vf[j][3] = x.w;
-            } else if constexpr (VB == 8) {
-                const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                vf[j][0] = x.x; vf[j][1] = x.y;
+            for (int a = 0; a < 2; ++a) {
+                half_k[a] = kb + pg[a] * p.c.ks[0] + ((key0 + 16 * a) & p.c.page_mask) * p.c.ks[2];
+                half_v[a] = vb + pg[a] * p.c.vs[0] + ((key0 + 16 * a) & p.c.page_mask) * p.c.vs[2];
+            }
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+            const char *src;
+            if constexpr (SMALL) {
+                const int row = i * ROWS + lane / UNITS;
+                src = kb + page_of(row) * p.c.ks[0] + ((key0 + row) & p.c.page_mask) * (int) p.c.ks[2] + lane % UNITS * 16;
             } else {
-                vf[j][0] = *reinterpret_cast<const unsigned *>(src);
+                src = half_k[i * ROWS / 16] + (i * ROWS % 16) * p.c.ks[2] + k_lane;
+            }
+            x.kr[i] = *reinterpret_cast<const u32x4 *>(src);
+        }
+        if constexpr (I8) {
+            const int page = SMALL || lane % 32 < 16 ? pg[0] : pg[1];
+            const long long at = page * p.c.ss[0] + kvh * p.c.ss[1] + ((key0 + (lane & (KT - 1))) & p.c.page_mask) * p.c.ss[2];
+            x.k_scale = p.c.k_scale[at];
+            x.v_scale = p.c.v_scale[at];
+        }
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const char *src;
+            if constexpr (SMALL) {
+                const int at = 16 * (j / 4) + 4 * lg + j % 4;
+                src = vb + page_of(at) * p.c.vs[0] + ((key0 + at) & p.c.page_mask) * (int) p.c.vs[2] + li * VB;
+            } else {
+                src = half_v[j / 4] + (j % 4) * p.c.vs[2] + v_lane;
+            }
+            if constexpr (VB == 16) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(src);
+                x.vf[j][0] = y.x; x.vf[j][1] = y.y; x.vf[j][2] = y.z; x.vf[j][3] = y.w;
+            } else if constexpr (VB == 8) {
+                const uint2 y = *reinterpret_cast<const uint2 *>(src);
+                x.vf[j][0] = y.x; x.vf[j][1] = y.y;
+            } else {
+                x.vf[j][0] = *reinterpret_cast<const unsigned *>(src);
             }
         }
-        float ksc[8], vsc[8];
-        if constexpr (I8) {   // lanes 0 to 31 fetch the scales of the keys, 32 to 63 those of the values
-            const int at = lane & 31, key = key0 + at;
-            const float *from = lane < 32 ? p.c.k_scale : p.c.v_scale;
-            float x = 0.0f;
-            const int page = SMALL ? pg[0] : at < 16 ? pg[0] : pg[1];
-            x = from[page * p.c.ss[0] + kvh * p.c.ss[1] + (key & p.c.page_mask) * p.c.ss[2]];
-            if (key < begin || key >= len) x = 0.0f;
-            if constexpr (DT == DT_F16) {   // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
-                float y = lane < 32 ? 0.0f : x;
+    };
+    auto work = [&](int t, Tile &tile) __attribute__((always_inline)) {
+        const int key0 = t * KT;
+        const bool whole = key0 >= begin && key0 + KT <= len;   // uniform
+        auto &vf = tile.vf;
 #pragma unroll
-                for (int i = 1; i < 64; i *= 2) y = fmaxf(y, __shfl_xor(y, i, 64));
-                const int e = y > 0.0f && y < INFINITY ? __builtin_amdgcn_frexp_expf(y) : -1000;
+        for (int i = 0; i < KW; ++i) mine[unit_at(i * ROWS + lane / UNITS, lane % UNITS)] = tile.kr[i];
+        float ksc[NS], vsc[NS];
+        if constexpr (I8) {
+            const int key = key0 + (lane & (KT - 1));
+            const bool seen = key >= begin && key < len;
+            const float x = seen ? tile.k_scale : 0.0f;
+            float y = seen ? tile.v_scale : 0.0f;
+            if constexpr (DT == DT_F16) {   // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
+                float most = y;
+#pragma unroll
+                for (int i = 1; i < KT; i *= 2) most = fmaxf(most, __shfl_xor(most, i, 64));
+                const int e = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : -1000;
                 if (e > unit) {   // uniform
 #pragma unroll
                     for (int i = 0; i < TILES; ++i)
@@ -166,34 +218,34 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
                         for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit - e);
                     unit = e;
                 }
-                x = lane < 32 ? x : ldexpf(x, -unit);
+                y = ldexpf(y, -unit);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < NS; ++j) {
                 const int from_lane = 16 * (j / 4) + 4 * lg + j % 4;
-                ksc[j] = __shfl(x, from_lane, 64);
-                vsc[j] = __shfl(x, 32 + from_lane, 64);
+                ksc[j] = __shfl(x * (p.cap2 > 0.0f ? 1.0f : p.scale2), from_lane, 64);
+                vsc[j] = __shfl(y, from_lane, 64);
             }
         }
-
         if (!whole) {   // a value that is not seen may be an infinity, and 0 of it is not 0
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < NS; ++j) {
                 const int key = key0 + 16 * (j / 4) + 4 * lg + j % 4;
 #pragma unroll
                 for (int i = 0; i < VW; ++i) vf[j][i] = key >= begin && key < len ? vf[j][i] : 0u;
             }
         }
 
-        // S^T: this lane's 8 scores are of head li and the keys 16 (j / 4) + 4 lg + j % 4
-        float s[8];
+        // S^T: this lane's scores are of head li and the keys 16 (j / 4) + 4 lg + j % 4
+        float s[NS];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (I8) {
+                u32x4 x;
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
-                    const uint4 &x = kf[a][st / 2];
+                    if (st % 2 == 0) x = mine[unit_at(16 * a + li, st * 2 + lg)];
                     const unsigned two[2] = {st % 2 ? x.z : x.x, st % 2 ? x.w : x.y};
                     unsigned y[4];
                     s8_to_h16<DT, 2>(two, y);
@@ -201,74 +253,99 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
                 }
             } else {
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) acc = mfma(kf[a][st], qf[st], acc);
+                for (int st = 0; st < STEPS; ++st) acc = mfma(__builtin_bit_cast(uint4, mine[unit_at(16 * a + li, st * 4 + lg)]), qf[st], acc);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[4 * a + r] = I8 ? acc[r] * ksc[4 * a + r] : acc[r];
         }
         if (p.cap2 > 0.0f) {   // uniform
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = capped(s[j], p.to_cap, p.cap2);
-        } else {
+            for (int j = 0; j < NS; ++j) s[j] = capped(s[j], p.to_cap, p.cap2);
+        } else if constexpr (!I8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] *= p.scale2;
+            for (int j = 0; j < NS; ++j) s[j] *= p.scale2;
         }
         if (p.slopes) {   // uniform
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = __builtin_fmaf(slope2, (float) (key0 + 16 * (j / 4) + 4 * lg + j % 4 - (len - 1)), s[j]);
+            for (int j = 0; j < NS; ++j) s[j] = __builtin_fmaf(slope2, (float) (key0 + 16 * (j / 4) + 4 * lg + j % 4 - (len - 1)), s[j]);
         }
         if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < NS; ++j) {
                 const int key = key0 + 16 * (j / 4) + 4 * lg + j % 4;
                 if (key < begin || key >= len) s[j] = -INFINITY;
             }
         }
         float top = s[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
+        for (int j = 1; j < NS; ++j) top = fmaxf(top, s[j]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float next = fmaxf(m, top), shift = next == -INFINITY ? 0.0f : next;
-        const float fade = __builtin_amdgcn_exp2f(m - shift);
-        m = next;
-        float e[8];
+        const bool far = top > m + 8.0f;   // the reference point follows a head's maximum when that is 2^8 above it: most tiles leave the sums alone
+        if (__any(far)) {
+            const float next = far ? top : m, fade = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+            m = next;
+            l *= fade;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(s[j] - shift + SHIFT);
-        l *= fade;
+            for (int i = 0; i < TILES; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) l += e[j];
+                for (int r = 0; r < 4; ++r) o[i][r] *= fade;
+        }
+        const float shift = m == -INFINITY ? 0.0f : SHIFT - m;
+        float e[NS];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[i][r] *= fade;
+        for (int j = 0; j < NS; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(s[j] + shift);
+            l += e[j];
+        }
         if constexpr (I8)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] *= vsc[j];
-        const uint4 pf = make_uint4(pack_h16<DT>(e[0], e[1]), pack_h16<DT>(e[2], e[3]), pack_h16<DT>(e[4], e[5]), pack_h16<DT>(e[6], e[7]));
+            for (int j = 0; j < NS; ++j) e[j] *= vsc[j];
         // out^T += V^T P^T: row i of channel tile n is the channel TILES i + n
+        const uint4 pf = make_uint4(pack_h16<DT>(e[0], e[1]), pack_h16<DT>(e[2], e[3]), pack_h16<DT>(e[4], e[5]), pack_h16<DT>(e[6], e[7]));
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
             unsigned a[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int i = 0; i < 4; ++i) {
                 if constexpr (I8) {
-                    const int x = (int) (vf[2 * j][n / 4] >> (n % 4 * 8)), y = (int) (vf[2 * j + 1][n / 4] >> (n % 4 * 8));
-                    a[j] = pack_h16<DT>((float) (signed char) x, (float) (signed char) y);
+                    const int x = (int) (vf[2 * i][n / 4] >> (n % 4 * 8)), y = (int) (vf[2 * i + 1][n / 4] >> (n % 4 * 8));
+                    a[i] = pack_h16<DT>((float) (signed char) x, (float) (signed char) y);
                 } else {
-                    a[j] = __builtin_amdgcn_perm(vf[2 * j + 1][n / 2], vf[2 * j][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
+                    a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][n / 2], vf[2 * i][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
                 }
             }
             o[n] = mfma(make_uint4(a[0], a[1], a[2], a[3]), pf, o[n]);
         }
-    }
+    };
 
+    int t = t_begin + wave;
+    if (t < t_end) {
+        Tile x, y;
+        Pages now, next;
+        const int last = t_end - 1;   // a tile asked for past the last one is the last one again, not worked on
+        find(t, now);
+        find(min(t + NW, last), next);
+        load(t, now, x);
+        for (;;) {
+            find(min(t + 2 * NW, last), now);
+            load(min(t + NW, last), next, y);
+            work(t, x);
+            t += NW;
+            if (t >= t_end) break;
+            find(min(t + 2 * NW, last), next);
+            load(min(t + NW, last), now, x);
+            work(t, y);
+            t += NW;
+            if (t >= t_end) break;
+        }
+    }
     if constexpr (I8 && DT == DT_F16)
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit);
-    // the four wavefronts' parts
+    // the eight wavefronts' parts
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (__any(bad) || too_long) l = NAN;
@@ -276,14 +353,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
         s_m[wave][li] = m;
         s_l[wave][li] = l;
     }
+    __syncthreads();   // the last keys have been read
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int n = 0; n < TILES; n += 4)
             *reinterpret_cast<float4 *>(&s_o[wave][li][(4 * lg + r) * TILES + n]) = make_float4(o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]);
     __syncthreads();
-    constexpr int PER = HD / 16;   // channels of a thread: 16 threads a head
-    const int oh = threadIdx.x / 16, d0 = threadIdx.x % 16 * PER;
+    constexpr int SHARE = 64 * NW / 16, PER = HD / SHARE;   // threads of a head, channels of a thread
+    const int oh = threadIdx.x / SHARE, d0 = threadIdx.x % SHARE * PER;
     if (hb * 16 + oh >= p.group) return;
     float mm = s_m[0][oh];
 #pragma unroll
@@ -304,7 +382,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
     if (p.splits > 1) {
         float *po = p.part_o + ((long long) row * p.splits + split) * HD + d0;
 #pragma unroll
-        for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4 *>(po + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2 *>(po + i) = make_float2(acc[i], acc[i + 1]);
         if (d0 == 0) *reinterpret_cast<float2 *>(p.part_ml + ((long long) row * p.splits + split) * 2) = make_float2(mm, ll);
         return;
     }
@@ -315,32 +393,49 @@ __global__ __launch_bounds__(256, HD == 128 ? 3 : 4) void attention_paged_kernel
         reinterpret_cast<unsigned *>(dst)[i / 2] = pack_h16<DT>(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// ---- the parts of a row joined: four wavefronts a row, a lane HD / 64 channels -------------------------------------------------
+// ---- the parts of a row joined: eight wavefronts a row, a lane HD / 64 channels ------------------------------------------------
+// Bound by its trips to memory: a wavefront asks for eight parts at a time, the first eight before it knows their weights.
 template <int DT, int HD>
-__global__ __launch_bounds__(256) void attention_join_kernel(const JoinParams p) {
-    constexpr int PER = HD / 64, NW = 4;
+__global__ __launch_bounds__(512) void attention_join_kernel(const JoinParams p) {
+    constexpr int PER = HD / 64, NW = 8, AHEAD = 8;
     __shared__ float s_acc[NW][HD], s_l[NW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long row = blockIdx.x;
-    const float *ml = p.ml + row * p.splits * 2, *o = p.o + row * p.splits * HD;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.ml) + row * p.splits;
+    const float *o = p.o + row * p.splits * HD + lane * PER;
+    float part[AHEAD][PER];
+    float2 own[AHEAD];
+    auto ask = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = min(s0 + i * NW, p.splits - 1);
+            own[i] = ml[s];
+#pragma unroll
+            for (int c = 0; c < PER; ++c) part[i][c] = o[(long long) s * HD + c];
+        }
+    };
+    ask(wave);
     float mm = -INFINITY;
-    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[2 * s]);
+    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[s].x);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
     const float shift = mm == -INFINITY ? 0.0f : mm;
     float acc[PER], l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-    for (int s = wave; s < p.splits; s += NW) {
-        const float ls = ml[2 * s + 1], f = __builtin_amdgcn_exp2f(ml[2 * s] - shift);
-        if (ls == 0.0f && f == 0.0f) continue;   // a part without keys (uniform in the wavefront); a NaN stays
-        l = __builtin_fmaf(ls, f, l);
-        if (ls != ls) l = NAN;
+    for (int c = 0; c < PER; ++c) acc[c] = 0.0f;
+    for (int s0 = wave; s0 < p.splits; s0 += AHEAD * NW) {
+        if (s0 != wave) ask(s0);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = __builtin_fmaf(o[(long long) s * HD + lane * PER + i], f, acc[i]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const bool there = s0 + i * NW < p.splits;
+            const float f = there ? __builtin_amdgcn_exp2f(own[i].x - shift) : 0.0f, ls = own[i].y;
+            l += !there || (f == 0.0f && ls == ls) ? 0.0f : ls * f;   // a NaN stays
+#pragma unroll
+            for (int c = 0; c < PER; ++c) acc[c] = f == 0.0f ? acc[c] : __builtin_fmaf(part[i][c], f, acc[c]);   // a part without keys has written nothing
+        }
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s_acc[wave][lane * PER + i] = acc[i];
+    for (int c = 0; c < PER; ++c) s_acc[wave][lane * PER + c] = acc[c];
     if (lane == 0) s_l[wave] = l;
     __syncthreads();
     if (threadIdx.x >= HD / 2) return;
@@ -359,22 +454,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const JoinParams p)
 
 int attention_join_launch(int dt, int hd, const JoinParams &p, hipStream_t stream) {
     const dim3 grid((unsigned) p.rows);
-    if (dt == DT_BF16 && hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 64>), grid, dim3(256), 0, stream, p);
-    else if (dt == DT_BF16) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 128>), grid, dim3(256), 0, stream, p);
-    else if (hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_F16, 64>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attention_join_kernel<DT_F16, 128>), grid, dim3(256), 0, stream, p);
+    if (dt == DT_BF16 && hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 64>), grid, dim3(512), 0, stream, p);
+    else if (dt == DT_BF16) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 128>), grid, dim3(512), 0, stream, p);
+    else if (hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_F16, 64>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((attention_join_kernel<DT_F16, 128>), grid, dim3(512), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
 
-// Workgroups that a sequence's head is cut into: enough for four a compute unit, 256 keys of the longest possible sequence each at least.
+// Workgroups that a sequence's head is cut into: one a compute unit (two were 6 to 50 % behind: 32 sequences of 4096 keys 79 and 85 us, 2 of 30000 with
+// one key-value head 14.6 and 21.8), 256 keys each at least.  Up to 1024 keys one, without a second launch (one sequence of 777 keys 9.6 us, in four
+// parts 9.3 and a launch more to queue).  int8, whose tiles are half the bytes in flight: two a compute unit where each still has 4096 keys
+// (4 of 65536 95 and 90 us; 32 of 4000 49 and 56).
 static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d) {
     const long long group = d->q_heads / c->kv_heads, rows = (long long) d->batch * c->kv_heads * ((group + 15) / 16);
     long long longest = (long long) d->table_pages * c->page_tokens;
     if (d->window > 0 && d->window < longest) longest = d->window;
-    const long long want = (1024 + rows - 1) / rows, most = (longest + 255) / 256;
-    const long long s = want < most ? want : most;
-    return s < 1 ? 1 : s > 256 ? 256 : (int) s;
+    if (longest <= 1024) return 1;
+    long long want = (256 + rows - 1) / rows;
+    if (c->quantised && longest / (2 * want) >= 4096) want *= 2;
+    const long long most = (longest + 255) / 256, s = want < most ? want : most;
+    return s > 256 ? 256 : (int) s;
 }
 
 static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, CacheView *view, int *dt) {
@@ -391,8 +491,8 @@ static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_
 
 template <int DT, int HD, bool I8>
 static int paged_launch(const PagedParams &p, unsigned blocks, hipStream_t stream) {
-    if (p.c.page_shift < 4) hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, true>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, false>), dim3(blocks), dim3(256), 0, stream, p);
+    if (p.c.page_shift < 4) hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, true>), dim3(blocks), dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((attention_paged_kernel<DT, HD, I8, false>), dim3(blocks), dim3(512), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }

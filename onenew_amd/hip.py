@@ -705,13 +705,19 @@ def attention(q, k, v, scale=1.0, out=None, merged_out=True):
 #
 # What a call has to check and to describe depends on types, devices, shapes and strides alone, and a step's calls repeat them: the checked
 # descriptions are kept by those (a call that finds its own takes 8 us of host time, with the checks 15 to 24).  Addresses are passed on each call.
+# The last key of an entry point is compared first: a step calls each with the same shapes layer after layer.
 _plans = {}
+_last = {}
 
 
-def _plan(key, make):
-    if len(_plans) >= 4096:
-        _plans.clear()
-    plan = _plans[key] = make()
+def _plan(what, key, make, *args):
+    plan = _plans.get((what, key))
+    if plan is None:
+        plan = make(*args)
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[what, key] = plan
+    _last[what] = (key, plan)
     return plan
 
 
@@ -719,8 +725,13 @@ def _meta(t):
     return t if t is None else (t.dtype, t.get_device(), t.shape, t.stride())
 
 
+def _flat(t):
+    """_meta of a contiguous array, whose number of elements says as much as its shape"""
+    return t if t is None else (t.dtype, t.get_device(), t.numel(), t.is_contiguous())
+
+
 def _device():
-    """torch's current device, without the checks around it that a tensor on a device has passed"""
+    """torch's current device, without torch.cuda.current_device()'s checks, which a tensor on a device has passed"""
     import torch
     return torch._C._cuda_getDevice()
 
@@ -802,13 +813,15 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
     norm of q's and k's heads where there are weights [head_dim] (fp32), rotation by positions [tokens] (int32) times inv_freq [pairs] (fp32)
     where there are frequencies, q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
     [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with fp32 scales [pages, kv_heads, page_tokens]"""
-    import torch
-    key = ("append", _device(), _meta(q), _meta(k), _meta(v), _meta(positions), _meta(slots), _meta(k_cache), _meta(v_cache), _meta(inv_freq),
-           _meta(q_weight), _meta(k_weight), eps, interleaved, _meta(k_scale), _meta(v_scale), _meta(q_out))
-    d, r, shape, empty = _plans.get(key) or _plan(key, lambda: _append_plan(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_weight, k_weight, eps,
-                                                                            interleaved, k_scale, v_scale, q_out))
+    key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
+           positions.dtype, positions.get_device(), positions.numel(), positions.is_contiguous(), slots.dtype, slots.get_device(), slots.numel(), slots.is_contiguous(),
+           k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
+           _flat(inv_freq), _flat(q_weight), _flat(k_weight), eps, interleaved, _meta(k_scale), _meta(v_scale), _meta(q_out))
+    last = _last.get("append")
+    d, r, shape, empty = last[1] if last is not None and last[0] == key else _plan(
+        "append", key, _append_plan, q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_weight, k_weight, eps, interleaved, k_scale, v_scale, q_out)
     if q_out is None:
-        q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        q_out = q.new_empty(shape)
     if not empty:
         _check(load().onhip_cache_append(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), r, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                          positions.data_ptr(), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream()),
@@ -839,24 +852,26 @@ def _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype
 def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
     """rows 0 .. tokens - 1 of every sequence (pages table [sequences, pages], lengths [sequences], int32), zeros behind its length: k and v
     [sequences, kv_heads, tokens, head_dim] in the cache's 16-bit type, or `dtype` for an int8 cache"""
-    import torch
     dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
-    key = ("read", _device(), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), tokens, _meta(k_scale), _meta(v_scale), dtype, _meta(k_out), _meta(v_out))
-    d, shape, step, pages, ks, vs, empty = _plans.get(key) or _plan(key, lambda: _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype, k_out, v_out))
+    key = (_device(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
+           table.dtype, table.get_device(), table.shape, table.stride(), lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(),
+           tokens, _meta(k_scale), _meta(v_scale), dtype, _meta(k_out), _meta(v_out))
+    last = _last.get("read")
+    d, shape, step, pages, ks, vs, empty = last[1] if last is not None and last[0] == key else _plan(
+        "read", key, _read_plan, k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype, k_out, v_out)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+        k_out = k_cache.new_empty(shape, dtype=dtype)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=k_cache.device)
+        v_out = k_cache.new_empty(shape, dtype=dtype)
     if not empty:
         _check(load().onhip_cache_read(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), step, pages, lengths.data_ptr(),
                                        shape[0], tokens, k_out.data_ptr(), ks, v_out.data_ptr(), vs, _stream()), "onhip_cache_read")
     return k_out, v_out
 
 
-def _workspace(nbytes, device):
-    """of one call alone, from torch's allocator: ordered on the stream, private to a graph that is being captured"""
-    import torch
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _workspace(nbytes, like):
+    """16-bit words of one call alone, from torch's allocator: ordered on the stream, private to a graph that is being captured"""
+    return like.new_empty(nbytes // 2)
 
 
 def _paged_plan(q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale, v_scale, out):
@@ -878,15 +893,16 @@ def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, so
     """attention of one new token a sequence, q [sequences, q_heads, head_dim], over the cache's rows table [sequences, pages] / lengths
     [sequences] (int32; the new token's row is the last): scores capped to softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the
     distance, the last `window` rows alone where it is above zero; returns [sequences, q_heads, head_dim]"""
-    import torch
-    key = ("paged", _device(), _meta(q), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), scale, window, softcap, _meta(slopes), _meta(k_scale),
-           _meta(v_scale), _meta(out))
-    c, d, shape, nbytes, empty = _plans.get(key) or _plan(key, lambda: _paged_plan(q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale,
-                                                                                   v_scale, out))
+    key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(),
+           v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(), table.dtype, table.get_device(), table.shape, table.stride(),
+           lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(), scale, window, softcap, _flat(slopes), _meta(k_scale), _meta(v_scale), _meta(out))
+    last = _last.get("paged")
+    c, d, shape, nbytes, empty = last[1] if last is not None and last[0] == key else _plan(
+        "paged", key, _paged_plan, q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale, v_scale, out)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     if not empty:
-        ws = _workspace(nbytes, q.device) if nbytes else None
+        ws = _workspace(nbytes, q) if nbytes else None
         _check(load().onhip_attention_paged(c, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), d, q.data_ptr(), table.data_ptr(),
                                             lengths.data_ptr(), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()), "onhip_attention_paged")
     return out
@@ -922,13 +938,15 @@ def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, sl
     softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the distance.  Returns [batch, q_tokens, q_heads * head_dim] (heads merged) or,
     with merged_out=False, [batch, q_heads, q_tokens, head_dim]; `out` may be such a tensor (merged: with a pitch above q_heads * head_dim).  Rows
     that see nothing are zeros"""
-    import torch
-    key = ("masked", _device(), _meta(q), _meta(k), _meta(v), scale, causal, window, softcap, _meta(slopes), _meta(ranges), q_offset, _meta(out), merged_out)
-    d, shape, nbytes, empty = _plans.get(key) or _plan(key, lambda: _masked_plan(q, k, v, scale, causal, window, softcap, slopes, ranges, q_offset, out, merged_out))
+    key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
+           scale, causal, window, softcap, _flat(slopes), _meta(ranges), q_offset, _meta(out), merged_out)
+    last = _last.get("masked")
+    d, shape, nbytes, empty = last[1] if last is not None and last[0] == key else _plan(
+        "masked", key, _masked_plan, q, k, v, scale, causal, window, softcap, slopes, ranges, q_offset, out, merged_out)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     if not empty:
-        ws = _workspace(nbytes, q.device) if nbytes else None
+        ws = _workspace(nbytes, q) if nbytes else None
         _check(load().onhip_attention_masked(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()),
                "onhip_attention_masked")
     return out

@@ -11,8 +11,13 @@
 // probabilities feed out^T = v^T P^T from the registers they are in.  Tiles of 64 keys of k and v go through LDS in two buffers, v
 // transposed on its way out by the transposing read.
 //
-// Rounded to the 16-bit type before the second product: 2^(s - m) times a constant, at most 2^8 of it (the reference point m follows the maximum when that is 2^8
-// above it, so that most tiles leave the sums alone).  Scores, maxima, sums and products' sums are fp32.
+// Rounded to the 16-bit type before the second product: 2^(s - m) times a constant, at most 2^8 of it (the reference point m follows a row's maximum when that is
+// 2^8 above it, so that most tiles leave the sums alone).  Scores, maxima, sums and products' sums are fp32.
+//
+// What bounds it: the matrix instructions and the vector instructions of the softmax, half of the cycles each, at a clock that falls under them (1.74 GHz): 8192
+// causal tokens of 32 heads of 128 on 8 in bf16 551 us, 1.0 PFLOP/s where a large library product reaches 1.2.  Capped scores add a third to the
+// vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 104 us.  Short rows are bound by a workgroup's chain of trips to
+// memory: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 46 us (their 67 MB take 13).
 #include "attention_join.hpp"
 
 namespace onhip {
@@ -25,8 +30,10 @@ struct MaskedParams {
     const float *slopes;
     int batch, q_heads, kv_heads, group, q_tokens, k_tokens, q_offset, causal, window;
     int blocks, splits;                     // row blocks of a key-value head; parts of the keys
+    Div31 by_splits, by_heads, by_kv_heads, by_group;
     int spread;                             // the (batch, key-value head) pairs divide evenly among the XCDs
-    float scale2, cap2, to_cap;             // |scale| * log2(e); cap * log2(e); scale / cap * 2 log2(e)
+    float scale2, cap2, to_cap, to_x;       // |scale| * log2(e); cap * log2(e); |scale| / cap * 2 log2(e); |scale| / cap
+    float tanh0, tanh1, tanh2, tanh3;       // cap2 times the coefficients of tanh(x) / x in x^2
     unsigned flip;                          // sign of the scale on q
     float *part_o, *part_ml;
 };
@@ -49,91 +56,102 @@ template <int DT> __device__ __forceinline__ unsigned finite_of(unsigned w) {
 }
 
 // GENERAL: scores are capped or biased, or the scale is zero (else one fused product takes them into the exponential)
-template <int DT, int HD, bool GENERAL>
-__global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedParams p) {
-    constexpr int KT = 64, NT = KT / 32, STEPS = HD / 16, DTILES = HD / 32;
+// RG: groups of 32 rows of a workgroup.  4: a wavefront has all keys of a tile for its rows.  2: two wavefronts share the rows, one has the first 32 keys of
+// every tile, one the others, and their results are joined in the end.
+template <int DT, int HD, bool GENERAL, int RG>
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel(const MaskedParams p) {
+    constexpr int KT = 64, NT = RG == 4 ? 2 : 1, STEPS = HD / 16, DTILES = HD / 32;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
     constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
     constexpr int UNITS = HD / 8, ROWS = 64 / UNITS;           // 16-byte units of a row; rows that a wavefront's load covers
     constexpr int LOADS = KT / ROWS / 4;                       // loads of a wavefront for its share of a tile of k (or v)
-    __shared__ uint4 Ks[2][KT * UNITS];
-    __shared__ __attribute__((aligned(16))) unsigned short Vs[2][KT * HD];
-    __shared__ int s_lo[4], s_hi[4], s_all_lo[4], s_all_hi[4], s_odd;
+    __shared__ uint4 s_kv[4][KT * UNITS];   // two tiles of k, two of v
+    uint4(*const Ks)[KT * UNITS] = s_kv;
+    unsigned short(*const Vs)[KT * HD] = reinterpret_cast<unsigned short(*)[KT * HD]>(s_kv[2]);
+    __shared__ int4 s_span[4];
+    __shared__ int s_odd;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 31, lh = lane >> 5;
+    const int li = lane & 31, lh = lane >> 5, rg = RG == 4 ? wave : wave >> 1, kh = RG == 4 ? 0 : wave & 1;
     // item -> (batch, key-value head, row block, part).  Workgroups go to the XCDs in turn; where the heads divide among them, an XCD has whole
-    // heads, so that its L2 holds their keys.  The last row blocks, which see most keys under a causal mask, start first.
-    unsigned id = blockIdx.x;
+    // heads, so that its L2 holds their keys.  The last row blocks, which see most keys under a causal mask, start first; where all items find room at
+    // once, a compute unit's second one is from the other end, so that its two (or three) together are no longer than another's.
     int bh, block, split;
     {
         const unsigned pairs = (unsigned) (p.batch * p.kv_heads);
-        unsigned local = id, heads = pairs, first = 0;
+        unsigned local = blockIdx.x, heads = pairs, first = 0, units = 256u;
         if (p.spread) {
             heads = pairs / 8u;
-            first = (id & 7u) * heads;
-            local = id >> 3;
+            first = (blockIdx.x & 7u) * heads;
+            local = blockIdx.x >> 3;
+            units = 32u;
         }
-        split = (int) (local % (unsigned) p.splits);
-        local /= (unsigned) p.splits;
-        bh = (int) (first + local % heads);
-        block = p.blocks - 1 - (int) (local / heads);
+        const unsigned items = heads * (unsigned) (p.blocks * p.splits);
+        if (items <= units * (HD == 64 ? 3u : 2u) && local >= units) local = local < 2u * units ? items - 1u - (local - units) : local - units;
+        const unsigned per_split = div31(local, p.by_splits);
+        split = (int) (local - per_split * (unsigned) p.splits);
+        const unsigned from_end = div31(per_split, p.by_heads);
+        bh = (int) (first + per_split - from_end * heads);
+        block = p.blocks - 1 - (int) from_end;
     }
-    const int b = bh / p.kv_heads, kvh = bh - b * p.kv_heads;
+    const int b = (int) div31((unsigned) bh, p.by_kv_heads), kvh = bh - b * p.kv_heads;
 
-    // this lane's row
-    const long long rows = (long long) p.q_tokens * p.group;
-    const long long r0 = (long long) block * 128 + wave * 32 + li;
-    const bool live = r0 < rows;
-    const int token = (int) ((live ? r0 : rows - 1) / p.group), head = kvh * p.group + (int) ((live ? r0 : rows - 1) - (long long) token * p.group);
+    // rows past the last one are the last one again, and not stored
+    const unsigned last_row = (unsigned) p.q_tokens * (unsigned) p.group - 1u, row0 = (unsigned) (block * (32 * RG) + rg * 32);
+    const unsigned own_row = min(row0 + (unsigned) li, last_row);
+    int token = (int) div31(own_row, p.by_group), head = kvh * p.group + (int) (own_row - (unsigned) token * (unsigned) p.group);
     const int place = token + p.q_offset;
-    int lo = 0, hi = p.k_tokens;
-    if (p.causal) hi = min(hi, place + 1);
-    if (p.window > 0) lo = max(lo, place - p.window + 1);
-    if (p.ranges) {
-        const int2 rg = reinterpret_cast<const int2 *>(p.ranges)[(long long) b * p.q_tokens + token];
-        lo = max(lo, rg.x);
-        hi = min(hi, rg.y);
-    }
-    if (lo >= hi) lo = hi = 0;   // sees nothing
-    // of the wavefront: the union and the intersection of its rows' intervals (a row past the last one repeats it)
-    int any_lo = lo < hi ? lo : 0x7fffffff, any_hi = hi, all_lo = lo, all_hi = hi;
+    auto first_key = [&](int t) __attribute__((always_inline)) { return p.window > 0 ? max(0, t + p.q_offset - p.window + 1) : 0; };
+    auto end_key = [&](int t) __attribute__((always_inline)) { return p.causal ? min(p.k_tokens, t + p.q_offset + 1) : p.k_tokens; };
+    int lo = first_key(token), hi = end_key(token);
+    // the union and the intersection of the rows' intervals, of the wavefront and of the workgroup (no smaller than the union, no larger than the intersection)
+    int any_lo, any_hi, all_lo, all_hi, wg_lo, wg_hi, wg_all_lo, wg_all_hi;
+    if (p.ranges) {   // uniform
+        const int2 rg2 = reinterpret_cast<const int2 *>(p.ranges)[(long long) b * p.q_tokens + token];
+        lo = max(lo, rg2.x);
+        hi = min(hi, rg2.y);
+        if (lo >= hi) lo = hi = 0;   // sees nothing
+        any_lo = lo < hi ? lo : 0x7fffffff;
+        any_hi = hi;
+        all_lo = lo;
+        all_hi = hi;
 #pragma unroll
-    for (int x = 1; x < 32; x *= 2) {
-        any_lo = min(any_lo, __shfl_xor(any_lo, x, 64));
-        any_hi = max(any_hi, __shfl_xor(any_hi, x, 64));
-        all_lo = max(all_lo, __shfl_xor(all_lo, x, 64));
-        all_hi = min(all_hi, __shfl_xor(all_hi, x, 64));
-    }
-    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
-    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    if (lane == 0) {
-        s_lo[wave] = any_lo;
-        s_hi[wave] = any_hi;
-        s_all_lo[wave] = all_lo;
-        s_all_hi[wave] = all_hi;
+        for (int x = 1; x < 32; x *= 2) {
+            any_lo = min(any_lo, __shfl_xor(any_lo, x, 64));
+            any_hi = max(any_hi, __shfl_xor(any_hi, x, 64));
+            all_lo = max(all_lo, __shfl_xor(all_lo, x, 64));
+            all_hi = min(all_hi, __shfl_xor(all_hi, x, 64));
+        }
+        any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+        any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        if (lane == 0) s_span[wave] = make_int4(any_lo, any_hi, all_lo, all_hi);
+        __syncthreads();
+        const int4 x = s_span[0], y = s_span[1], z = s_span[2], w = s_span[3];
+        wg_lo = __builtin_amdgcn_readfirstlane(min(min(x.x, y.x), min(z.x, w.x)));
+        wg_hi = __builtin_amdgcn_readfirstlane(max(max(x.y, y.y), max(z.y, w.y)));
+        wg_all_lo = __builtin_amdgcn_readfirstlane(max(max(x.z, y.z), max(z.z, w.z)));
+        wg_all_hi = __builtin_amdgcn_readfirstlane(min(min(x.w, y.w), min(z.w, w.w)));
+    } else {   // both ends grow with the token: the first row's and the last row's are all there is to know
+        if (lo >= hi) lo = hi = 0;
+        const int t0 = (int) div31(min(row0, last_row), p.by_group), t1 = (int) div31(min(row0 + 31u, last_row), p.by_group);
+        any_lo = first_key(t0);
+        any_hi = end_key(t1);
+        all_lo = first_key(t1);
+        all_hi = end_key(t0);
+        const unsigned wg_row = (unsigned) (block * (32 * RG));
+        const int w0 = (int) div31(wg_row, p.by_group), w1 = (int) div31(min(wg_row + 32u * RG - 1u, last_row), p.by_group);
+        wg_lo = first_key(w0);
+        wg_hi = end_key(w1);
+        wg_all_lo = first_key(w1);
+        wg_all_hi = end_key(w0);
     }
     if (tid == 0) s_odd = 0;
-    // q: the channels 16 s + 8 (lane / 32) .. + 7 of step s
-    uint4 qf[STEPS];
-    {
-        const unsigned short *src = p.q + b * p.qs[0] + head * p.qs[1] + token * p.qs[2] + lh * 8;
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(src + st * 16);
-            qf[st] = make_uint4(x.x ^ p.flip, x.y ^ p.flip, x.z ^ p.flip, x.w ^ p.flip);
-        }
-    }
-    __syncthreads();
-    const int wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-    const int wg_all_lo = __builtin_amdgcn_readfirstlane(max(max(s_all_lo[0], s_all_lo[1]), max(s_all_lo[2], s_all_lo[3])));
-    const int wg_all_hi = __builtin_amdgcn_readfirstlane(min(min(s_all_hi[0], s_all_hi[1]), min(s_all_hi[2], s_all_hi[3])));
-    int t_begin = __builtin_amdgcn_readfirstlane(wg_lo / KT), t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
-    if (wg_hi <= 0) t_begin = t_end = 0;
+    int t_begin = wg_lo / KT, t_end = wg_hi > 0 ? (wg_hi + KT - 1) / KT : 0;
+    t_begin = min(t_begin, t_end);   // no key at all: no tile
     if (p.splits > 1) {
-        const int per = (t_end - t_begin + p.splits - 1) / p.splits;
+        const int per = (int) div31((unsigned) (t_end - t_begin + p.splits - 1), p.by_splits);
         t_begin = min(t_end, t_begin + split * per);
         t_end = min(t_end, t_begin + per);
     }
@@ -203,6 +221,24 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
         return make_uint4(x.x, x.y, y.x, y.y);
     };
 
+    if (t_begin < t_end) fetch(t_begin);
+    // q: whole rows from memory, through the wavefront's part of the second buffers into the channels 16 s + 8 (lane / 32) .. + 7 of step s (a row a
+    // lane, each load keeps a compute unit's address path busy for 64 cycles)
+    uint4 qf[STEPS];
+    {
+        uint4 *const rows = s_kv[1 + (wave & 2)] + (wave & 1) * 32 * UNITS;
+        uint4 x[32 / ROWS];
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i) {
+            const unsigned row = min(row0 + (unsigned) (i * ROWS + lane / UNITS), last_row), tk = div31(row, p.by_group);
+            x[i] = *reinterpret_cast<const uint4 *>(p.q + b * p.qs[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.qs[1] + tk * p.qs[2] + lane % UNITS * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i)
+            rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)] = make_uint4(x[i].x ^ p.flip, x[i].y ^ p.flip, x[i].z ^ p.flip, x[i].w ^ p.flip);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) qf[st] = rows[k_unit(li, 2 * st + lh)];
+    }
     f32x16 o[DTILES];
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
@@ -212,38 +248,74 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
     const float slope2 = GENERAL && p.slopes ? p.slopes[head] * 1.44269504088896340736f : 0.0f;
 
     auto tile = [&](int t, int buf) __attribute__((always_inline)) {
-        const int key0 = t * KT;
-        if (key0 >= any_hi || key0 + KT <= any_lo) return;   // uniform: none of the wavefront's rows sees the tile
-        const bool whole = key0 >= all_lo && key0 + KT <= all_hi;
+        const int key0 = t * KT + 32 * kh;   // the wavefront's part of the tile: 32 NT keys
+        if (key0 >= any_hi || key0 + 32 * NT <= any_lo) return;   // uniform: none of the wavefront's rows sees it
+        const bool whole = key0 >= all_lo && key0 + 32 * NT <= all_hi;
+        // The order of a tile's instructions is kept as it stands here: operands AHEAD products before their use (the compiler, short of registers, asks for
+        // each where it needs it)
+        constexpr int AHEAD = 4;
         f32x16 s[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
+        auto k_frag = [&](int i) __attribute__((always_inline)) { return Ks[buf][k_unit(32 * (i / STEPS + kh) + li, 2 * (i % STEPS) + lh)]; };
+        uint4 ring[AHEAD];
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) s[n] = mfma(Ks[buf][k_unit(32 * n + li, 2 * st + lh)], qf[st], s[n]);
+        for (int i = 0; i < AHEAD; ++i) ring[i] = k_frag(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NT * STEPS; ++i) {
+            s[i / STEPS] = mfma(ring[i % AHEAD], qf[i % STEPS], s[i / STEPS]);
+            if (i + AHEAD < NT * STEPS) ring[i % AHEAD] = k_frag(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (GENERAL) {
             if (p.cap2 > 0.0f) {   // uniform
+                float most = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {   // tanh(x) = 1 - 2 / (e^2x + 1)
-                        const float e = __builtin_amdgcn_exp2f(s[n][r] * p.to_cap);
-                        s[n][r] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(e + 1.0f);
-                    }
+                    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[n][r]));
+                if (!__any(most * p.to_x > 0.5f)) {
+                    // where all scores are below half of the cap, as most are: tanh(x) = x P(x^2), P of degree 3 fitted to the smallest largest error up to
+                    // 0.5, 1.6 10^-7 in fp32; 24 cycles a score and not the 44 of an exponential and a reciprocal
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float x = s[n][r] * p.to_x, y = x * x;
+                            s[n][r] = x * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p.tanh3, y, p.tanh2), y, p.tanh1), y, p.tanh0);
+                        }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {   // tanh(x) = 1 - 2 / (e^2x + 1)
+                            const float e = __builtin_amdgcn_exp2f(s[n][r] * p.to_cap);
+                            s[n][r] = __builtin_fmaf(-2.0f * p.cap2, __builtin_amdgcn_rcpf(e + 1.0f), p.cap2);
+                        }
+                }
+            }
+            const float mul = p.cap2 > 0.0f ? 1.0f : p.scale2;
+            const float away = (float) (place - key0 - 4 * lh);   // of the lane's first key; the others follow at constant distances
+            if (!p.slopes) {   // uniform
+                if (!(p.cap2 > 0.0f))
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[n][r] *= mul;
+            } else if (p.causal) {   // the keys that count lie behind: the distance has no sign to lose
+                const float base = -slope2 * away;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], mul, __builtin_fmaf(slope2, (float) (32 * n + 8 * (r / 4) + r % 4), base));
             } else {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][r] *= p.scale2;
-            }
-            if (p.slopes) {   // uniform
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[n][r] = __builtin_fmaf(-slope2, fabsf((float) (place - (key0 + 32 * n + 8 * (r / 4) + 4 * lh + r % 4))), s[n][r]);
+                    for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], mul, -slope2 * fabsf(away - (float) (32 * n + 8 * (r / 4) + r % 4)));
             }
         }
         if (!whole) {
@@ -272,30 +344,36 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         const float shift = m == -INFINITY ? 0.0f : SHIFT - m;
+        constexpr int PRODUCTS = 2 * DTILES;   // of 32 keys
+        auto v_ask = [&](int i) __attribute__((always_inline)) { return v_frag(buf, i / PRODUCTS + kh, i % PRODUCTS / DTILES, i % DTILES); };
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < AHEAD; ++i) ring[i] = v_ask(i);
+        __builtin_amdgcn_sched_barrier(0);
+        unsigned pk[NT][8];
+        auto weigh = [&](int n, int j) __attribute__((always_inline)) {   // two probabilities
+            const float x = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j] + shift : __builtin_fmaf(s[n][2 * j], p.scale2, shift));
+            const float y = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j + 1] + shift : __builtin_fmaf(s[n][2 * j + 1], p.scale2, shift));
+            l += x;
+            l += y;
+            pk[n][j] = pack_h16<DT>(x, y);
+        };
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[n][r] = __builtin_amdgcn_exp2f(GENERAL ? s[n][r] + shift : __builtin_fmaf(s[n][r], p.scale2, shift));
-                l += s[n][r];
-            }
-        uint4 pf[NT][2];
+        for (int j = 0; j < 8; ++j) weigh(0, j);
+        __builtin_amdgcn_sched_barrier(0);
+        // the second 32 keys' probabilities between the first ones' products
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < NT * PRODUCTS; ++i) {
+            const int n = i / PRODUCTS, g = i % PRODUCTS / DTILES, d = i % DTILES;
+            o[d] = mfma(ring[i % AHEAD], make_uint4(pk[n][4 * g], pk[n][4 * g + 1], pk[n][4 * g + 2], pk[n][4 * g + 3]), o[d]);
+            if (i + AHEAD < NT * PRODUCTS) ring[i % AHEAD] = v_ask(i + AHEAD);
+            if (NT == 2 && n == 0)
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-                pf[n][g] = make_uint4(pack_h16<DT>(s[n][8 * g], s[n][8 * g + 1]), pack_h16<DT>(s[n][8 * g + 2], s[n][8 * g + 3]),
-                                      pack_h16<DT>(s[n][8 * g + 4], s[n][8 * g + 5]), pack_h16<DT>(s[n][8 * g + 6], s[n][8 * g + 7]));
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int d = 0; d < DTILES; ++d) o[d] = mfma(v_frag(buf, n, g, d), pf[n][g], o[d]);
+                for (int j = 0; j < 8 / PRODUCTS; ++j) weigh(1, i * (8 / PRODUCTS) + j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     if (t_begin < t_end) {
-        fetch(t_begin);
         put(0, mixed(t_begin));
         if (t_begin + 1 < t_end) fetch(t_begin + 1);
         for (int t = t_begin; t < t_end; ++t) {
@@ -309,6 +387,30 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
 
     if (__any(odd != 0u) && lane == 0) s_odd = 1;
     __syncthreads();
+    l += __shfl_xor(l, 32, 64);
+    if constexpr (RG == 2) {   // the two halves of the keys: the second wavefront's results to the first
+        float *const half = reinterpret_cast<float *>(s_kv) + rg * (DTILES * 16 + 2) * 64 + lane;
+        static_assert(2 * (DTILES * 16 + 2) * 64 * 4 <= sizeof(s_kv), "room for two row groups");
+        if (kh) {
+            half[0] = m;
+            half[64] = l;
+#pragma unroll
+            for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) half[(2 + d * 16 + r) * 64] = o[d][r];
+        }
+        __syncthreads();
+        if (!kh) {
+            const float other = half[0], next = fmaxf(m, other), ref = next == -INFINITY ? 0.0f : next;
+            const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(other - ref);
+            m = next;
+            l = l * f0 + half[64] * f1;
+#pragma unroll
+            for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f0 + half[(2 + d * 16 + r) * 64] * f1;
+        }
+    }
     if (s_odd) {   // uniform and rare: for infinities of either sign and NaN, how many of a channel a row sees
         constexpr unsigned ONE = DT == DT_BF16 ? 0x3f80u : 0x3c00u;
         const unsigned span = (unsigned) (hi - lo);
@@ -327,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
                     put(0, false);
                     __syncthreads();
 #pragma unroll 1
-                    for (int i = 0; i < 2 * NT; ++i) {
+                    for (int i = 0; i < KT / 16; ++i) {
                         unsigned seen[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -343,11 +445,17 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] += z[r] > 0.0f ? value : 0.0f;
             }
+        __syncthreads();
     }
 
-    l += __shfl_xor(l, 32, 64);
-    if (!live) return;
+    if (kh) return;
     if (p.splits > 1) {
+        unsigned again = row0;   // the row's token and head anew, not kept through the loop
+        asm volatile("" : "+s"(again));
+        again += (unsigned) li;
+        if (again > last_row) return;
+        token = (int) div31(again, p.by_group);
+        head = kvh * p.group + (int) (again - (unsigned) token * (unsigned) p.group);
         const long long row = ((long long) b * p.q_heads + head) * p.q_tokens + token;
         if (lh == 0) *reinterpret_cast<float2 *>(p.part_ml + (row * p.splits + split) * 2) = make_float2(m, l);
         if (t_begin >= t_end) return;
@@ -359,28 +467,37 @@ __global__ __launch_bounds__(256, 2) void attention_masked_kernel(const MaskedPa
                 *reinterpret_cast<float4 *>(po + 32 * d + 8 * g + 4 * lh) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
         return;
     }
+    // the result as q came, through LDS: whole rows to memory (in the place of k, or behind what the halves of the keys were joined from)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    unsigned short *dst = p.out + b * p.os[0] + head * p.os[1] + token * p.os[2];
+    uint4 *const rows = s_kv[0] + (RG == 4 ? 0 : 160 * UNITS) + rg * 32 * UNITS;
+    static_assert(RG == 4 || 2 * (DTILES * 16 + 2) * 64 * 4 <= 160 * UNITS * 16, "the halves end before the rows");
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint2 *>(dst + 32 * d + 8 * g + 4 * lh) =
+            reinterpret_cast<uint2 *>(rows + k_unit(li, 4 * d + g))[lh] =
                 make_uint2(pack_h16<DT>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), pack_h16<DT>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+#pragma unroll
+    for (int i = 0; i < 32 / ROWS; ++i) {
+        const unsigned row = row0 + (unsigned) (i * ROWS + lane / UNITS), tk = div31(min(row, last_row), p.by_group);
+        const uint4 x = rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)];
+        if (row <= last_row)
+            *reinterpret_cast<uint4 *>(p.out + b * p.os[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.os[1] + tk * p.os[2] + lane % UNITS * 8) = x;
+    }
 }
 
-// Parts of the keys: where row blocks alone leave compute units without work, 512 keys a part at least.
+// Parts of the keys: where row blocks alone leave compute units without work, 256 keys a part at least (one token of 32 heads on 4096 keys 13.5 us, with
+// 512 keys a part 17).
 static int masked_splits(const onhip_masked_attention_desc_t *d, long long blocks) {
     const long long all = blocks * d->batch * d->kv_heads;
-    const long long want = (512 + all - 1) / all;
+    if (all >= 256) return 1;
     long long keys = d->k_tokens;
     if (d->window > 0 && d->window + 128LL < keys) keys = d->window + 128LL;
-    const long long most = (keys + 511) / 512;
-    const long long s = all >= 256 ? 1 : want < most ? want : most;
+    const long long want = (512 + all - 1) / all, most = (keys + 255) / 256, s = want < most ? want : most;
     return s < 1 ? 1 : s > 256 ? 256 : (int) s;
 }
 
-static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *blocks, int *splits) {
+static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg, int *blocks, int *splits) {
     constexpr int MOST = 1 << 29;
     if (!d || d->batch < 1 || d->q_heads < 1 || d->kv_heads < 1 || d->q_tokens < 1 || d->k_tokens < 1) return set_error(ONHIP_ERR_ARG, "masked attention: bad shape");
     if (d->compute == ONHIP_COMPUTE_BF16) *dt = DT_BF16;
@@ -391,7 +508,11 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *bl
     if (d->k_tokens > MOST || d->q_tokens > MOST || d->q_offset > MOST || d->q_offset < -MOST) return set_error(ONHIP_ERR_ARG, "masked attention: lengths and places are at most 2^29");
     if (d->window < 0 || d->window > MOST) return set_error(ONHIP_ERR_ARG, "masked attention: a window of %d", d->window);
     if (!(d->softcap >= 0.0f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.0f)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be finite, the cap not negative");
-    const long long n = ((long long) d->q_tokens * (d->q_heads / d->kv_heads) + 127) / 128;
+    // 64 rows a workgroup where 128 give no more than one a compute unit (4096 causal tokens of 8 heads on one 91 -> 72 us, 2048 of 16 heads of 64 34.5 -> 27,
+    // 77 of 12 7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us)
+    const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads);
+    *rg = (total + 127) / 128 * d->batch * d->kv_heads <= 256 ? 2 : 4;
+    const long long n = (total + 32 * *rg - 1) / (32 * *rg);
     if (n * d->batch * d->kv_heads >= (1LL << 22) || (long long) d->batch * d->q_heads * d->q_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
     *blocks = (int) n;
     *splits = masked_splits(d, n);
@@ -399,10 +520,12 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *bl
 }
 
 template <int DT, int HD>
-static int masked_launch(const MaskedParams &p, bool general, hipStream_t stream) {
+static int masked_launch(const MaskedParams &p, int rg, bool general, hipStream_t stream) {
     const dim3 grid((unsigned) p.batch * p.kv_heads * p.blocks * p.splits);
-    if (general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false>), grid, dim3(256), 0, stream, p);
+    if (rg == 2 && general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true, 2>), grid, dim3(256), 0, stream, p);
+    else if (rg == 2) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false, 2>), grid, dim3(256), 0, stream, p);
+    else if (general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true, 4>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false, 4>), grid, dim3(256), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
@@ -414,16 +537,16 @@ using namespace onhip;
 extern "C" {
 
 size_t onhip_attention_masked_workspace(const onhip_masked_attention_desc_t *d) {
-    int dt, blocks, splits;
-    if (masked_check(d, &dt, &blocks, &splits)) return 0;
+    int dt, rg, blocks, splits;
+    if (masked_check(d, &dt, &rg, &blocks, &splits)) return 0;
     return join_bytes((long long) d->batch * d->q_heads * d->q_tokens, splits, d->head_dim);
 }
 
 int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q, const void *k, const void *v, const int32_t *ranges,
                            const float *slopes, void *out, void *workspace, size_t workspace_bytes, void *stream) {
     MaskedParams p;
-    int dt;
-    const int rc = masked_check(d, &dt, &p.blocks, &p.splits);
+    int dt, rg;
+    const int rc = masked_check(d, &dt, &rg, &p.blocks, &p.splits);
     if (rc) return rc;
     if (!q || !k || !v || !out) return set_error(ONHIP_ERR_ARG, "masked attention: null tensor pointer");
     if (reinterpret_cast<uintptr_t>(ranges) % 8) return set_error(ONHIP_ERR_ARG, "masked attention: ranges must be 8-byte aligned");
@@ -461,15 +584,21 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     p.causal = d->causal;
     p.window = d->window;
     p.spread = (long long) d->batch * d->kv_heads % 8 == 0;
+    p.by_splits = make_div31((unsigned) p.splits);
+    p.by_heads = make_div31((unsigned) (d->batch * d->kv_heads) / (p.spread ? 8u : 1u));
+    p.by_kv_heads = make_div31((unsigned) d->kv_heads);
+    p.by_group = make_div31((unsigned) p.group);
     p.flip = d->scale < 0.0f ? 0x80008000u : 0u;
     p.scale2 = fabsf(d->scale) * 1.44269504088896340736f;
     p.cap2 = d->softcap * 1.44269504088896340736f;
     p.to_cap = d->softcap > 0.0f ? fabsf(d->scale) / d->softcap * 2.0f * 1.44269504088896340736f : 0.0f;
+    p.to_x = d->softcap > 0.0f ? fabsf(d->scale) / d->softcap : 0.0f;
+    p.tanh0 = p.cap2 * 0.999997675f; p.tanh1 = p.cap2 * -0.333206564f; p.tanh2 = p.cap2 * 0.131451443f; p.tanh3 = p.cap2 * -0.0433724485f;
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * p.splits * d->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const bool general = d->softcap > 0.0f || slopes || p.scale2 == 0.0f;
-    auto by_size = [&]<int DT>() { return d->head_dim == 64 ? masked_launch<DT, 64>(p, general, st) : masked_launch<DT, 128>(p, general, st); };
+    auto by_size = [&]<int DT>() { return d->head_dim == 64 ? masked_launch<DT, 64>(p, rg, general, st) : masked_launch<DT, 128>(p, rg, general, st); };
     const int done = dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
     if (done || p.splits == 1) return done;
     JoinParams j;

@@ -7,8 +7,13 @@
 //
 // A lane has 8 consecutive values of a row (16 bytes in, 16 or 8 out), D / 8 lanes a row, a wavefront four or eight heads of one
 // token at a time.  The angles are the token's alone: a lane forms one, the product and its reduction to a revolution in 64 bits
-// (position 10^6 times a frequency of 1 keeps 2^-31 of a revolution), and the lanes fetch the cosines of their values from each other.  A
-// partner value R elements away comes from the lane R / 8 away as the packed pairs that were loaded.
+// (position 10^6 times a frequency of 1 keeps 2^-31 of a revolution), and the lanes fetch the cosines of their values from each other.  Sums, maxima and
+// the partner values of a full rotation go from lane to lane in the vector pipe (through LDS they and the whole numbers' conversions were
+// 49.9 us of the int8 case below).
+//
+// Bound by memory, and by the vector pipe next to it: 8191 tokens of 32 + 8 + 8 heads of 128 in bf16 201 MB in 41 us with norms and a full rotation, 38 without
+// norms (a large copy of as many bytes 40); into an int8 cache 184 MB in 44; a step of 32 tokens 3.3 us, a launch.  Read back: 8 sequences of up to 8192, 8 heads of 128,
+// 377 MB of int8 and its values in 75 us, 480 MB of bf16 in 93.
 #include "kv_common.hpp"
 
 namespace onhip {
@@ -75,16 +80,27 @@ struct AppendParams {
     int waves;       // wavefronts that share a token's heads
 };
 
-// the largest of a value over the LANES lanes of a row
-template <int LANES> __device__ __forceinline__ float row_max(float x) {
-#pragma unroll
-    for (int m = 1; m < LANES; m *= 2) x = fmaxf(x, __shfl_xor(x, m, 64));
-    return x;
+// lane i's value from lane i ^ 1, i ^ 2, 7 - i (of eight) or 15 - i (of sixteen), through the vector pipe
+enum { DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_REVERSE4 = 0x1B, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140, DPP_ROTATE8 = 0x128 };
+template <int HOW> __device__ __forceinline__ unsigned lane_moved(unsigned x) { return (unsigned) __builtin_amdgcn_update_dpp(0, (int) x, HOW, 0xf, 0xf, true); }
+template <int HOW> __device__ __forceinline__ float lane_moved(float x) { return __uint_as_float(lane_moved<HOW>(__float_as_uint(x))); }
+
+// over the LANES lanes of a row: each step joins groups that the last one made equal
+template <int LANES> __device__ __forceinline__ unsigned row_max(unsigned x) {
+    x = max(x, lane_moved<DPP_XOR1>(x));
+    x = max(x, lane_moved<DPP_XOR2>(x));
+    x = max(x, lane_moved<DPP_MIRROR8>(x));
+    return LANES == 16 ? max(x, lane_moved<DPP_MIRROR16>(x)) : x;
 }
 template <int LANES> __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-    for (int m = 1; m < LANES; m *= 2) x += __shfl_xor(x, m, 64);
-    return x;
+    x += lane_moved<DPP_XOR1>(x);
+    x += lane_moved<DPP_XOR2>(x);
+    x += lane_moved<DPP_MIRROR8>(x);
+    return LANES == 16 ? x + lane_moved<DPP_MIRROR16>(x) : x;
+}
+// the value of the lane half a row away
+template <int LANES> __device__ __forceinline__ float row_half(float x) {
+    return LANES == 16 ? lane_moved<DPP_ROTATE8>(x) : lane_moved<DPP_REVERSE4>(lane_moved<DPP_MIRROR8>(x));
 }
 
 // NI: heads that a lane group takes one after the other, all of them asked for before the first is worked on
@@ -165,23 +181,26 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
             if (INTERLEAVED) {
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                    y[j] = x[j] * c8[j] - x[j + 1] * s8[j];
-                    y[j + 1] = x[j + 1] * c8[j] + x[j] * s8[j];
+                    y[j] = __builtin_fmaf(x[j], c8[j], -(x[j + 1] * s8[j]));
+                    y[j + 1] = __builtin_fmaf(x[j + 1], c8[j], x[j] * s8[j]);
                 }
+            } else if (2 * p.pairs == HD) {   // uniform
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[j], c8[j], row_half<LANES>(x[j]) * s8[j]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = x[j] * c8[j] + __shfl(x[j], partner, 64) * s8[j];
+                for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[j], c8[j], __shfl(x[j], partner, 64) * s8[j]);
             }
             if (turned && !is_v)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = y[j];
         }
         const uint4 packed = make_uint4(pack_h16<DT>(x[0], x[1]), pack_h16<DT>(x[2], x[3]), pack_h16<DT>(x[4], x[5]), pack_h16<DT>(x[6], x[7]));
-        float top = 0.0f;
+        unsigned top_bits = 0u;   // of max|x|: as whole numbers, an infinity is above every number and a NaN above that
         if constexpr (I8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]) <= 3.402823466e38f ? fabsf(x[j]) : INFINITY);   // a NaN counts as an infinity
-            top = row_max<LANES>(top);
+            for (int j = 0; j < 8; ++j) top_bits = max(top_bits, __float_as_uint(x[j]) & 0x7fffffffu);
+            top_bits = row_max<LANES>(top_bits);
         }
         if (h >= heads) continue;
         if (is_q) {
@@ -194,15 +213,26 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
         if constexpr (!I8) {
             *reinterpret_cast<uint4 *>(dst + l * 16) = packed;
         } else {
-            // 127 / max leaves fp32's range below 2^-121: such rows are scaled up first, exactly
-            const bool fine = top < INFINITY;
-            const float up = top < 0x1p-100f ? 0x1p100f : 1.0f;
-            const float inv = top > 0.0f && fine ? 127.0f / (top * up) : 0.0f;
+            const bool fine = top_bits < 0x7f800000u;
+            const float top = __uint_as_float(top_bits);
+            // 127 / max leaves fp32's range below 2^-121, and the reciprocal its normal numbers above 2^126: such rows are scaled first, exactly
+            float up = 1.0f;
+            if (__any(top < 0x1p-100f || top > 0x1p100f)) {
+                up = top < 0x1p-100f ? 0x1p100f : top > 0x1p100f ? 0x1p-100f : 1.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= up;
+            }
+            const float inv = top > 0.0f && fine ? 127.0f * __builtin_amdgcn_rcpf(top * up) : 0.0f;   // a unit and a half unit off: a value 1 / 60000 of a step
+            // to the nearest whole number by adding 1.5 2^23, whose sum has it in its lowest byte
             unsigned b[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = fine ? (unsigned) (int) rintf(x[j] * up * inv) & 0xffu : 0u;
-            *reinterpret_cast<uint2 *>(dst + l * 8) = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
-            if (l == 0) (is_v ? p.c.v_scale : p.c.k_scale)[page * p.c.ss[0] + kh * p.c.ss[1] + row * p.c.ss[2]] = fine ? top / 127.0f : NAN;
+            for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(x[j] * inv + 12582912.0f);
+            unsigned q8[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                q8[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * j + 3], b[4 * j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(b[4 * j + 1], b[4 * j], 0x0c0c0400u), 0x05040100u);
+            *reinterpret_cast<uint2 *>(dst + l * 8) = fine ? make_uint2(q8[0], q8[1]) : make_uint2(0u, 0u);
+            if (l == 0) (is_v ? p.c.v_scale : p.c.k_scale)[page * p.c.ss[0] + kh * p.c.ss[1] + row * p.c.ss[2]] = fine ? top * (1.0f / 127.0f) : NAN;
         }
     }
 }

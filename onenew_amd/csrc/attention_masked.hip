@@ -353,9 +353,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         auto weigh = [&](int n, int j) __attribute__((always_inline)) {   // two probabilities
             const float x = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j] + shift : __builtin_fmaf(s[n][2 * j], p.scale2, shift));
             const float y = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j + 1] + shift : __builtin_fmaf(s[n][2 * j + 1], p.scale2, shift));
-            l += x;
-            l += y;
             pk[n][j] = pack_h16<DT>(x, y);
+            // the sum is of the rounded ones: what rounding adds to all of a row's weights is divided out again
+            if constexpr (DT == DT_BF16) l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk[n][j]), bf16x2{(__bf16) 1.0f, (__bf16) 1.0f}, l, false);
+            else l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pk[n][j]), f16x2{(_Float16) 1.0f, (_Float16) 1.0f}, l, false);
         };
 #pragma unroll
         for (int j = 0; j < 8; ++j) weigh(0, j);

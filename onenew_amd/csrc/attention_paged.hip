@@ -14,8 +14,9 @@
 // (sequence, head) pairs alone would leave compute units idle.
 //
 // int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
-// probability.  What is rounded to the 16-bit type before the second product is 2^(s - m) (times a constant, and the scale), half a step each; scores, maximum,
-// sum and products' sums are fp32.
+// probability.  Before the second product 2^(s - m) (times a constant, and the scale) is rounded to fp16 with fp16 and int8 values, half of one of its eleven bits; with
+// bf16's it goes in as two bf16 parts, sixteen bits: the cache's trip leaves the matrix cores time for both.  Scores, maximum, sum and
+// products' sums are fp32.
 #include "attention_join.hpp"
 #include "kv_common.hpp"
 
@@ -52,7 +53,8 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
     constexpr int VB = (I8 ? 1 : 2) * HD / 16;        // bytes of a lane's part of a value: 4, 8 or 16
     constexpr int VW = VB / 4;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
-    constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
+    constexpr int PT = I8 ? DT_F16 : DT;   // type of the second product
+    constexpr float SHIFT = PT == DT_BF16 ? -24.0f : 7.0f;
     // a wavefront's tile of keys on its way into operands, in the end the wavefronts' results
     constexpr int KEY_BYTES = NW * KT * UNITS * 16, OUT_BYTES = NW * 16 * (HD + 4) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char s_mem[KEY_BYTES > OUT_BYTES ? KEY_BYTES : OUT_BYTES];
@@ -90,8 +92,8 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
     }
     const float slope2 = p.slopes && live ? p.slopes[qh] * LOG2E : 0.0f;
 
-    auto mfma = [](const uint4 &x, const uint4 &y, f32x4 c) __attribute__((always_inline)) {
-        if constexpr (DT == DT_BF16)
+    auto mfma = []<int T>(const uint4 &x, const uint4 &y, f32x4 c) __attribute__((always_inline)) {
+        if constexpr (T == DT_BF16)
             return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
         else
             return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
     for (int t = 0; t < TILES; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    int unit = -1000;   // int8 and fp16: o is in units of 2^unit
+    int unit = -1000;   // int8: o is in units of 2^unit
     bool bad = false;
     const int *table = p.table + b * p.table_stride;
     const char *kb = p.c.k + kvh * p.c.ks[1], *vb = p.c.v + kvh * p.c.vs[1];
@@ -206,20 +208,22 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             const bool seen = key >= begin && key < len;
             const float x = seen ? tile.k_scale : 0.0f;
             float y = seen ? tile.v_scale : 0.0f;
-            if constexpr (DT == DT_F16) {   // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
-                float most = y;
+            // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
+            unsigned most = __float_as_uint(y) & 0x7fffffffu;   // as whole numbers, an infinity is above every number and a NaN above that
+            most = max(most, lane_moved<DPP_XOR1>(most));
+            most = max(most, lane_moved<DPP_XOR2>(most));
+            most = max(most, lane_moved<DPP_MIRROR8>(most));
+            most = max(most, lane_moved<DPP_MIRROR16>(most));
+            most = max((unsigned) __builtin_amdgcn_readlane((int) most, 0), (unsigned) __builtin_amdgcn_readlane((int) most, 16));
+            const int e = most != 0u && most < 0x7f800000u ? (int) (most >> 23) - 126 : -1000;
+            if (e > unit) {   // uniform
 #pragma unroll
-                for (int i = 1; i < KT; i *= 2) most = fmaxf(most, __shfl_xor(most, i, 64));
-                const int e = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : -1000;
-                if (e > unit) {   // uniform
+                for (int i = 0; i < TILES; ++i)
 #pragma unroll
-                    for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit - e);
-                    unit = e;
-                }
-                y = ldexpf(y, -unit);
+                    for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit - e);
+                unit = e;
             }
+            y = ldexpf(y, -unit);
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 const int from_lane = 16 * (j / 4) + 4 * lg + j % 4;
@@ -249,11 +253,11 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
                     const unsigned two[2] = {st % 2 ? x.z : x.x, st % 2 ? x.w : x.y};
                     unsigned y[4];
                     s8_to_h16<DT, 2>(two, y);
-                    acc = mfma(make_uint4(y[0], y[1], y[2], y[3]), qf[st], acc);
+                    acc = mfma.template operator()<DT>(make_uint4(y[0], y[1], y[2], y[3]), qf[st], acc);
                 }
             } else {
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) acc = mfma(__builtin_bit_cast(uint4, mine[unit_at(16 * a + li, st * 4 + lg)]), qf[st], acc);
+                for (int st = 0; st < STEPS; ++st) acc = mfma.template operator()<DT>(__builtin_bit_cast(uint4, mine[unit_at(16 * a + li, st * 4 + lg)]), qf[st], acc);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[4 * a + r] = I8 ? acc[r] * ksc[4 * a + r] : acc[r];
@@ -302,7 +306,19 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
             for (int j = 0; j < NS; ++j) e[j] *= vsc[j];
         // out^T += V^T P^T: row i of channel tile n is the channel TILES i + n
-        const uint4 pf = make_uint4(pack_h16<DT>(e[0], e[1]), pack_h16<DT>(e[2], e[3]), pack_h16<DT>(e[4], e[5]), pack_h16<DT>(e[6], e[7]));
+        unsigned hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (PT == DT_BF16) {
+                // a bf16 below the probability, and the rest in a product of its own: of one sign both, so that an infinity stays one
+                const unsigned x = __float_as_uint(e[2 * i]), y = __float_as_uint(e[2 * i + 1]), x1 = x - (x != 0u), y1 = y - (y != 0u);
+                hi[i] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                lo[i] = pack_h16<PT>(e[2 * i] - __uint_as_float(x1 & 0xffff0000u), e[2 * i + 1] - __uint_as_float(y1 & 0xffff0000u));
+            } else {
+                hi[i] = pack_h16<PT>(e[2 * i], e[2 * i + 1]);
+                lo[i] = 0u;
+            }
+        }
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
             unsigned a[4];
@@ -310,12 +326,14 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             for (int i = 0; i < 4; ++i) {
                 if constexpr (I8) {
                     const int x = (int) (vf[2 * i][n / 4] >> (n % 4 * 8)), y = (int) (vf[2 * i + 1][n / 4] >> (n % 4 * 8));
-                    a[i] = pack_h16<DT>((float) (signed char) x, (float) (signed char) y);
+                    a[i] = pack_h16<PT>((float) (signed char) x, (float) (signed char) y);
                 } else {
                     a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][n / 2], vf[2 * i][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
                 }
             }
-            o[n] = mfma(make_uint4(a[0], a[1], a[2], a[3]), pf, o[n]);
+            const uint4 v4 = make_uint4(a[0], a[1], a[2], a[3]);
+            o[n] = mfma.template operator()<PT>(v4, make_uint4(hi[0], hi[1], hi[2], hi[3]), o[n]);
+            if constexpr (PT == DT_BF16) o[n] = mfma.template operator()<PT>(v4, make_uint4(lo[0], lo[1], lo[2], lo[3]), o[n]);
         }
     };
 
@@ -340,7 +358,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             if (t >= t_end) break;
         }
     }
-    if constexpr (I8 && DT == DT_F16)
+    if constexpr (I8)
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
 #pragma unroll

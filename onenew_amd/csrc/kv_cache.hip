@@ -80,11 +80,6 @@ struct AppendParams {
     int waves;       // wavefronts that share a token's heads
 };
 
-// lane i's value from lane i ^ 1, i ^ 2, 7 - i (of eight) or 15 - i (of sixteen), through the vector pipe
-enum { DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_REVERSE4 = 0x1B, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140, DPP_ROTATE8 = 0x128 };
-template <int HOW> __device__ __forceinline__ unsigned lane_moved(unsigned x) { return (unsigned) __builtin_amdgcn_update_dpp(0, (int) x, HOW, 0xf, 0xf, true); }
-template <int HOW> __device__ __forceinline__ float lane_moved(float x) { return __uint_as_float(lane_moved<HOW>(__float_as_uint(x))); }
-
 // over the LANES lanes of a row: each step joins groups that the last one made equal
 template <int LANES> __device__ __forceinline__ unsigned row_max(unsigned x) {
     x = max(x, lane_moved<DPP_XOR1>(x));

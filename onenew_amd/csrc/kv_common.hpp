@@ -18,6 +18,11 @@ int cache_shape(const char *what, const onhip_cache_desc_t *c, CacheView *view, 
 // checks the addresses and fills them in
 int cache_memory(const char *what, const onhip_cache_desc_t *c, const void *k, const void *v, const float *k_scale, const float *v_scale, CacheView *view);
 
+// lane i's value from lane i ^ 1, i ^ 2, 7 - i (of eight) or 15 - i (of sixteen), through the vector pipe
+enum { DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_REVERSE4 = 0x1B, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140, DPP_ROTATE8 = 0x128 };
+template <int HOW> __device__ __forceinline__ unsigned lane_moved(unsigned x) { return (unsigned) __builtin_amdgcn_update_dpp(0, (int) x, HOW, 0xf, 0xf, true); }
+template <int HOW> __device__ __forceinline__ float lane_moved(float x) { return __uint_as_float(lane_moved<HOW>(__float_as_uint(x))); }
+
 // eight (NV = 2) or four (NV = 1) signed bytes as pairs of the 16-bit type: every int8 is a bf16 and an fp16
 template <int DT, int NV> __device__ __forceinline__ void s8_to_h16(const unsigned (&x)[NV], unsigned (&y)[2 * NV]) {
 #pragma unroll

@@ -371,7 +371,7 @@ int onhip_attention(const onhip_attention_desc_t *d, const void *q, const void *
  * No counterparts in the reference, whose KV_CACHE_INFO_S (common/nn_common.h) has nothing behind it.  Tensors are bf16 or fp16
  * (`compute`: ONHIP_COMPUTE_BF16 or _F16), the head dimension 64 or 128 and contiguous, everything 16-byte aligned, strides in elements and
  * multiples of 8.  Indices, lengths, tables and ranges are int32 arrays in device memory that the kernels check themselves: nothing outside
- * the cache is read or written whatever they hold.  The calls use no shared workspace: calls on different streams may overlap, as long as
+ * the cache is read or written whatever they hold.  A stride over a single element is not looked at.  The calls use no shared workspace: calls on different streams may overlap, as long as
  * they are not handed the same workspace, result or cache rows that one of them writes.
  *
  * The cache: `pages` pages of `page_tokens` rows (a power of two up to 1024) for each of `kv_heads` heads; element (page, head, row, channel)
@@ -389,7 +389,7 @@ typedef struct onhip_cache_desc {
  *   rotation   of q and k: the first 2 * pairs channels in pairs (a, b) -> (a cos - b sin, b cos + a sin), pair i being the channels i and
  *              i + pairs, or with `interleaved` 2 i and 2 i + 1, by the angle positions[token] * inv_freq[i] (product and reduction in 64 bits);
  *              pairs a multiple of 8, 0 for no rotation
- *   q          rounded to q_out, which may be q itself
+ *   q          rounded to q_out, which may be q itself with its strides
  *   k, v       to row slots[token] % page_tokens of page slots[token] / page_tokens, rounded to the 16-bit type, or as
  *              rint(x * 127 / max|x|) with the scale max|x| / 127 (0 for a row of zeros, NaN for a row with an infinity or a NaN in it).
  * A token whose slot is outside the cache (-1 for padding) leaves the cache as it is; a slot belongs to one token of a call (one that is
@@ -416,7 +416,7 @@ int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const voi
  *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * (lengths[b] - 1 - j) where slopes are given
  *   out = Softmax(s) v   over j in [0, lengths[b]), or with window > 0 the last `window` of them.
  * Query head h reads key-value head h / (q_heads / kv_heads).  Strides are (sequence, head).  A sequence of length 0 or less gives zeros; one
- * whose table names a page that does not exist, or is longer than its table, NaN.  The keys of a sequence may be shared out among
+ * whose table names a page that does not exist, or is longer than its table, NaN.  out may not be q.  The keys of a sequence may be shared out among
  * workgroups whose parts go through `workspace` (16-byte aligned, onhip_attention_paged_workspace bytes; 0: none needed) and are joined in a
  * fixed order: the same call gives the same bits. */
 typedef struct onhip_paged_attention_desc {
@@ -437,7 +437,7 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
  *   window     P - j < window               (where window > 0)
  *   ranges     begin <= j < end, the pair ranges[(b * q_tokens + i) * 2] (where given: documents of a packed batch, prefixes, padded lengths)
  *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * |P - j| where slopes are given
- *   out = Softmax(s) v over the keys seen, zeros where none is.
+ *   out = Softmax(s) v over the keys seen, zeros where none is (k_tokens 0 among them).  out may not be q, k or v.
  * Keys and values that a row does not see are kept out of it whatever they hold, infinities and NaN included.  Query head h reads key-value
  * head h / (q_heads / kv_heads).  Strides are (batch, head, token).  workspace as for onhip_attention_paged.  onhip_attention is the form for
  * at most 256 tokens without a mask, and for fp32. */

@@ -500,7 +500,7 @@ static int masked_splits(const onhip_masked_attention_desc_t *d, long long block
 
 static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg, int *blocks, int *splits) {
     constexpr int MOST = 1 << 29;
-    if (!d || d->batch < 1 || d->q_heads < 1 || d->kv_heads < 1 || d->q_tokens < 1 || d->k_tokens < 1) return set_error(ONHIP_ERR_ARG, "masked attention: bad shape");
+    if (!d || d->batch < 1 || d->q_heads < 1 || d->kv_heads < 1 || d->q_tokens < 1 || d->k_tokens < 0) return set_error(ONHIP_ERR_ARG, "masked attention: bad shape");
     if (d->compute == ONHIP_COMPUTE_BF16) *dt = DT_BF16;
     else if (d->compute == ONHIP_COMPUTE_F16) *dt = DT_F16;
     else return set_error(ONHIP_ERR_ARG, "masked attention: compute type %d is neither bf16 nor fp16", d->compute);
@@ -549,19 +549,26 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     int dt, rg;
     const int rc = masked_check(d, &dt, &rg, &p.blocks, &p.splits);
     if (rc) return rc;
-    if (!q || !k || !v || !out) return set_error(ONHIP_ERR_ARG, "masked attention: null tensor pointer");
+    if (!q || !out || (d->k_tokens > 0 && (!k || !v))) return set_error(ONHIP_ERR_ARG, "masked attention: null tensor pointer");
+    if (out == q || (d->k_tokens > 0 && (out == k || out == v))) return set_error(ONHIP_ERR_ARG, "masked attention: the result may not be an operand");
     if (reinterpret_cast<uintptr_t>(ranges) % 8) return set_error(ONHIP_ERR_ARG, "masked attention: ranges must be 8-byte aligned");
     const long long *strides[4] = {d->q_strides, d->k_strides, d->v_strides, d->out_strides};
     const void *ptrs[4] = {q, k, v, out};
+    const int q_extent[3] = {d->batch, d->q_heads, d->q_tokens}, k_extent[3] = {d->batch, d->kv_heads, d->k_tokens};
+    long long *const own[4] = {p.qs, p.ks, p.vs, p.os};
     for (int t = 0; t < 4; ++t) {
+        const bool of_k = t == 1 || t == 2;
         if (reinterpret_cast<uintptr_t>(ptrs[t]) % 16) return set_error(ONHIP_ERR_ARG, "masked attention: tensors must be 16-byte aligned");
-        for (int i = 0; i < 3; ++i)
+        for (int i = 0; i < 3; ++i) {
+            own[t][i] = 0;   // a stride that is never stepped over
+            if ((of_k ? k_extent : q_extent)[i] <= 1) continue;
             if (strides[t][i] < 0 || strides[t][i] % 8) return set_error(ONHIP_ERR_ARG, "masked attention: strides must be non-negative multiples of 8");
+            own[t][i] = strides[t][i];
+        }
     }
-    const int extent[3] = {d->batch, d->q_heads, d->q_tokens};
     for (int i = 0; i < 3; ++i)
-        if (extent[i] > 1 && d->out_strides[i] < d->head_dim) return set_error(ONHIP_ERR_ARG, "masked attention: rows of the result overlap");
-    if (d->k_strides[2] >= (1LL << 23) || d->v_strides[2] >= (1LL << 23)) return set_error(ONHIP_ERR_ARG, "masked attention: token strides of k and v must be below 2^23");
+        if (q_extent[i] > 1 && d->out_strides[i] < d->head_dim) return set_error(ONHIP_ERR_ARG, "masked attention: rows of the result overlap");
+    if (p.ks[2] >= (1LL << 23) || p.vs[2] >= (1LL << 23)) return set_error(ONHIP_ERR_ARG, "masked attention: token strides of k and v must be below 2^23");
     const long long rows = (long long) d->batch * d->q_heads * d->q_tokens;
     const size_t need = join_bytes(rows, p.splits, d->head_dim);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
@@ -570,9 +577,6 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     p.k = reinterpret_cast<const unsigned short *>(k);
     p.v = reinterpret_cast<const unsigned short *>(v);
     p.out = reinterpret_cast<unsigned short *>(out);
-    for (int i = 0; i < 3; ++i) {
-        p.qs[i] = d->q_strides[i]; p.ks[i] = d->k_strides[i]; p.vs[i] = d->v_strides[i]; p.os[i] = d->out_strides[i];
-    }
     p.ranges = ranges;
     p.slopes = slopes;
     p.batch = d->batch;

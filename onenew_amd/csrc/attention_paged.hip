@@ -498,7 +498,7 @@ static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention
 static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d, CacheView *view, int *dt) {
     const int rc = cache_shape("paged attention", c, view, dt);
     if (rc) return rc;
-    if (!d || d->batch < 1 || d->q_heads < 1 || d->table_pages < 1 || d->table_stride < 0) return set_error(ONHIP_ERR_ARG, "paged attention: bad shape");
+    if (!d || d->batch < 1 || d->q_heads < 1 || d->table_pages < 0 || d->table_stride < 0) return set_error(ONHIP_ERR_ARG, "paged attention: bad shape");
     if (d->q_heads % c->kv_heads) return set_error(ONHIP_ERR_ARG, "paged attention: %d query heads for %d key-value heads", d->q_heads, c->kv_heads);
     if ((long long) d->batch * d->q_heads >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "paged attention: %d sequences of %d heads", d->batch, d->q_heads);
     if ((long long) d->table_pages * c->page_tokens > (1LL << 30)) return set_error(ONHIP_ERR_ARG, "paged attention: a table of %d pages", d->table_pages);
@@ -535,12 +535,15 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
     int dt, rc = paged_check(c, d, &p.c, &dt);
     if (!rc) rc = cache_memory("paged attention", c, k_cache, v_cache, k_scale, v_scale, &p.c);
     if (rc) return rc;
-    if (!q || !out || !table || !lengths) return set_error(ONHIP_ERR_ARG, "paged attention: null pointer");
+    if (!q || !out || !lengths || (d->table_pages > 0 && !table)) return set_error(ONHIP_ERR_ARG, "paged attention: null pointer");
+    if (out == q) return set_error(ONHIP_ERR_ARG, "paged attention: the result may not be an operand");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16) return set_error(ONHIP_ERR_ARG, "paged attention: tensors must be 16-byte aligned");
     for (int i = 0; i < 2; ++i) {
+        p.qs[i] = p.os[i] = 0;   // strides that are never stepped over
+        if ((i == 0 ? d->batch : d->q_heads) == 1) continue;
         if (d->q_strides[i] < 0 || d->q_strides[i] % 8 || d->out_strides[i] < 0 || d->out_strides[i] % 8)
             return set_error(ONHIP_ERR_ARG, "paged attention: strides must be non-negative multiples of 8");
-        if ((i == 0 ? d->batch : d->q_heads) > 1 && d->out_strides[i] < c->head_dim) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
+        if (d->out_strides[i] < c->head_dim) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
         p.qs[i] = d->q_strides[i];
         p.os[i] = d->out_strides[i];
     }

@@ -346,22 +346,27 @@ int onhip_cache_append(const onhip_cache_desc_t *c, void *k_cache, void *v_cache
     if (r->pairs < 0 || r->pairs % 8 || 2 * r->pairs > c->head_dim) return set_error(ONHIP_ERR_ARG, "cache append: %d pairs (a multiple of 8, at most half of the head dimension)", r->pairs);
     if (r->pairs && (!positions || !inv_freq)) return set_error(ONHIP_ERR_ARG, "cache append: a rotation needs positions and frequencies");
     if ((q_weight || k_weight) && !(r->eps >= 0.0f)) return set_error(ONHIP_ERR_ARG, "cache append: eps must not be negative");
+    if (q_out == k || q_out == v) return set_error(ONHIP_ERR_ARG, "cache append: the result may be q alone");
     const void *ptrs[4] = {q, k, v, q_out};
     const long long *strides[4] = {r->q_strides, r->k_strides, r->v_strides, r->out_strides};
+    long long *const own[4] = {p.qs, p.ks, p.vs, p.os};
     for (int t = 0; t < 4; ++t) {
         if (reinterpret_cast<uintptr_t>(ptrs[t]) % 16) return set_error(ONHIP_ERR_ARG, "cache append: tensors must be 16-byte aligned");
-        for (int i = 0; i < 2; ++i)
+        const int extent[2] = {r->tokens, t == 0 || t == 3 ? r->q_heads : c->kv_heads};
+        for (int i = 0; i < 2; ++i) {
+            own[t][i] = 0;   // a stride that is never stepped over
+            if (extent[i] == 1) continue;
             if (strides[t][i] < 0 || strides[t][i] % 8) return set_error(ONHIP_ERR_ARG, "cache append: strides must be non-negative multiples of 8");
+            own[t][i] = strides[t][i];
+        }
     }
+    if (q_out == q && (p.os[0] != p.qs[0] || p.os[1] != p.qs[1])) return set_error(ONHIP_ERR_ARG, "cache append: a result in q's place has q's strides");
     if ((r->tokens > 1 && r->out_strides[0] < c->head_dim) || (r->q_heads > 1 && r->out_strides[1] < c->head_dim))
         return set_error(ONHIP_ERR_ARG, "cache append: rows of the result overlap");
     p.q = reinterpret_cast<const unsigned short *>(q);
     p.k = reinterpret_cast<const unsigned short *>(k);
     p.v = reinterpret_cast<const unsigned short *>(v);
     p.q_out = reinterpret_cast<unsigned short *>(q_out);
-    for (int i = 0; i < 2; ++i) {
-        p.qs[i] = r->q_strides[i]; p.ks[i] = r->k_strides[i]; p.vs[i] = r->v_strides[i]; p.os[i] = r->out_strides[i];
-    }
     p.positions = positions;
     p.slots = slots;
     p.inv_freq = inv_freq;
@@ -391,16 +396,19 @@ int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const voi
     int dt, rc = cache_shape("cache read", c, &p.c, &dt);
     if (!rc) rc = cache_memory("cache read", c, k_cache, v_cache, k_scale, v_scale, &p.c);
     if (rc) return rc;
-    if (batch < 1 || tokens < 1 || table_pages < 1 || table_stride < 0) return set_error(ONHIP_ERR_ARG, "cache read: bad shape");
+    if (batch < 1 || tokens < 1 || table_pages < 0 || table_stride < 0) return set_error(ONHIP_ERR_ARG, "cache read: bad shape");
     if (batch > 32767 || c->kv_heads > 65535) return set_error(ONHIP_ERR_ARG, "cache read: %d sequences of %d heads", batch, c->kv_heads);
     if (tokens > (1 << 30)) return set_error(ONHIP_ERR_ARG, "cache read: %d tokens", tokens);
-    if (!table || !lengths || !k_out || !v_out || !k_out_strides || !v_out_strides) return set_error(ONHIP_ERR_ARG, "cache read: null pointer");
+    if ((table_pages > 0 && !table) || !lengths || !k_out || !v_out || !k_out_strides || !v_out_strides) return set_error(ONHIP_ERR_ARG, "cache read: null pointer");
     if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16) return set_error(ONHIP_ERR_ARG, "cache read: results must be 16-byte aligned");
+    if (k_out == v_out) return set_error(ONHIP_ERR_ARG, "cache read: one result for k and v");
     const long long *strides[2] = {k_out_strides, v_out_strides};
     const int extent[3] = {batch, c->kv_heads, tokens};
     for (int t = 0; t < 2; ++t)
         for (int i = 0; i < 3; ++i) {
-            if (strides[t][i] < 0 || strides[t][i] % 8 || (extent[i] > 1 && strides[t][i] < c->head_dim))
+            p.os[t][i] = 0;   // a stride that is never stepped over
+            if (extent[i] == 1) continue;
+            if (strides[t][i] % 8 || strides[t][i] < c->head_dim)
                 return set_error(ONHIP_ERR_ARG, "cache read: strides of the results must be multiples of 8, at least the head dimension");
             p.os[t][i] = strides[t][i];
         }

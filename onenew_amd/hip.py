@@ -811,10 +811,10 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
                  k_scale=None, v_scale=None, q_out=None):
     """q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim] (any token and head strides, e.g. slices of one projection's rows):
     norm of q's and k's heads where there are weights [head_dim] (fp32), rotation by positions [tokens] (int32) times inv_freq [pairs] (fp32)
-    where there are frequencies, q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
+    where there are frequencies (else positions may be None), q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
     [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with fp32 scales [pages, kv_heads, page_tokens]"""
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
-           positions.dtype, positions.get_device(), positions.numel(), positions.is_contiguous(), slots.dtype, slots.get_device(), slots.numel(), slots.is_contiguous(),
+           _flat(positions), slots.dtype, slots.get_device(), slots.numel(), slots.is_contiguous(),
            k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
            _flat(inv_freq), _flat(q_weight), _flat(k_weight), eps, interleaved, _meta(k_scale), _meta(v_scale), _meta(q_out))
     last = _last.get("append")
@@ -824,7 +824,7 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
         q_out = q.new_empty(shape)
     if not empty:
         _check(load().onhip_cache_append(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), r, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                         positions.data_ptr(), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream()),
+                                         _ptr(positions), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream()),
                "onhip_cache_append")
     return q_out
 

@@ -53,6 +53,45 @@ def test_causal(dtype, hd, b, hq, hkv, tq, tk):
     _run(dtype, b, hq, hkv, tq, tk, hd)
 
 
+# more than one workgroup a compute unit: 128 rows each, heads divided among the XCDs and not
+MANY = [(33, 16, 8, 130, 200, 64), (37, 14, 7, 70, 65, 128), (300, 1, 1, 33, 70, 64), (9, 32, 32, 129, 129, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_many_rows(dtype, i):
+    b, hq, hkv, tq, tk, hd = MANY[i]
+    _run(dtype, b, hq, hkv, tq, tk, hd)
+    _run(dtype, b, hq, hkv, tq, tk, hd, window=40, cap=20.0, bias=i % 2 == 0)
+    g = torch.Generator().manual_seed(i)
+    edge = torch.randint(-20, tk + 20, (b, tq, 2), generator=g, dtype=torch.int32)
+    _run(dtype, b, hq, hkv, tq, tk, hd, causal=i % 2 == 0, ranges=edge, q_offset=tk // 2)
+
+
+def test_scores_above_half_of_the_cap():
+    """capped by a polynomial below, by an exponential above"""
+    for scale in (0.05, 0.3, 1.0, 5.0, -2.0):
+        _run("f16", 1, 2, 1, 64, 130, 64, scale=scale, cap=6.0)
+        _run("bf16", 60, 16, 8, 100, 130, 128, scale=scale, cap=6.0, causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_parts(dtype):
+    _run(dtype, 1, 1, 1, 1, 70000, 64)
+    _run(dtype, 1, 2, 1, 5, 33333, 128, window=20000)
+
+
+def test_no_keys():
+    hip.init(0)
+    q = torch.randn((2, 4, 9, 64), device="cuda").half()
+    k = torch.empty((2, 2, 0, 64), device="cuda", dtype=torch.float16)
+    got = hip.attention_masked(q, k, k, causal=True)
+    torch.cuda.synchronize()
+    assert got.shape == (2, 9, 256) and not got.any()
+    for empty in (q[:0], q[:, :, :0]):
+        assert hip.attention_masked(empty, q[: empty.shape[0], :2], q[: empty.shape[0], :2]).numel() == 0
+
+
 MORE = [dict(causal=False), dict(scale=0.0), dict(scale=-0.3, causal=False), dict(window=1), dict(window=37), dict(window=64, causal=False), dict(cap=3.0), dict(cap=50.0, window=100),
         dict(bias=True), dict(bias=True, causal=False), dict(bias=True, cap=5.0, window=90), dict(q_offset=-20), dict(q_offset=0), dict(q_offset=500, window=300),
         dict(q_offset=1000, window=100), dict(q_offset=-400), dict(scale=3.0)]
@@ -84,19 +123,21 @@ def test_ranges(dtype, tq, tk, causal):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("tq,tk", [(100, 100), (20, 2000)])
-def test_unseen_values(dtype, hd, tq, tk):
+@pytest.mark.parametrize("tq,tk,b", [(100, 100, 1), (20, 2000, 1), (100, 150, 300)])
+def test_unseen_values(dtype, hd, tq, tk, b):
     """what a row does not see leaves its bits alone, infinities and NaN of k and v included; what it sees does not"""
     hip.init(0)
-    print(dtype, hd, tq, tk, flush=True)
-    q, k, v = [x.cuda() for x in _inputs(1, 2, 1, tq, tk, hd, DT[dtype])]
+    print(dtype, hd, tq, tk, b, flush=True)
+    q, k, v = [x.cuda() for x in _inputs(b, 2, 1, tq, tk, hd, DT[dtype])]
+    if b > 1:
+        q, k, v = (x[:1].expand(b, -1, -1, -1) for x in (q, k, v))
     cut = tk - tq // 2      # rows whose place is below see nothing from here on
-    clean = hip.attention_masked(q, k, v, causal=True, scale=0.1).view(tq, 2, hd)
+    clean = hip.attention_masked(q, k, v, causal=True, scale=0.1)[-1].view(tq, 2, hd)
     k2, v2 = k.clone(), v.clone()
     k2[:, :, cut + 1], k2[:, :, cut + 2, 3] = math.nan, math.inf
     v2[:, :, cut, 0], v2[:, :, cut, 1], v2[:, :, cut, 2] = math.inf, -math.inf, math.nan
     v2[:, :, cut + 3, 1] = math.inf
-    got = hip.attention_masked(q, k2, v2, causal=True, scale=0.1).view(tq, 2, hd)
+    got = hip.attention_masked(q, k2, v2, causal=True, scale=0.1)[-1].view(tq, 2, hd)
     torch.cuda.synchronize()
     first = cut - (tk - tq)   # the first row that sees key `cut`
     assert torch.equal(got[:first], clean[:first])
@@ -106,7 +147,7 @@ def test_unseen_values(dtype, hd, tq, tk):
     assert float(err.max()) == 0.0          # its k is clean, so the other channels are
     assert bool(got[first + 1:].float().isnan().all())   # a score that is NaN
     # the same with k clean: infinities of both signs in one channel are no number
-    got = hip.attention_masked(q, k, v2, causal=True, scale=0.1).view(tq, 2, hd).float()
+    got = hip.attention_masked(q, k, v2, causal=True, scale=0.1)[-1].view(tq, 2, hd).float()
     torch.cuda.synchronize()
     assert bool((got[first:first + 3, :, 1] == -math.inf).all()) and bool(got[first + 3:, :, 1].isnan().all())
     assert bool((got[first:, :, 0] == math.inf).all()) and bool(got[first:, :, 2].isnan().all())

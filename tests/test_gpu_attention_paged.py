@@ -58,7 +58,8 @@ def _run(dtype, int8, lengths, hq, hkv, hd, page, scale=None, window=0, cap=0.0,
 
 
 SHAPES = [([1], 1, 1, 1), ([0, 1, 2], 2, 1, 1), ([31, 32, 33, 0, -7], 3, 3, 2), ([15, 16, 17, 127, 128, 129], 6, 2, 4), ([500], 8, 1, 8), ([777, 3], 16, 1, 16),
-          ([1000, 1, 513], 34, 2, 32), ([64, 4097], 40, 1, 64), ([2000] * 3, 4, 4, 1024), ([300] * 40, 12, 12, 16), ([9000, 100], 5, 5, 128)]
+          ([1000, 1, 513], 34, 2, 32), ([64, 4097], 40, 1, 64), ([2000] * 3, 4, 4, 1024), ([300] * 40, 12, 12, 16), ([9000, 100], 5, 5, 128),
+          ([70001], 1, 1, 256), ([33000, 1, 12345], 2, 1, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -78,6 +79,20 @@ MORE = [dict(scale=0.0), dict(scale=-0.4), dict(scale=2.0), dict(window=1), dict
 @pytest.mark.parametrize("i", range(len(MORE)))
 def test_windows_caps_and_biases(dtype, int8, i):
     _run(dtype, int8, [0, 1, 32, 70, 333, 1500], 6, 2, 128 if i % 2 else 64, [4, 16, 64][i % 3], **MORE[i])
+
+
+def test_no_pages():
+    hip.init(0)
+    q, cache, _, _ = _case([5, 5], 4, 2, 64, 16, torch.float16, False)
+    k, v, _, _ = _dev(*cache)
+    table, n = torch.empty((2, 0), dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    got = hip.attention_paged(q.cuda(), k, v, table, n)
+    a, b = hip.cache_read(k, v, table, n, 4)
+    torch.cuda.synchronize()
+    assert not got[0].any() and bool(got[1].isnan().all())
+    for x in (a, b):
+        assert not x[0].any() and bool(x[1, :, :3].isnan().all()) and not x[1, :, 3:].any()
+    assert hip.attention_paged(q.cuda()[:0], k, v, table[:0], n[:0]).numel() == 0
 
 
 @pytest.mark.parametrize("int8", [False, True])

@@ -75,6 +75,22 @@ def test_append(dtype, int8, i):
         assert torch.equal(was, cache.cpu())    # every other row as it was
 
 
+def test_nothing_but_the_write():
+    """no norm, no rotation, no positions; no tokens"""
+    hip.init(0)
+    x = torch.randn((5, 4, 128), device="cuda").bfloat16()
+    k, v, _, _ = _cache(2, 1, 4, 128, torch.bfloat16, False)
+    slots = torch.tensor([7, 0, 3, 5, 1], dtype=torch.int32, device="cuda")
+    q = hip.cache_append(x[:, :2], x[:, 2:3], x[:, 3:], None, slots, k, v)
+    torch.cuda.synchronize()
+    assert torch.equal(q, x[:, :2])
+    for cache, y in ((k, x[:, 2]), (v, x[:, 3])):
+        assert torch.equal(cache[slots.long() // 4, 0, slots.long() % 4], y) and bool((cache[[0, 1, 1], 0, [2, 0, 2]] == 7.0).all())
+    assert hip.cache_append(x[:0, :2], x[:0, 2:3], x[:0, 3:], None, slots[:0], k, v).shape == (0, 2, 128)
+    with pytest.raises(hip.OnhipError):
+        hip.cache_append(x[:, :2], x[:, 2:3], x[:, 3:], None, slots, k, v, inv_freq=torch.ones(64, device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_int8_rows_out_of_the_ordinary(dtype):
     hip.init(0)

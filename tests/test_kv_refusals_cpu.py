@@ -35,7 +35,10 @@ def _memory(more):
     return [more.get(n, at) for n, at in (("k", A), ("v", A), ("k_scale", None), ("v_scale", None))]
 
 
-def _append(c, r, q=A, k=A, v=A, positions=A, slots=A, inv_freq=A, qw=None, kw=None, out=A, memory=(A, A, None, None)):
+B = A + (1 << 16)   # of results
+
+
+def _append(c, r, q=A, k=A, v=A, positions=A, slots=A, inv_freq=A, qw=None, kw=None, out=B, memory=(A, A, None, None)):
     return hip.load().onhip_cache_append(None if c is None else C.byref(c), *memory, None if r is None else C.byref(r), q, k, v, positions, slots, inv_freq, qw, kw, out, None)
 
 
@@ -53,9 +56,9 @@ def test_caches(i):
     c, memory = _cache(**BAD_CACHES[i]), _memory(BAD_CACHES[i])
     _refused(_append(c, _rows(), memory=memory), "cache append")
     three = (C.c_longlong * 3)(4096, 1024, 64)
-    _refused(hip.load().onhip_cache_read(C.byref(c), *memory, A, 4, 4, A, 1, 5, A, three, A, three, None), "cache read")
+    _refused(hip.load().onhip_cache_read(C.byref(c), *memory, A, 4, 4, A, 1, 5, A, three, B, three, None), "cache read")
     d = abi.PagedAttentionDesc(1, 4, 4, 0, 4, (256, 64), (256, 64), 1.0, 0.0)
-    _refused(hip.load().onhip_attention_paged(C.byref(c), *memory, C.byref(d), A, A, A, None, A, None, 0, None), "paged attention")
+    _refused(hip.load().onhip_attention_paged(C.byref(c), *memory, C.byref(d), A, A, A, None, B, None, 0, None), "paged attention")
     if not set(BAD_CACHES[i]) & {"k", "v", "k_scale"}:
         assert hip.load().onhip_attention_paged_workspace(C.byref(c), C.byref(d)) == 0
 
@@ -67,7 +70,7 @@ def test_append():
     for name in ("q", "k", "v", "slots", "out"):
         _refused(_append(c, _rows(), **{name: None}), "null")
     for name in ("q", "k", "v", "out"):
-        _refused(_append(c, _rows(), **{name: A + 8}), "aligned")
+        _refused(_append(c, _rows(), **{name: B + 8}), "aligned")
     _refused(_append(c, _rows(), positions=None), "positions")
     _refused(_append(c, _rows(), inv_freq=None), "frequencies")
     for more in (dict(tokens=0), dict(q_heads=0), dict(tokens=-4)):
@@ -78,6 +81,9 @@ def test_append():
         _refused(_append(c, _rows(**{name: (512, 60)})), "multiples of 8")
         _refused(_append(c, _rows(**{name: (-512, 64)})), "non-negative")
     _refused(_append(c, _rows(out_strides=(256, 0))), "overlap")
+    for name in ("k", "v"):
+        _refused(_append(c, _rows(), **{name: B}), "q alone")
+    _refused(_append(c, _rows(), q=B), "strides")
     for eps in (-1.0, float("nan")):
         _refused(_append(c, _rows(eps=eps), qw=A), "eps")
 
@@ -86,12 +92,12 @@ def test_read():
     c, lib = _cache(), hip.load()
     three = lambda *x: (C.c_longlong * 3)(*x)  # noqa: E731
 
-    def read(table=A, stride=4, pages=4, lengths=A, batch=2, tokens=5, k=A, ks=three(4096, 1024, 64), v=A, vs=three(4096, 1024, 64)):
+    def read(table=A, stride=4, pages=4, lengths=A, batch=2, tokens=5, k=A, ks=three(4096, 1024, 64), v=B, vs=three(4096, 1024, 64)):
         return lib.onhip_cache_read(C.byref(c), A, A, None, None, table, stride, pages, lengths, batch, tokens, k, ks, v, vs, None)
 
     for more in (dict(table=None), dict(lengths=None), dict(k=None), dict(v=None), dict(ks=None), dict(vs=None)):
         _refused(read(**more), "null")
-    for more in (dict(batch=0), dict(tokens=0), dict(pages=0), dict(stride=-1)):
+    for more in (dict(batch=0), dict(tokens=0), dict(pages=-1), dict(stride=-1)):
         _refused(read(**more), "shape")
     for more in (dict(ks=three(4096, 1024, 60)), dict(vs=three(4096, 0, 64)), dict(ks=three(-8, 1024, 64))):
         _refused(read(**more), "strides")
@@ -103,7 +109,7 @@ def test_read():
 def test_paged():
     c, lib = _cache(), hip.load()
 
-    def paged(q=A, table=A, lengths=A, out=A, ws=None, nbytes=0, **more):
+    def paged(q=A, table=A, lengths=A, out=B, ws=None, nbytes=0, **more):
         f = dict(batch=1, q_heads=4, table_pages=4, window=0, table_stride=4, q_strides=(256, 64), out_strides=(256, 64), scale=1.0, softcap=0.0)
         f.update(more)
         d = abi.PagedAttentionDesc(*f.values())
@@ -111,7 +117,7 @@ def test_paged():
 
     for more in (dict(q=None), dict(table=None), dict(lengths=None), dict(out=None)):
         _refused(paged(**more), "null")
-    for more in (dict(batch=0), dict(q_heads=0), dict(table_pages=0), dict(table_stride=-1)):
+    for more in (dict(batch=0), dict(q_heads=0), dict(table_pages=-1), dict(table_stride=-1)):
         _refused(paged(**more), "shape")
     _refused(paged(q_heads=3), "query heads")
     _refused(paged(window=-1), "window")
@@ -119,10 +125,11 @@ def test_paged():
     _refused(paged(table_pages=1 << 27), "table")
     for more in (dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(scale=float("inf")), dict(scale=float("nan"))):
         _refused(paged(**more), "finite")
-    for more in (dict(q_strides=(256, 60)), dict(out_strides=(256, -64))):
+    for more in (dict(q_strides=(256, 60)), dict(out_strides=(256, -64)), dict(q_strides=(100, 64), batch=2)):
         _refused(paged(**more), "multiples of 8")
     _refused(paged(out_strides=(256, 0)), "overlap")
     _refused(paged(q=A + 8), "aligned")
+    _refused(paged(q=B), "operand")
     # a long table: parts, hence a workspace
     d = abi.PagedAttentionDesc(1, 4, 400, 0, 400, (256, 64), (256, 64), 1.0, 0.0)
     need = lib.onhip_attention_paged_workspace(C.byref(c), C.byref(d))
@@ -134,17 +141,17 @@ def test_paged():
 def test_masked():
     lib = hip.load()
 
-    def masked(q=A, k=A, v=A, ranges=None, out=A, ws=None, nbytes=0, size=False, **more):
+    def masked(q=A, k=A, v=A, ranges=None, out=B, ws=None, nbytes=0, size=False, **more):
         f = dict(batch=1, q_heads=4, kv_heads=2, q_tokens=8, k_tokens=8, head_dim=64, q_strides=(2048, 64, 256), k_strides=(1024, 64, 128), v_strides=(1024, 64, 128),
                  out_strides=(2048, 64, 256), scale=1.0, softcap=0.0, causal=1, window=0, q_offset=0, compute=abi.COMPUTE_F16)
         f.update(more)
         d = abi.MaskedAttentionDesc(*f.values())
         return lib.onhip_attention_masked_workspace(C.byref(d)) if size else lib.onhip_attention_masked(C.byref(d), q, k, v, ranges, None, out, ws, nbytes, None)
 
-    assert lib.onhip_attention_masked(None, A, A, A, None, None, A, None, 0, None) == -1
+    assert lib.onhip_attention_masked(None, A, A, A, None, None, B, None, 0, None) == -1
     for more in (dict(q=None), dict(k=None), dict(v=None), dict(out=None)):
         _refused(masked(**more), "null")
-    for more in (dict(batch=0), dict(q_heads=0), dict(kv_heads=0), dict(q_tokens=0), dict(k_tokens=0)):
+    for more in (dict(batch=0), dict(q_heads=0), dict(kv_heads=0), dict(q_tokens=0), dict(k_tokens=-1)):
         _refused(masked(**more), "shape")
     _refused(masked(q_heads=3), "query heads")
     _refused(masked(compute=abi.COMPUTE_F32), "neither")
@@ -158,11 +165,13 @@ def test_masked():
         _refused(masked(**more), "finite")
     for name in ("q_strides", "k_strides", "v_strides", "out_strides"):
         _refused(masked(**{name: (2048, 64, 252)}), "multiples of 8")
-        _refused(masked(**{name: (-2048, 64, 256)}), "non-negative")
+        _refused(masked(batch=2, **{name: (-2048, 64, 256)}), "non-negative")
     _refused(masked(out_strides=(2048, 64, 0)), "overlap")
     _refused(masked(k_strides=(1024, 64, 1 << 23)), "token strides")
-    for more in (dict(q=A + 8), dict(out=A + 2)):
+    for more in (dict(q=A + 8), dict(out=B + 2)):
         _refused(masked(**more), "aligned")
+    for more in (dict(q=B), dict(k=B), dict(v=B)):
+        _refused(masked(**more), "operand")
     _refused(masked(ranges=A + 4), "ranges")
     need = masked(size=True, k_tokens=5000)
     assert need > 0 and masked(size=True) == 0 and masked(size=True, batch=0) == 0

@@ -101,6 +101,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     const unsigned own_row = min(row0 + (unsigned) li, last_row);
     int token = (int) div31(own_row, p.by_group), head = kvh * p.group + (int) (own_row - (unsigned) token * (unsigned) p.group);
     const int place = token + p.q_offset;
+    // q: asked for first, whole rows at a time (a row a lane, each load keeps a compute unit's address path busy for 64 cycles)
+    u32x4 qr[32 / ROWS];
+#pragma unroll
+    for (int i = 0; i < 32 / ROWS; ++i) {
+        const unsigned row = min(row0 + (unsigned) (i * ROWS + lane / UNITS), last_row), tk = div31(row, p.by_group);
+        qr[i] = *reinterpret_cast<const u32x4 *>(p.q + b * p.qs[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.qs[1] + tk * p.qs[2] + lane % UNITS * 8);
+    }
     auto first_key = [&](int t) __attribute__((always_inline)) { return p.window > 0 ? max(0, t + p.q_offset - p.window + 1) : 0; };
     auto end_key = [&](int t) __attribute__((always_inline)) { return p.causal ? min(p.k_tokens, t + p.q_offset + 1) : p.k_tokens; };
     int lo = first_key(token), hi = end_key(token);
@@ -222,20 +229,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     };
 
     if (t_begin < t_end) fetch(t_begin);
-    // q: whole rows from memory, through the wavefront's part of the second buffers into the channels 16 s + 8 (lane / 32) .. + 7 of step s (a row a
-    // lane, each load keeps a compute unit's address path busy for 64 cycles)
+    // q on into the channels 16 s + 8 (lane / 32) .. + 7 of step s, through the wavefront's part of the second buffers
     uint4 qf[STEPS];
     {
         uint4 *const rows = s_kv[1 + (wave & 2)] + (wave & 1) * 32 * UNITS;
-        uint4 x[32 / ROWS];
-#pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i) {
-            const unsigned row = min(row0 + (unsigned) (i * ROWS + lane / UNITS), last_row), tk = div31(row, p.by_group);
-            x[i] = *reinterpret_cast<const uint4 *>(p.q + b * p.qs[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.qs[1] + tk * p.qs[2] + lane % UNITS * 8);
-        }
 #pragma unroll
         for (int i = 0; i < 32 / ROWS; ++i)
-            rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)] = make_uint4(x[i].x ^ p.flip, x[i].y ^ p.flip, x[i].z ^ p.flip, x[i].w ^ p.flip);
+            rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)] = make_uint4(qr[i].x ^ p.flip, qr[i].y ^ p.flip, qr[i].z ^ p.flip, qr[i].w ^ p.flip);
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) qf[st] = rows[k_unit(li, 2 * st + lh)];
     }

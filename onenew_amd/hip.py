@@ -823,9 +823,10 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
     if q_out is None:
         q_out = q.new_empty(shape)
     if not empty:
-        _check(load().onhip_cache_append(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), r, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                         _ptr(positions), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream()),
-               "onhip_cache_append")
+        rc = (_lib or load()).onhip_cache_append(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), r, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                         _ptr(positions), slots.data_ptr(), _ptr(inv_freq), _ptr(q_weight), _ptr(k_weight), q_out.data_ptr(), _stream())
+        if rc:
+            _check(rc, "onhip_cache_append")
     return q_out
 
 
@@ -852,6 +853,7 @@ def _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype
 def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=None, dtype=None, k_out=None, v_out=None):
     """rows 0 .. tokens - 1 of every sequence (pages table [sequences, pages], lengths [sequences], int32), zeros behind its length: k and v
     [sequences, kv_heads, tokens, head_dim] in the cache's 16-bit type, or `dtype` for an int8 cache"""
+    import torch
     dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
     key = (_device(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
            table.dtype, table.get_device(), table.shape, table.stride(), lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(),
@@ -862,10 +864,12 @@ def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=N
     if k_out is None:
         k_out = k_cache.new_empty(shape, dtype=dtype)
     if v_out is None:
-        v_out = k_cache.new_empty(shape, dtype=dtype)
+        v_out = torch.empty_like(k_out) if k_out.is_contiguous() else k_cache.new_empty(shape, dtype=dtype)
     if not empty:
-        _check(load().onhip_cache_read(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), step, pages, lengths.data_ptr(),
-                                       shape[0], tokens, k_out.data_ptr(), ks, v_out.data_ptr(), vs, _stream()), "onhip_cache_read")
+        rc = (_lib or load()).onhip_cache_read(d, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), step, pages, lengths.data_ptr(),
+                                       shape[0], tokens, k_out.data_ptr(), ks, v_out.data_ptr(), vs, _stream())
+        if rc:
+            _check(rc, "onhip_cache_read")
     return k_out, v_out
 
 
@@ -903,8 +907,10 @@ def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, so
         out = q.new_empty(shape)
     if not empty:
         ws = _workspace(nbytes, q) if nbytes else None
-        _check(load().onhip_attention_paged(c, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), d, q.data_ptr(), table.data_ptr(),
-                                            lengths.data_ptr(), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()), "onhip_attention_paged")
+        rc = (_lib or load()).onhip_attention_paged(c, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), d, q.data_ptr(), table.data_ptr(),
+                                            lengths.data_ptr(), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream())
+        if rc:
+            _check(rc, "onhip_attention_paged")
     return out
 
 
@@ -947,8 +953,9 @@ def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, sl
         out = q.new_empty(shape)
     if not empty:
         ws = _workspace(nbytes, q) if nbytes else None
-        _check(load().onhip_attention_masked(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream()),
-               "onhip_attention_masked")
+        rc = (_lib or load()).onhip_attention_masked(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream())
+        if rc:
+            _check(rc, "onhip_attention_masked")
     return out
 
 

@@ -14,10 +14,12 @@
 // Rounded to the 16-bit type before the second product: 2^(s - m) times a constant, at most 2^8 of it (the reference point m follows a row's maximum when that is
 // 2^8 above it, so that most tiles leave the sums alone).  Scores, maxima, sums and products' sums are fp32.
 //
-// What bounds it: the matrix instructions and the vector instructions of the softmax, half of the cycles each, at a clock that falls under them (1.74 GHz): 8192
-// causal tokens of 32 heads of 128 on 8 in bf16 551 us, 1.0 PFLOP/s where a large library product reaches 1.2.  Capped scores add a third to the
-// vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 104 us.  Short rows are bound by a workgroup's chain of trips to
-// memory: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 46 us (their 67 MB take 13).
+// What bounds it: per tile of 64 keys the matrix instructions take 1024 cycles of a SIMD, the softmax's vector instructions as many (half of the exponentials run
+// between the second product's matrix instructions), LDS 1300 for operands and staging; two workgroups a compute unit overlap them to 50 % of
+// each, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 540 us, 1.0 PFLOP/s where a large library product
+// reaches 1.2.  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 101 us.  Short rows are bound by a
+// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 45 us (their 67 MB take 13).  Tiles of 32 keys with
+// three workgroups a compute unit, eight operands ahead and a higher wave priority in the products were level.
 #include "attention_join.hpp"
 
 namespace onhip {
@@ -65,9 +67,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
     constexpr int UNITS = HD / 8, ROWS = 64 / UNITS;           // 16-byte units of a row; rows that a wavefront's load covers
     constexpr int LOADS = KT / ROWS / 4;                       // loads of a wavefront for its share of a tile of k (or v)
-    __shared__ uint4 s_kv[4][KT * UNITS];   // two tiles of k, two of v
-    uint4(*const Ks)[KT * UNITS] = s_kv;
-    unsigned short(*const Vs)[KT * HD] = reinterpret_cast<unsigned short(*)[KT * HD]>(s_kv[2]);
+    // Two tiles of k, two of v.  Rows have a pitch by which 16 lanes that take one 16-byte unit of 16 rows of k, and the transposing read's 64 bytes of four rows
+    // of v, meet every bank once, and a read's place in its row is a constant of the instruction (units exchanged by row number cost an address register each).
+    constexpr int KP = HD * 2 + 16, VP = HD * 2 + 64;
+    __shared__ __attribute__((aligned(16))) unsigned char s_kv[2 * KT * (KP + VP)];
+    unsigned char *const Vs = s_kv + 2 * KT * KP;
     __shared__ int4 s_span[4];
     __shared__ int s_odd;
 
@@ -179,10 +183,6 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
             v_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, row * v_step + s_unit * 16, 0, 0);
         }
     };
-    // Where unit u of a row lies.  k: 16 lanes that take one unit of 16 rows meet every bank once.  v: the transposing read takes 64 bytes of four
-    // rows: those four segments are spread over the banks too.
-    auto k_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 15) : u ^ (row >> 1 & 7)); };
-    auto v_unit = [](int row, int u) { return row * UNITS + (HD == 128 ? u ^ (row & 3) * 4 : u ^ (row >> 1 & 1) * 4); };
     // Where some row does not see all of a tile, an infinity or a NaN in v times its probability of zero is not zero: those values go into LDS as
     // zeros, and are added to the rows that see them behind the loop.
     unsigned odd = 0u;
@@ -201,8 +201,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int row = s_row + i * ROWS;
-            Ks[buf][k_unit(row, s_unit)] = __builtin_bit_cast(uint4, k_reg[i]);
-            reinterpret_cast<uint4 *>(Vs[buf])[v_unit(row, s_unit)] = __builtin_bit_cast(uint4, v_reg[i]);
+            *reinterpret_cast<u32x4 *>(s_kv + (buf * KT + row) * KP + s_unit * 16) = k_reg[i];
+            *reinterpret_cast<u32x4 *>(Vs + (buf * KT + row) * VP + s_unit * 16) = v_reg[i];
         }
     };
     auto mfma = [](const uint4 &x, const uint4 &y, f32x16 c) __attribute__((always_inline)) {
@@ -215,16 +215,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_t;
     // of 16 lanes, four read the 32 bytes of 16 channels of one key, and each gets four keys of one channel
     const int j16 = lane & 15;
-    int v_at[DTILES];   // shorts
-#pragma unroll
-    for (int d = 0; d < DTILES; ++d) {
-        const int row = 4 * lh + j16 / 4;
-        v_at[d] = v_unit(row, 4 * d) * 8 + li / 16 * 16 + j16 % 4 * 4;
-    }
+    const unsigned char *const v_at = Vs + (4 * lh + j16 / 4) * VP + li / 16 * 32 + j16 % 4 * 8;
     auto v_frag = [&](int buf, int t, int g, int d) __attribute__((always_inline)) {   // keys 32 t + 16 g + 4 lh + .. and 8 + .. of channel tile d
-        const unsigned short *at = Vs[buf] + v_at[d] + (32 * t + 16 * g) * HD;
+        const unsigned char *at = v_at + buf * KT * VP + (32 * t + 16 * g) * VP + 64 * d;
         const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t) at));
-        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t) (at + 8 * HD)));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t) (at + 8 * VP)));
         return make_uint4(x.x, x.y, y.x, y.y);
     };
 
@@ -232,13 +227,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     // q on into the channels 16 s + 8 (lane / 32) .. + 7 of step s, through the wavefront's part of the second buffers
     uint4 qf[STEPS];
     {
-        uint4 *const rows = s_kv[1 + (wave & 2)] + (wave & 1) * 32 * UNITS;
+        unsigned char *const rows = KT == 32 ? s_kv + wave * 32 * KP : (wave < 2 ? s_kv + KT * KP : Vs + KT * VP) + (wave & 1) * 32 * KP;
 #pragma unroll
         for (int i = 0; i < 32 / ROWS; ++i)
-            rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)] = make_uint4(qr[i].x ^ p.flip, qr[i].y ^ p.flip, qr[i].z ^ p.flip, qr[i].w ^ p.flip);
+            *reinterpret_cast<u32x4 *>(rows + (i * ROWS + lane / UNITS) * KP + lane % UNITS * 16) = qr[i] ^ u32x4{p.flip, p.flip, p.flip, p.flip};
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) qf[st] = rows[k_unit(li, 2 * st + lh)];
+        for (int st = 0; st < STEPS; ++st) qf[st] = __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4 *>(rows + li * KP + lh * 16 + st * 32));
     }
+    if (KT == 32) __syncthreads();   // every part of the buffers was some wavefront's
     f32x16 o[DTILES];
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
@@ -259,7 +255,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
-        auto k_frag = [&](int i) __attribute__((always_inline)) { return Ks[buf][k_unit(32 * (i / STEPS + kh) + li, 2 * (i % STEPS) + lh)]; };
+        const unsigned char *const k_at = s_kv + (buf * KT + 32 * kh + li) * KP + lh * 16;
+        auto k_frag = [&](int i) __attribute__((always_inline)) {
+            return __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4 *>(k_at + i / STEPS * 32 * KP + i % STEPS * 32));
+        };
         uint4 ring[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) ring[i] = k_frag(i);
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     l += __shfl_xor(l, 32, 64);
     if constexpr (RG == 2) {   // the two halves of the keys: the second wavefront's results to the first
         float *const half = reinterpret_cast<float *>(s_kv) + rg * (DTILES * 16 + 2) * 64 + lane;
-        static_assert(2 * (DTILES * 16 + 2) * 64 * 4 <= sizeof(s_kv), "room for two row groups");
+        static_assert(2 * (DTILES * 16 + 2) * 64 * 4 <= 2 * KT * KP, "two row groups, in the place of k");
         if (kh) {
             half[0] = m;
             half[64] = l;
@@ -468,22 +467,21 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
                 *reinterpret_cast<float4 *>(po + 32 * d + 8 * g + 4 * lh) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
         return;
     }
-    // the result as q came, through LDS: whole rows to memory (in the place of k, or behind what the halves of the keys were joined from)
+    // the result as q came, through LDS: whole rows to memory (in the place of k, or of v where the halves of the keys are joined in that)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint4 *const rows = s_kv[0] + (RG == 4 ? 0 : 160 * UNITS) + rg * 32 * UNITS;
-    static_assert(RG == 4 || 2 * (DTILES * 16 + 2) * 64 * 4 <= 160 * UNITS * 16, "the halves end before the rows");
+    unsigned char *const rows = (RG == 4 ? s_kv : Vs) + rg * 32 * KP;
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            reinterpret_cast<uint2 *>(rows + k_unit(li, 4 * d + g))[lh] =
+            *reinterpret_cast<uint2 *>(rows + li * KP + 64 * d + 16 * g + 8 * lh) =
                 make_uint2(pack_h16<DT>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), pack_h16<DT>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 #pragma unroll
     for (int i = 0; i < 32 / ROWS; ++i) {
         const unsigned row = row0 + (unsigned) (i * ROWS + lane / UNITS), tk = div31(min(row, last_row), p.by_group);
-        const uint4 x = rows[k_unit(i * ROWS + lane / UNITS, lane % UNITS)];
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(rows + (i * ROWS + lane / UNITS) * KP + lane % UNITS * 16);
         if (row <= last_row)
-            *reinterpret_cast<uint4 *>(p.out + b * p.os[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.os[1] + tk * p.os[2] + lane % UNITS * 8) = x;
+            *reinterpret_cast<u32x4 *>(p.out + b * p.os[0] + (long long) (kvh * p.group + (int) (row - tk * (unsigned) p.group)) * p.os[1] + tk * p.os[2] + lane % UNITS * 8) = x;
     }
 }
 

@@ -34,8 +34,8 @@ struct MaskedParams {
     int blocks, splits;                     // row blocks of a key-value head; parts of the keys
     Div31 by_splits, by_heads, by_kv_heads, by_group;
     int spread;                             // the (batch, key-value head) pairs divide evenly among the XCDs
-    float scale2, cap2, to_cap, to_x;       // |scale| * log2(e); cap * log2(e); |scale| / cap * 2 log2(e); |scale| / cap
-    float tanh0, tanh1, tanh2, tanh3;       // cap2 times the coefficients of tanh(x) / x in x^2
+    float scale2;                           // |scale| * log2(e)
+    Cap cap;
     unsigned flip;                          // sign of the scale on q
     float *part_o, *part_ml;
 };
@@ -270,36 +270,18 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (GENERAL) {
-            if (p.cap2 > 0.0f) {   // uniform
-                float most = 0.0f;
+            if (p.cap.cap2 > 0.0f) {   // uniform
+                float x[16 * NT];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int i = 0; i < 16 * NT; ++i) x[i] = s[i / 16][i % 16];
+                cap_scores(p.cap, x);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[n][r]));
-                if (!__any(most * p.to_x > 0.5f)) {
-                    // where all scores are below half of the cap, as most are: tanh(x) = x P(x^2), P of degree 3 fitted to the smallest largest error up to
-                    // 0.5, 1.6 10^-7 in fp32; 24 cycles a score and not the 44 of an exponential and a reciprocal
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float x = s[n][r] * p.to_x, y = x * x;
-                            s[n][r] = x * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p.tanh3, y, p.tanh2), y, p.tanh1), y, p.tanh0);
-                        }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {   // tanh(x) = 1 - 2 / (e^2x + 1)
-                            const float e = __builtin_amdgcn_exp2f(s[n][r] * p.to_cap);
-                            s[n][r] = __builtin_fmaf(-2.0f * p.cap2, __builtin_amdgcn_rcpf(e + 1.0f), p.cap2);
-                        }
-                }
+                for (int i = 0; i < 16 * NT; ++i) s[i / 16][i % 16] = x[i];
             }
-            const float mul = p.cap2 > 0.0f ? 1.0f : p.scale2;
+            const float mul = p.cap.cap2 > 0.0f ? 1.0f : p.scale2;
             const float away = (float) (place - key0 - 4 * lh);   // of the lane's first key; the others follow at constant distances
             if (!p.slopes) {   // uniform
-                if (!(p.cap2 > 0.0f))
+                if (!(p.cap.cap2 > 0.0f))
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -506,7 +488,7 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg
     if (d->q_heads % d->kv_heads) return set_error(ONHIP_ERR_ARG, "masked attention: %d query heads for %d key-value heads", d->q_heads, d->kv_heads);
     if (d->k_tokens > MOST || d->q_tokens > MOST || d->q_offset > MOST || d->q_offset < -MOST) return set_error(ONHIP_ERR_ARG, "masked attention: lengths and places are at most 2^29");
     if (d->window < 0 || d->window > MOST) return set_error(ONHIP_ERR_ARG, "masked attention: a window of %d", d->window);
-    if (!(d->softcap >= 0.0f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.0f)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be finite, the cap not negative");
+    if (!cap_fits(d->scale, d->softcap)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be below 10^30 and finite, the cap not negative, their quotient between 10^-30 and 10^30");
     // 64 rows a workgroup where 128 give no more than one a compute unit (4096 causal tokens of 8 heads on one 91 -> 72 us, 2048 of 16 heads of 64 34.5 -> 27,
     // 77 of 12 7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us)
     const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads);
@@ -593,10 +575,7 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     p.by_group = make_div31((unsigned) p.group);
     p.flip = d->scale < 0.0f ? 0x80008000u : 0u;
     p.scale2 = fabsf(d->scale) * 1.44269504088896340736f;
-    p.cap2 = d->softcap * 1.44269504088896340736f;
-    p.to_cap = d->softcap > 0.0f ? fabsf(d->scale) / d->softcap * 2.0f * 1.44269504088896340736f : 0.0f;
-    p.to_x = d->softcap > 0.0f ? fabsf(d->scale) / d->softcap : 0.0f;
-    p.tanh0 = p.cap2 * 0.999997675f; p.tanh1 = p.cap2 * -0.333206564f; p.tanh2 = p.cap2 * 0.131451443f; p.tanh3 = p.cap2 * -0.0433724485f;
+    p.cap = make_cap(fabsf(d->scale), d->softcap);
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * p.splits * d->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);

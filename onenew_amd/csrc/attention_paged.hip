@@ -31,17 +31,12 @@ struct PagedParams {
     const float *slopes;
     long long table_stride;
     int table_pages, batch, q_heads, kv_heads, group, head_blocks, splits, window;
-    float scale2, cap2, to_cap;  // scale * log2(e); cap * log2(e); scale / cap * 2 log2(e)
+    float scale2;                // scale * log2(e)
+    Cap cap;
     float *part_o, *part_ml;
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
-
-// cap tanh(s scale / cap) log2(e): tanh(x) = 1 - 2 / (e^2x + 1), which is off by 2^-23 of the cap at most, a hundred-thousandth of a score of 50
-__device__ __forceinline__ float capped(float s, float to_cap, float cap2) {
-    const float e = __builtin_amdgcn_exp2f(s * to_cap);
-    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(e + 1.0f);
-}
 
 // SMALL: pages of fewer than 16 tokens (a tile then has a page a lane; else two pages, the same for all lanes)
 template <int DT, int HD, bool I8, bool SMALL>
@@ -227,7 +222,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 const int from_lane = 16 * (j / 4) + 4 * lg + j % 4;
-                ksc[j] = __shfl(x * (p.cap2 > 0.0f ? 1.0f : p.scale2), from_lane, 64);
+                ksc[j] = __shfl(x * (p.cap.cap2 > 0.0f ? 1.0f : p.scale2), from_lane, 64);
                 vsc[j] = __shfl(y, from_lane, 64);
             }
         }
@@ -262,9 +257,8 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[4 * a + r] = I8 ? acc[r] * ksc[4 * a + r] : acc[r];
         }
-        if (p.cap2 > 0.0f) {   // uniform
-#pragma unroll
-            for (int j = 0; j < NS; ++j) s[j] = capped(s[j], p.to_cap, p.cap2);
+        if (p.cap.cap2 > 0.0f) {   // uniform
+            cap_scores(p.cap, s);
         } else if constexpr (!I8) {
 #pragma unroll
             for (int j = 0; j < NS; ++j) s[j] *= p.scale2;
@@ -503,7 +497,7 @@ static int paged_check(const onhip_cache_desc_t *c, const onhip_paged_attention_
     if ((long long) d->batch * d->q_heads >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "paged attention: %d sequences of %d heads", d->batch, d->q_heads);
     if ((long long) d->table_pages * c->page_tokens > (1LL << 30)) return set_error(ONHIP_ERR_ARG, "paged attention: a table of %d pages", d->table_pages);
     if (d->window < 0) return set_error(ONHIP_ERR_ARG, "paged attention: a window of %d", d->window);
-    if (!(d->softcap >= 0.0f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.0f)) return set_error(ONHIP_ERR_ARG, "paged attention: scale and cap must be finite, the cap not negative");
+    if (!cap_fits(d->scale, d->softcap)) return set_error(ONHIP_ERR_ARG, "paged attention: scale and cap must be below 10^30 and finite, the cap not negative, their quotient between 10^-30 and 10^30");
     return ONHIP_OK;
 }
 
@@ -566,8 +560,7 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
     p.head_blocks = (p.group + 15) / 16;
     p.window = d->window;
     p.scale2 = d->scale * LOG2E;
-    p.cap2 = d->softcap * LOG2E;
-    p.to_cap = d->softcap > 0.0f ? d->scale / d->softcap * 2.0f * LOG2E : 0.0f;
+    p.cap = make_cap(d->scale, d->softcap);
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * p.splits * c->head_dim;
     const unsigned blocks = (unsigned) (d->batch * c->kv_heads * p.head_blocks * p.splits);

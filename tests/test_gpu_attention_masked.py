@@ -76,6 +76,32 @@ def test_scores_above_half_of_the_cap():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_cap_far_above_the_scores(dtype):
+    """is no cap: s - cap tanh(s / cap) = s^3 / (3 cap^2) is 10^-8 at most here, and the polynomial's 2.4 10^-6 |s| are within the bound's allowance
+    for a score, hd 2^-24 sum |q k| scale"""
+    hip.init(0)
+    q, k, v = _inputs(2, 4, 2, 50, 200, 64, DT[dtype])
+    for cap in (1e6, 1e25):
+        got = hip.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=0.125, causal=True, softcap=cap)
+        torch.cuda.synchronize()
+        _check(q, k, v, got, 0.125, True, 0, 0.0, None, 150, None)
+
+
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (16, 4)])
+def test_a_rows_bits_are_its_own(hq, hkv):
+    """whatever the scores of the rows beside it are"""
+    hip.init(0)
+    q, k, v = (x.cuda() for x in _inputs(1, hq, hkv, 100, 300, 64, torch.bfloat16))
+    more = q.clone()
+    more[:, 1::2] *= 40
+    more[:, :, 1::2] *= 40
+    for cap in (0.0, 8.0):
+        a, b = (hip.attention_masked(x, k, v, scale=0.125, causal=True, softcap=cap, merged_out=False) for x in (q, more))
+        torch.cuda.synchronize()
+        assert torch.equal(a[:, ::2, ::2], b[:, ::2, ::2]) and not torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_many_parts(dtype):
     _run(dtype, 1, 1, 1, 1, 70000, 64)
     _run(dtype, 1, 2, 1, 5, 33333, 128, window=20000)

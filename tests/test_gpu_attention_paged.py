@@ -81,6 +81,26 @@ def test_windows_caps_and_biases(dtype, int8, i):
     _run(dtype, int8, [0, 1, 32, 70, 333, 1500], 6, 2, 128 if i % 2 else 64, [4, 16, 64][i % 3], **MORE[i])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_cap_far_above_the_scores(dtype, int8):
+    """is no cap: s - cap tanh(s / cap) = s^3 / (3 cap^2) is 10^-8 at most here, and the polynomial's 2.4 10^-6 |s| are within the bound's allowance
+    for a score, hd 2^-24 sum |q k| scale; and a head's bits do not depend on the scores of the heads beside it"""
+    hip.init(0)
+    q, cache, table, n = _case([1, 70, 1500], 6, 2, 64, 16, DT[dtype], int8)
+    k, v, ks, vs = _dev(*cache)
+    run = lambda q, cap: hip.attention_paged(q.cuda(), k, v, table.cuda(), n.cuda(), scale=0.125, softcap=cap, k_scale=ks, v_scale=vs)
+    for cap in (1e6, 1e25):
+        got = run(q, cap)
+        torch.cuda.synchronize()
+        _check(got, q, cache, table, n, 0.125)
+    more = q.clone()
+    more[:, 1::2] *= 40
+    a, b = run(q, 8.0), run(more, 8.0)
+    torch.cuda.synchronize()
+    assert torch.equal(a[:, ::2], b[:, ::2]) and not torch.equal(a, b)
+
+
 def test_no_pages():
     hip.init(0)
     q, cache, _, _ = _case([5, 5], 4, 2, 64, 16, torch.float16, False)

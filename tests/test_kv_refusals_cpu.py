@@ -125,6 +125,8 @@ def test_paged():
     _refused(paged(table_pages=1 << 27), "table")
     for more in (dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(scale=float("inf")), dict(scale=float("nan"))):
         _refused(paged(**more), "finite")
+    for more in (dict(softcap=1e30), dict(softcap=1e-31), dict(scale=1e-10, softcap=1e25), dict(scale=-1e30)):
+        _refused(paged(**more), "quotient")
     for more in (dict(q_strides=(256, 60)), dict(out_strides=(256, -64)), dict(q_strides=(100, 64), batch=2)):
         _refused(paged(**more), "multiples of 8")
     _refused(paged(out_strides=(256, 0)), "overlap")
@@ -163,6 +165,8 @@ def test_masked():
     _refused(masked(q_tokens=1 << 29, q_heads=8), "too many rows")
     for more in (dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(scale=float("inf")), dict(scale=float("nan"))):
         _refused(masked(**more), "finite")
+    for more in (dict(softcap=1e30), dict(softcap=1e-31), dict(scale=1e-10, softcap=1e25), dict(scale=-1e30)):
+        _refused(masked(**more), "quotient")
     for name in ("q_strides", "k_strides", "v_strides", "out_strides"):
         _refused(masked(**{name: (2048, 64, 252)}), "multiples of 8")
         _refused(masked(batch=2, **{name: (-2048, 64, 256)}), "non-negative")

@@ -32,6 +32,8 @@ inline bool cap_fits(float scale, float cap) {
     if (!(s < 1e30f) || !(cap >= 0.0f) || !(cap < 1e30f)) return false;
     return cap == 0.0f || s == 0.0f || (s / cap > 1e-30f && s / cap < 1e30f);
 }
+// a slope of 10^28 leaves one key to a row as a larger one does, and times a distance stays in fp32's range
+__device__ __forceinline__ float slope_within(float x) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -1e28f, 1e28f); }
 __device__ __forceinline__ float cap_near(const Cap &c, float s) {
     const float x = s * c.to_x, y = x * x;
     return x * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c.tanh3, y, c.tanh2), y, c.tanh1), y, c.tanh0);

@@ -18,7 +18,7 @@
 // between the second product's matrix instructions), LDS 1300 for operands and staging; two workgroups a compute unit overlap them to 50 % of
 // each, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 540 us, 1.0 PFLOP/s where a large library product
 // reaches 1.2.  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 101 us.  Short rows are bound by a
-// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 45 us (their 67 MB take 13).  Tiles of 32 keys with
+// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 43 us (their 67 MB take 13).  Tiles of 32 keys with
 // three workgroups a compute unit, eight operands ahead and a higher wave priority in the products were level.
 #include "attention_join.hpp"
 
@@ -34,7 +34,7 @@ struct MaskedParams {
     int blocks, splits;                     // row blocks of a key-value head; parts of the keys
     Div31 by_splits, by_heads, by_kv_heads, by_group;
     int spread;                             // the (batch, key-value head) pairs divide evenly among the XCDs
-    float scale2;                           // |scale| * log2(e)
+    float scale2, far;                      // |scale| * log2(e); how far a score may lie above the reference point, 8 in units of the scores
     Cap cap;
     unsigned flip;                          // sign of the scale on q
     float *part_o, *part_ml;
@@ -189,14 +189,19 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     auto mixed = [&](int t) __attribute__((always_inline)) { return t * KT < wg_all_lo || t * KT + KT > wg_all_hi; };
     auto put = [&](int buf, bool clean) __attribute__((always_inline)) {
         if (clean) {   // uniform
+            constexpr unsigned EXP = DT == DT_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = EXP & ~(EXP << 1);   // the exponents, and one in each: the sum's top bits are their carries
+            unsigned any = 0u;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const unsigned x = v_reg[i][j], y = finite_of<DT>(x);
-                    odd |= x ^ y;
-                    v_reg[i][j] = y;
-                }
+                for (int j = 0; j < 4; ++j) any |= (v_reg[i][j] & EXP) + ONE;
+            if (__any((any & 0x80008000u) != 0u)) {
+                odd = 1u;
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v_reg[i][j] = finite_of<DT>(v_reg[i][j]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -240,8 +245,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     for (int d = 0; d < DTILES; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    const float unit = GENERAL ? 1.0f : p.scale2;   // of the scores and of m, in units of the exponential base 2
     float m = -INFINITY, l = 0.0f;
-    const float slope2 = GENERAL && p.slopes ? p.slopes[head] * 1.44269504088896340736f : 0.0f;
+    const float slope2 = GENERAL && p.slopes ? slope_within(p.slopes[head] * 1.44269504088896340736f) : 0.0f;
 
     auto tile = [&](int t, int buf) __attribute__((always_inline)) {
         const int key0 = t * KT + 32 * kh;   // the wavefront's part of the tile: 32 NT keys
@@ -299,13 +305,18 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
                     for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], mul, -slope2 * fabsf(away - (float) (32 * n + 8 * (r / 4) + r % 4)));
             }
         }
-        if (!whole) {
-            const unsigned span = (unsigned) (hi - lo);
+        if (!whole) {   // the row's interval as bits of the lane's keys: two instructions a score
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                const int from = key0 + 32 * n + 4 * lh;
+                auto below = [](int x) __attribute__((always_inline)) { return (1u << min(max(x, 0), 31)) - 1u; };   // bits up to 27 count
+                const unsigned seen = below(hi - from) & ~below(lo - from);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((unsigned) (key0 + 32 * n + 8 * (r / 4) + 4 * lh + r % 4 - lo) >= span) s[n][r] = -INFINITY;
+                for (int r = 0; r < 16; ++r) {
+                    const unsigned keep = (unsigned) ((int) (seen << (31 - (8 * (r / 4) + r % 4))) >> 31);
+                    s[n][r] = __uint_as_float((__float_as_uint(s[n][r]) & keep) | (0xff800000u & ~keep));
+                }
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -313,10 +324,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if constexpr (!GENERAL) top *= p.scale2;
-        const bool far = top > m + 8.0f;   // each row by itself: its bits do not depend on the rows beside it
+        const bool far = top > m + p.far;   // each row by itself: its bits do not depend on the rows beside it
         if (__any(far)) {
-            const float next = far ? top : m, fade = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+            const float next = far ? top : m, fade = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.0f : next)) * unit);
             m = next;
             l *= fade;
 #pragma unroll
@@ -324,7 +334,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
-        const float shift = m == -INFINITY ? 0.0f : SHIFT - m;
+        float shift = m == -INFINITY ? 0.0f : __builtin_fmaf(-m, unit, SHIFT);
+        if constexpr (!GENERAL)
+            if (__any(fabsf(shift) > 65536.0f)) {   // the fused product would count the rounding of m scale2: such rows' scores have m taken off first
+                const bool high = fabsf(shift) > 65536.0f;
+                const float from = high ? m : 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] -= from;
+                shift = high ? SHIFT : shift;
+            }
         constexpr int PRODUCTS = 2 * DTILES;   // of 32 keys
         auto v_ask = [&](int i) __attribute__((always_inline)) { return v_frag(buf, i / PRODUCTS + kh, i % PRODUCTS / DTILES, i % DTILES); };
 #pragma unroll
@@ -367,9 +387,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         }
     }
 
-    if (__any(odd != 0u) && lane == 0) s_odd = 1;
+    if (odd && lane == 0) s_odd = 1;
     __syncthreads();
     l += __shfl_xor(l, 32, 64);
+    m *= unit;
     if constexpr (RG == 2) {   // the two halves of the keys: the second wavefront's results to the first
         float *const half = reinterpret_cast<float *>(s_kv) + rg * (DTILES * 16 + 2) * 64 + lane;
         static_assert(2 * (DTILES * 16 + 2) * 64 * 4 <= 2 * KT * KP, "two row groups, in the place of k");
@@ -579,7 +600,8 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * p.splits * d->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const bool general = d->softcap > 0.0f || slopes || p.scale2 == 0.0f;
+    const bool general = d->softcap > 0.0f || slopes || fabsf(d->scale) < 1e-6f;   // 8 / scale2 stays far from the end of fp32's range
+    p.far = general ? 8.0f : 8.0f / p.scale2;
     auto by_size = [&]<int DT>() { return d->head_dim == 64 ? masked_launch<DT, 64>(p, rg, general, st) : masked_launch<DT, 128>(p, rg, general, st); };
     const int done = dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
     if (done || p.splits == 1) return done;

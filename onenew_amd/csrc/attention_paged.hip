@@ -85,7 +85,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
         const int d = I8 ? st / 2 * 64 + lg * 16 + st % 2 * 8 : st * 32 + lg * 8;
         if (live) qf[st] = *reinterpret_cast<const uint4 *>(p.q + b * p.qs[0] + qh * p.qs[1] + d);
     }
-    const float slope2 = p.slopes && live ? p.slopes[qh] * LOG2E : 0.0f;
+    const float slope2 = p.slopes && live ? slope_within(p.slopes[qh] * LOG2E) : 0.0f;
 
     auto mfma = []<int T>(const uint4 &x, const uint4 &y, f32x4 c) __attribute__((always_inline)) {
         if constexpr (T == DT_BF16)

@@ -101,6 +101,46 @@ def test_a_rows_bits_are_its_own(hq, hkv):
         assert torch.equal(a[:, ::2, ::2], b[:, ::2, ::2]) and not torch.equal(a, b)
 
 
+@pytest.mark.parametrize("scale", [1e-5, 1e-7, -0.02, 30.0])
+@pytest.mark.parametrize("causal", [True, False])
+def test_biases_next_to_small_and_large_scales(causal, scale):
+    for dtype, hd in (("bf16", 64), ("f16", 128)):
+        _run(dtype, 2, 4, 2, 200, 300, hd, scale=scale, causal=causal, bias=True, window=150)
+        _run(dtype, 3, 16, 16, 700, 700, hd, scale=scale, causal=causal, bias=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_slopes_that_leave_one_key(dtype):
+    """with slopes from 200 on a key's probability is below 2^-280 of the next one's (scores differ by less than 10): the row's own place alone"""
+    hip.init(0)
+    q, k, v = _inputs(1, 4, 2, 90, 90, 64, DT[dtype])
+    slopes = torch.tensor([200.0, 1e10, 1e30, 3e37])
+    got = hip.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=0.01, causal=True, slopes=slopes.cuda(), merged_out=False)
+    torch.cuda.synchronize()
+    assert torch.equal(got.cpu(), v.repeat_interleave(2, dim=1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,merged", [(100, 1), (100, 30)])
+def test_scores_of_any_size(dtype, tokens, merged):
+    """a row's largest score lies 10^9 above the next one: its own key alone, beside rows of ordinary scores"""
+    hip.init(0)
+    q, k, v = _inputs(merged, 16, 8, tokens, tokens, 64, DT[dtype])
+    q[:, ::2] = 0.0
+    q[:, ::2, :, 0] = 60000.0
+    k[..., 0] = torch.arange(tokens) * 512.0    # a number of seven bits
+    q[:, 1::2, :, 0] = 0.0
+    for bias in (None, torch.full((16,), 1.0)):
+        got = hip.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=40.0, causal=True, slopes=None if bias is None else bias.cuda(), merged_out=False)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:, ::2].cpu(), v)
+        assert bool(got.isfinite().all())
+        even = torch.arange(0, 16, 2)
+        seen, away = kv_oracle.seen_by(tokens, tokens, True, 0, 0)
+        ref, bound = kv_oracle.attention(q[0, even + 1], k[0], v[0], seen, 40.0, 0.0, None if bias is None else bias[even + 1], away)
+        assert bool(((got[0, even + 1].double().cpu() - ref).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_many_parts(dtype):
     _run(dtype, 1, 1, 1, 1, 70000, 64)

@@ -101,6 +101,19 @@ def test_a_cap_far_above_the_scores(dtype, int8):
     assert torch.equal(a[:, ::2], b[:, ::2]) and not torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_slopes_that_leave_one_key(dtype):
+    """with slopes from 200 on a key's probability is below 2^-280 of the next one's (scores differ by less than 10): the new token's alone"""
+    hip.init(0)
+    q, cache, table, n = _case([1, 70, 1500], 6, 2, 64, 16, DT[dtype], False)
+    k, v = _dev(*cache[:2])
+    slopes = torch.tensor([200.0, 1e10, 1e30, 3e37, 3e38, 300.0])
+    got = hip.attention_paged(q.cuda(), k, v, table.cuda(), n.cuda(), scale=0.01, slopes=slopes.cuda())
+    torch.cuda.synchronize()
+    for b, m in enumerate(n.tolist()):
+        assert torch.equal(got[b].double().cpu(), kv_oracle.rows(cache[1], None, table[b], m)[:, -1].repeat_interleave(3, dim=0))
+
+
 def test_no_pages():
     hip.init(0)
     q, cache, _, _ = _case([5, 5], 4, 2, 64, 16, torch.float16, False)

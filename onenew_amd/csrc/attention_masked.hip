@@ -18,7 +18,7 @@
 // between the second product's matrix instructions), LDS 1300 for operands and staging; two workgroups a compute unit overlap them to 50 % of
 // each, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 540 us, 1.0 PFLOP/s where a large library product
 // reaches 1.2.  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 101 us.  Short rows are bound by a
-// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 43 us (their 67 MB take 13).  Tiles of 32 keys with
+// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 us (their 67 MB take 13).  Tiles of 32 keys with
 // three workgroups a compute unit, eight operands ahead and a higher wave priority in the products were level.
 #include "attention_join.hpp"
 
@@ -34,7 +34,7 @@ struct MaskedParams {
     int blocks, splits;                     // row blocks of a key-value head; parts of the keys
     Div31 by_splits, by_heads, by_kv_heads, by_group;
     int spread;                             // the (batch, key-value head) pairs divide evenly among the XCDs
-    float scale2, far;                      // |scale| * log2(e); how far a score may lie above the reference point, 8 in units of the scores
+    float scale2, per_scale, far;           // |scale| * log2(e); 1 / |scale|; how far a score may lie above the reference point, 8 in units of the scores
     Cap cap;
     unsigned flip;                          // sign of the scale on q
     float *part_o, *part_ml;
@@ -57,10 +57,14 @@ template <int DT> __device__ __forceinline__ unsigned finite_of(unsigned w) {
     return ((w & INF) == INF ? 0u : w & 0xffffu) | ((w >> 16 & INF) == INF ? 0u : w & 0xffff0000u);
 }
 
-// GENERAL: scores are capped or biased, or the scale is zero (else one fused product takes them into the exponential)
+// HOW the scores become exponents.  PLAIN: one fused product takes them there.  BIASED: as that, where every key that counts lies behind its query, so that the
+// bias is slope / scale times (the key's number - the row's place): one more matrix instruction, of the number in the tile of 64 (a whole number) and of one
+// with the quotient and the rest in three bf16 parts each, all of their 24 bits (documents of 16 heads 40 us, as GENERAL 43).  GENERAL: capped, a
+// bias on keys on both sides, or a scale of (nearly) zero.
+enum { PLAIN, BIASED, GENERAL };
 // RG: groups of 32 rows of a workgroup.  4: a wavefront has all keys of a tile for its rows.  2: two wavefronts share the rows, one has the first 32 keys of
 // every tile, one the others, and their results are joined in the end.
-template <int DT, int HD, bool GENERAL, int RG>
+template <int DT, int HD, int HOW, int RG>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel(const MaskedParams p) {
     constexpr int KT = 64, NT = RG == 4 ? 2 : 1, STEPS = HD / 16, DTILES = HD / 32;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
@@ -245,9 +249,32 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     for (int d = 0; d < DTILES; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-    const float unit = GENERAL ? 1.0f : p.scale2;   // of the scores and of m, in units of the exponential base 2
+    const float unit = HOW == GENERAL ? 1.0f : p.scale2;   // of the scores and of m, in units of the exponential base 2
     float m = -INFINITY, l = 0.0f;
-    const float slope2 = GENERAL && p.slopes ? slope_within(p.slopes[head] * 1.44269504088896340736f) : 0.0f;
+    const float slope2 = HOW == GENERAL && p.slopes ? slope_within(p.slopes[head] * 1.44269504088896340736f) : 0.0f;
+    // BIASED: keys' numbers in the channels 0 .. 2 and ones in 3 .. 5 times the parts of the quotient and of the rest
+    const float ratio = HOW == BIASED ? slope_within(p.slopes[head] * p.per_scale) : 0.0f;
+    uint4 numbers[NT], quotient = make_uint4(0u, 0u, 0u, 0u);
+    auto parts_of = [](float x, unsigned (&part)[3]) __attribute__((always_inline)) {   // x as a sum of three bf16, in the upper halves
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            part[i] = __float_as_uint(x) & 0xffff0000u;
+            x -= __uint_as_float(part[i]);
+        }
+    };
+    if constexpr (HOW == BIASED) {
+        unsigned part[3];
+        parts_of(ratio, part);
+        if (lh == 0) {
+            quotient.x = part[0] >> 16 | part[1];
+            quotient.y = part[2] >> 16;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const unsigned number = __float_as_uint((float) (32 * n + li)) >> 16;
+            numbers[n] = make_uint4(number | number << 16, number | 0x3f800000u, 0x3f803f80u, 0u);   // times zeros in the lanes 32 ..
+        }
+    }
 
     auto tile = [&](int t, int buf) __attribute__((always_inline)) {
         const int key0 = t * KT + 32 * kh;   // the wavefront's part of the tile: 32 NT keys
@@ -261,6 +288,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
+        if constexpr (HOW == BIASED) {
+            unsigned part[3];
+            parts_of(lh == 0 ? ratio * (float) (key0 - place) : 0.0f, part);
+            const uint4 by = make_uint4(quotient.x, quotient.y | part[0], part[1] >> 16 | part[2], 0u);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, numbers[n]), __builtin_bit_cast(bf16x8, by), s[n], 0, 0, 0);
+        }
         const unsigned char *const k_at = s_kv + (buf * KT + 32 * kh + li) * KP + lh * 16;
         auto k_frag = [&](int i) __attribute__((always_inline)) {
             return __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4 *>(k_at + i / STEPS * 32 * KP + i % STEPS * 32));
@@ -275,7 +309,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
             if (i + AHEAD < NT * STEPS) ring[i % AHEAD] = k_frag(i + AHEAD);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (GENERAL) {
+        if constexpr (HOW == GENERAL) {
             if (p.cap.cap2 > 0.0f) {   // uniform
                 float x[16 * NT];
 #pragma unroll
@@ -335,7 +369,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         float shift = m == -INFINITY ? 0.0f : __builtin_fmaf(-m, unit, SHIFT);
-        if constexpr (!GENERAL)
+        if constexpr (HOW != GENERAL)
             if (__any(fabsf(shift) > 65536.0f)) {   // the fused product would count the rounding of m scale2: such rows' scores have m taken off first
                 const bool high = fabsf(shift) > 65536.0f;
                 const float from = high ? m : 0.0f;
@@ -352,8 +386,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         __builtin_amdgcn_sched_barrier(0);
         unsigned pk[NT][8];
         auto weigh = [&](int n, int j) __attribute__((always_inline)) {   // two probabilities
-            const float x = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j] + shift : __builtin_fmaf(s[n][2 * j], p.scale2, shift));
-            const float y = __builtin_amdgcn_exp2f(GENERAL ? s[n][2 * j + 1] + shift : __builtin_fmaf(s[n][2 * j + 1], p.scale2, shift));
+            const float x = __builtin_amdgcn_exp2f(HOW == GENERAL ? s[n][2 * j] + shift : __builtin_fmaf(s[n][2 * j], p.scale2, shift));
+            const float y = __builtin_amdgcn_exp2f(HOW == GENERAL ? s[n][2 * j + 1] + shift : __builtin_fmaf(s[n][2 * j + 1], p.scale2, shift));
             pk[n][j] = pack_h16<DT>(x, y);
             // the sum is of the rounded ones: what rounding adds to all of a row's weights is divided out again
             if constexpr (DT == DT_BF16) l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk[n][j]), bf16x2{(__bf16) 1.0f, (__bf16) 1.0f}, l, false);
@@ -521,13 +555,11 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg
     return ONHIP_OK;
 }
 
-template <int DT, int HD>
-static int masked_launch(const MaskedParams &p, int rg, bool general, hipStream_t stream) {
+template <int DT, int HD, int HOW>
+static int masked_launch(const MaskedParams &p, int rg, hipStream_t stream) {
     const dim3 grid((unsigned) p.batch * p.kv_heads * p.blocks * p.splits);
-    if (rg == 2 && general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true, 2>), grid, dim3(256), 0, stream, p);
-    else if (rg == 2) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false, 2>), grid, dim3(256), 0, stream, p);
-    else if (general) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, true, 4>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, false, 4>), grid, dim3(256), 0, stream, p);
+    if (rg == 2) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, HOW, 2>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, HOW, 4>), grid, dim3(256), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
@@ -600,9 +632,14 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * p.splits * d->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const bool general = d->softcap > 0.0f || slopes || fabsf(d->scale) < 1e-6f;   // 8 / scale2 stays far from the end of fp32's range
-    p.far = general ? 8.0f : 8.0f / p.scale2;
-    auto by_size = [&]<int DT>() { return d->head_dim == 64 ? masked_launch<DT, 64>(p, rg, general, st) : masked_launch<DT, 128>(p, rg, general, st); };
+    const bool usual = d->softcap == 0.0f && fabsf(d->scale) >= 1e-6f;   // a quotient of slope and scale stays in fp32's range
+    p.per_scale = usual ? 1.0f / fabsf(d->scale) : 0.0f;
+    p.far = usual && (!slopes || d->causal) ? 8.0f / p.scale2 : 8.0f;
+    auto by_how = [&]<int DT, int HD>() {
+        if (usual && !slopes) return masked_launch<DT, HD, PLAIN>(p, rg, st);
+        return usual && d->causal ? masked_launch<DT, HD, BIASED>(p, rg, st) : masked_launch<DT, HD, GENERAL>(p, rg, st);
+    };
+    auto by_size = [&]<int DT>() { return d->head_dim == 64 ? by_how.template operator()<DT, 64>() : by_how.template operator()<DT, 128>(); };
     const int done = dt == DT_BF16 ? by_size.template operator()<DT_BF16>() : by_size.template operator()<DT_F16>();
     if (done || p.splits == 1) return done;
     JoinParams j;

@@ -5,7 +5,7 @@
 // [begin, end) (documents of a packed batch, prefixes, lengths) are intersected once.  Tiles outside the union of a workgroup's intervals
 // are not touched, tiles inside the intersection of a wavefront's are computed without a mask.
 //
-// Rows: a workgroup has 128 rows of one key-value head, (token, head of the group) with the head running fastest, so that heads that share
+// Rows: a workgroup has 64, 128 or 256 rows of one key-value head, (token, head of the group) with the head running fastest, so that heads that share
 // keys share the tiles that are staged.  A wavefront has 32 of them and computes the transposed scores S^T = k q^T with
 // v_mfma_f32_32x32x16, so a lane owns one row and, per 32 keys, the 16 keys 8 (r / 4) + 4 (lane / 32) + r % 4; its softmax is the lane's own, and the
 // probabilities feed out^T = v^T P^T from the registers they are in.  Tiles of 64 keys of k and v go through LDS in two buffers, v
@@ -15,11 +15,11 @@
 // 2^8 above it, so that most tiles leave the sums alone).  Scores, maxima, sums and products' sums are fp32.
 //
 // What bounds it: per tile of 64 keys the matrix instructions take 1024 cycles of a SIMD, the softmax's vector instructions as many (half of the exponentials run
-// between the second product's matrix instructions), LDS 1300 for operands and staging; two workgroups a compute unit overlap them to 50 % of
-// each, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 540 us, 1.0 PFLOP/s where a large library product
-// reaches 1.2.  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 101 us.  Short rows are bound by a
+// between the second product's matrix instructions), LDS 1300 for operands and staging; two wavefronts a SIMD overlap them to half of the
+// time, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 500 to 535 us, 1.02 to 1.10 PFLOP/s where a large library
+// product reaches 1.2 (540 to 565 with a tile staged for 128 rows, not 256).  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 99 us.  Short rows are bound by a
 // workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 us (their 67 MB take 13).  Tiles of 32 keys with
-// three workgroups a compute unit, eight operands ahead and a higher wave priority in the products were level.
+// three workgroups a compute unit, eight operands ahead, a higher wave priority in the products, and 256 rows on four buffers with a barrier every second tile were level.
 #include "attention_join.hpp"
 
 namespace onhip {
@@ -62,25 +62,25 @@ template <int DT> __device__ __forceinline__ unsigned finite_of(unsigned w) {
 // with the quotient and the rest in three bf16 parts each, all of their 24 bits (documents of 16 heads 40 us, as GENERAL 43).  GENERAL: capped, a
 // bias on keys on both sides, or a scale of (nearly) zero.
 enum { PLAIN, BIASED, GENERAL };
-// RG: groups of 32 rows of a workgroup.  4: a wavefront has all keys of a tile for its rows.  2: two wavefronts share the rows, one has the first 32 keys of
+// RG: groups of 32 rows of a workgroup.  4 and 8: a wavefront has all keys of a tile for its rows.  2: two wavefronts share the rows, one has the first 32 keys of
 // every tile, one the others, and their results are joined in the end.
 template <int DT, int HD, int HOW, int RG>
-__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel(const MaskedParams p) {
-    constexpr int KT = 64, NT = RG == 4 ? 2 : 1, STEPS = HD / 16, DTILES = HD / 32;
+__global__ __launch_bounds__(RG == 8 ? 512 : 256, HD == 64 ? 3 : 2) void attention_masked_kernel(const MaskedParams p) {
+    constexpr int KT = 64, NT = RG >= 4 ? 2 : 1, NWV = RG == 8 ? 8 : 4, STEPS = HD / 16, DTILES = HD / 32;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
     constexpr float SHIFT = DT == DT_BF16 ? -24.0f : 7.0f;
     constexpr int UNITS = HD / 8, ROWS = 64 / UNITS;           // 16-byte units of a row; rows that a wavefront's load covers
-    constexpr int LOADS = KT / ROWS / 4;                       // loads of a wavefront for its share of a tile of k (or v)
+    constexpr int LOADS = KT / ROWS / NWV;                       // loads of a wavefront for its share of a tile of k (or v)
     // Two tiles of k, two of v.  Rows have a pitch by which 16 lanes that take one 16-byte unit of 16 rows of k, and the transposing read's 64 bytes of four rows
     // of v, meet every bank once, and a read's place in its row is a constant of the instruction (units exchanged by row number cost an address register each).
     constexpr int KP = HD * 2 + 16, VP = HD * 2 + 64;
     __shared__ __attribute__((aligned(16))) unsigned char s_kv[2 * KT * (KP + VP)];
     unsigned char *const Vs = s_kv + 2 * KT * KP;
-    __shared__ int4 s_span[4];
+    __shared__ int4 s_span[NWV];
     __shared__ int s_odd;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 31, lh = lane >> 5, rg = RG == 4 ? wave : wave >> 1, kh = RG == 4 ? 0 : wave & 1;
+    const int li = lane & 31, lh = lane >> 5, rg = RG >= 4 ? wave : wave >> 1, kh = RG >= 4 ? 0 : wave & 1;
     // item -> (batch, key-value head, row block, part).  Workgroups go to the XCDs in turn; where the heads divide among them, an XCD has whole
     // heads, so that its L2 holds their keys.  The last row blocks, which see most keys under a causal mask, start first; where all items find room at
     // once, a compute unit's second one is from the other end, so that its two (or three) together are no longer than another's.
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
             units = 32u;
         }
         const unsigned items = heads * (unsigned) (p.blocks * p.splits);
-        if (items <= units * (HD == 64 ? 3u : 2u) && local >= units) local = local < 2u * units ? items - 1u - (local - units) : local - units;
+        if (items <= units * (RG == 8 ? 1u : HD == 64 ? 3u : 2u) && local >= units) local = local < 2u * units ? items - 1u - (local - units) : local - units;
         const unsigned per_split = div31(local, p.by_splits);
         split = (int) (local - per_split * (unsigned) p.splits);
         const unsigned from_end = div31(per_split, p.by_heads);
@@ -143,7 +143,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
         all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         if (lane == 0) s_span[wave] = make_int4(any_lo, any_hi, all_lo, all_hi);
         __syncthreads();
-        const int4 x = s_span[0], y = s_span[1], z = s_span[2], w = s_span[3];
+        int4 x = s_span[0], y = s_span[1], z = s_span[2], w = s_span[3];
+        if constexpr (RG == 8) {
+            auto both = [](const int4 &a, const int4 &b) __attribute__((always_inline)) { return make_int4(min(a.x, b.x), max(a.y, b.y), max(a.z, b.z), min(a.w, b.w)); };
+            x = both(x, s_span[4]);
+            y = both(y, s_span[5]);
+            z = both(z, s_span[6]);
+            w = both(w, s_span[7]);
+        }
         wg_lo = __builtin_amdgcn_readfirstlane(min(min(x.x, y.x), min(z.x, w.x)));
         wg_hi = __builtin_amdgcn_readfirstlane(max(max(x.y, y.y), max(z.y, w.y)));
         wg_all_lo = __builtin_amdgcn_readfirstlane(max(max(x.z, y.z), max(z.z, w.z)));
@@ -233,17 +240,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     };
 
     if (t_begin < t_end) fetch(t_begin);
-    // q on into the channels 16 s + 8 (lane / 32) .. + 7 of step s, through the wavefront's part of the second buffers
+    // q on into the channels 16 s + 8 (lane / 32) .. + 7 of step s, through the wavefront's part of the second buffers (RG 8: of both)
     uint4 qf[STEPS];
     {
-        unsigned char *const rows = KT == 32 ? s_kv + wave * 32 * KP : (wave < 2 ? s_kv + KT * KP : Vs + KT * VP) + (wave & 1) * 32 * KP;
+        unsigned char *const rows = RG == 8 ? s_kv + wave * 32 * KP : (wave < 2 ? s_kv + KT * KP : Vs + KT * VP) + (wave & 1) * 32 * KP;
 #pragma unroll
         for (int i = 0; i < 32 / ROWS; ++i)
             *reinterpret_cast<u32x4 *>(rows + (i * ROWS + lane / UNITS) * KP + lane % UNITS * 16) = qr[i] ^ u32x4{p.flip, p.flip, p.flip, p.flip};
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) qf[st] = __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4 *>(rows + li * KP + lh * 16 + st * 32));
     }
-    if (KT == 32) __syncthreads();   // every part of the buffers was some wavefront's
+    if (RG == 8) __syncthreads();   // the first buffers were some wavefronts' parts
     f32x16 o[DTILES];
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
@@ -506,7 +513,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void attention_masked_kernel
     }
     // the result as q came, through LDS: whole rows to memory (in the place of k, or of v where the halves of the keys are joined in that)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    unsigned char *const rows = (RG == 4 ? s_kv : Vs) + rg * 32 * KP;
+    unsigned char *const rows = (RG >= 4 ? s_kv : Vs) + rg * 32 * KP;
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
 #pragma unroll
@@ -544,12 +551,18 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg
     if (d->k_tokens > MOST || d->q_tokens > MOST || d->q_offset > MOST || d->q_offset < -MOST) return set_error(ONHIP_ERR_ARG, "masked attention: lengths and places are at most 2^29");
     if (d->window < 0 || d->window > MOST) return set_error(ONHIP_ERR_ARG, "masked attention: a window of %d", d->window);
     if (!cap_fits(d->scale, d->softcap)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be below 10^30 and finite, the cap not negative, their quotient between 10^-30 and 10^30");
+    const long long heads = (long long) d->batch * d->q_heads;
+    if (heads >= (1LL << 31) || heads * d->q_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
     // 64 rows a workgroup where 128 give no more than one a compute unit (4096 causal tokens of 8 heads on one 91 -> 72 us, 2048 of 16 heads of 64 34.5 -> 27,
-    // 77 of 12 7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us)
-    const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads);
-    *rg = (total + 127) / 128 * d->batch * d->kv_heads <= 256 ? 2 : 4;
+    // 77 of 12 7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us).  256 rows, for which a tile is staged half as
+    // often, with head dimension 128 where workgroups, one a compute unit, fill seven eighths of their rounds and blocks are no more than a sixteenth larger than the
+    // rows (4096 causal tokens of 32 heads 162 -> 141 us, 4096 on 16384 keys 970 -> 873; 2560 causal tokens, 320 workgroups in 512 places, 74 and 77, 16 x 260 of 32 heads on 32 46 and 59; 8192 of 16 heads of
+    // 64, whose registers give way, 182 and 214)
+    const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads), pairs = (long long) d->batch * d->kv_heads;
+    const long long most = (total + 255) / 256, rounds = (most * pairs + 255) / 256;
+    *rg = (total + 127) / 128 * pairs <= 256 ? 2 : d->head_dim == 128 && most * 256 <= total + total / 16 && most * pairs * 8 >= rounds * 256 * 7 && rounds > 1 ? 8 : 4;
     const long long n = (total + 32 * *rg - 1) / (32 * *rg);
-    if (n * d->batch * d->kv_heads >= (1LL << 22) || (long long) d->batch * d->q_heads * d->q_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
+    if (n * pairs >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
     *blocks = (int) n;
     *splits = masked_splits(d, n);
     return ONHIP_OK;
@@ -558,6 +571,12 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg
 template <int DT, int HD, int HOW>
 static int masked_launch(const MaskedParams &p, int rg, hipStream_t stream) {
     const dim3 grid((unsigned) p.batch * p.kv_heads * p.blocks * p.splits);
+    if constexpr (HD == 128)
+        if (rg == 8) {
+            hipLaunchKernelGGL((attention_masked_kernel<DT, HD, HOW, 8>), grid, dim3(512), 0, stream, p);
+            ONHIP_CHECK_HIP(hipGetLastError());
+            return ONHIP_OK;
+        }
     if (rg == 2) hipLaunchKernelGGL((attention_masked_kernel<DT, HD, HOW, 2>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((attention_masked_kernel<DT, HD, HOW, 4>), grid, dim3(256), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());

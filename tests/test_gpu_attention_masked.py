@@ -68,6 +68,25 @@ def test_many_rows(dtype, i):
     _run(dtype, b, hq, hkv, tq, tk, hd, causal=i % 2 == 0, ranges=edge, q_offset=tk // 2)
 
 
+# workgroups of 256 rows: a block of heads of one key-value head that is (nearly) 256 rows, and 448 to 512 or 1792 to 2048 of them
+WIDE = [(56, 8, 8, 250, 300), (61, 16, 8, 128, 77), (4, 32, 8, 1001, 1001), (30, 30, 15, 128, 400), (120, 16, 16, 256, 70)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("i", range(len(WIDE)))
+def test_blocks_of_256_rows(dtype, i):
+    b, hq, hkv, tq, tk = WIDE[i]
+    _run(dtype, b, hq, hkv, tq, tk, 128, causal=i % 2 == 0)
+    if i == 2:
+        _run(dtype, b, hq, hkv, tq, tk, 128, bias=True)
+        return
+    _run(dtype, b, hq, hkv, tq, tk, 128, window=40, cap=20.0, bias=i % 2 == 0)
+    _run(dtype, b, hq, hkv, tq, tk, 128, bias=True, window=0 if i else 90)
+    g = torch.Generator().manual_seed(i)
+    edge = torch.randint(-20, tk + 20, (b, tq, 2), generator=g, dtype=torch.int32)
+    _run(dtype, b, hq, hkv, tq, tk, 128, causal=i % 2 == 0, ranges=edge, q_offset=tk // 2)
+
+
 def test_scores_above_half_of_the_cap():
     """capped by a polynomial below, by an exponential above"""
     for scale in (0.05, 0.3, 1.0, 5.0, -2.0):
@@ -189,7 +208,7 @@ def test_ranges(dtype, tq, tk, causal):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("tq,tk,b", [(100, 100, 1), (20, 2000, 1), (100, 150, 300)])
+@pytest.mark.parametrize("tq,tk,b", [(100, 100, 1), (20, 2000, 1), (100, 150, 300), (125, 190, 460)])
 def test_unseen_values(dtype, hd, tq, tk, b):
     """what a row does not see leaves its bits alone, infinities and NaN of k and v included; what it sees does not"""
     hip.init(0)

@@ -2,14 +2,14 @@
 // over the keys j of [max(0, len - window), len), in one pass over the cache with the running maximum and sum of a softmax.
 //
 // Up to 16 query heads that share a key-value head are the columns of the matrix instructions (v_mfma_f32_16x16x32), so the cache is read
-// once for all of them.  A wavefront takes tiles of 32 or 64 keys by itself, with no barrier until its end: S^T = K q^T, whose result leaves a
+// once for all of them.  A wavefront takes tiles of 32 keys by itself, with no barrier until its end: S^T = K q^T, whose result leaves a
 // lane with a quarter of the scores of one head; and out^T = V^T P^T, whose second operand is those scores' exponentials where they are.  Both operands of
 // the cache are read whole rows at a time, 4 to 16 lanes a row.  K turns into operands through the wavefront's own part of LDS (straight into them,
 // a row a lane, cost 64 cycles of a compute unit's address path a load: 2.1 us for 128 KB, and 0.9 now).  V needs no such turn: a lane has the channels 8 li .. + 7
 // (HD 128) of 8 keys, and channel 8 li + t of them is its operand for channel tile t, put together from the halves (or bytes) of those registers.
 //
 // Bound by memory: a byte of the cache takes part in 2 to 16 operations.  Measured against a large copy's 5.1 TB/s: 32 sequences of 2048 to 4096 keys, 8
-// key-value heads of 128 in bf16, 407 MB in 79 us; 4 of up to 65536 in int8 450 MB in 90 us; one of 65536 in bf16 268 MB in 55 us; one of 777 9.6 us, its chain of
+// key-value heads of 128 in bf16, 407 MB in 80 us; 4 of up to 65536 in int8 450 MB in 93 us; one of 65536 in bf16 268 MB in 55 us; one of 777 10 us, its chain of
 // trips to memory.  A sequence's tiles are shared out among `splits` workgroups of eight wavefronts, whose parts a second launch joins, where
 // (sequence, head) pairs alone would leave compute units idle.
 //
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
                     if (st % 2 == 0) x = mine[unit_at(16 * a + li, st * 2 + lg)];
                     const unsigned two[2] = {st % 2 ? x.z : x.x, st % 2 ? x.w : x.y};
                     unsigned y[4];
-                    s8_to_h16<DT, 2>(two, y);
+                    s8_to_h16<DT>(two, y);
                     acc = mfma.template operator()<DT>(make_uint4(y[0], y[1], y[2], y[3]), qf[st], acc);
                 }
             } else {
@@ -474,10 +474,10 @@ int attention_join_launch(int dt, int hd, const JoinParams &p, hipStream_t strea
     return ONHIP_OK;
 }
 
-// Workgroups that a sequence's head is cut into: one a compute unit (two were 6 to 50 % behind: 32 sequences of 4096 keys 79 and 85 us, 2 of 30000 with
-// one key-value head 14.6 and 21.8), 256 keys each at least.  Up to 1024 keys one, without a second launch (one sequence of 777 keys 9.6 us, in four
-// parts 9.3 and a launch more to queue).  int8, whose tiles are half the bytes in flight: two a compute unit where each still has 4096 keys
-// (4 of 65536 95 and 90 us; 32 of 4000 49 and 56).
+// Workgroups that a sequence's head is cut into: one a compute unit (two were 6 to 46 % behind: 32 sequences of 4096 keys 80 and 86 us, 2 of 30000 with
+// one key-value head 15.1 and 22.1), 256 keys each at least.  Up to 1024 keys one, without a second launch (one sequence of 300 keys 7.3 us, in two parts
+// 9.7; of 777 10.1 and in four 9.7, with a launch more to queue).  int8, whose tiles are half the bytes in flight: two a compute unit where each still has
+// 4096 keys (4 of 65536 99 and 93 us; 32 of 4000 50 and 58).
 static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d) {
     const long long group = d->q_heads / c->kv_heads, rows = (long long) d->batch * c->kv_heads * ((group + 15) / 16);
     long long longest = (long long) d->table_pages * c->page_tokens;

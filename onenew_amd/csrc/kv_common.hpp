@@ -23,10 +23,10 @@ enum { DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_REVERSE4 = 0x1B, DPP_MIRROR8 = 0x14
 template <int HOW> __device__ __forceinline__ unsigned lane_moved(unsigned x) { return (unsigned) __builtin_amdgcn_update_dpp(0, (int) x, HOW, 0xf, 0xf, true); }
 template <int HOW> __device__ __forceinline__ float lane_moved(float x) { return __uint_as_float(lane_moved<HOW>(__float_as_uint(x))); }
 
-// eight (NV = 2) or four (NV = 1) signed bytes as pairs of the 16-bit type: every int8 is a bf16 and an fp16
-template <int DT, int NV> __device__ __forceinline__ void s8_to_h16(const unsigned (&x)[NV], unsigned (&y)[2 * NV]) {
+// eight signed bytes as pairs of the 16-bit type: every int8 is a bf16 and an fp16
+template <int DT> __device__ __forceinline__ void s8_to_h16(const unsigned (&x)[2], unsigned (&y)[4]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    for (int i = 0; i < 2; ++i) {
         const int w = (int) x[i];
         y[2 * i] = pack_h16<DT>((float) (signed char) w, (float) (signed char) (w >> 8));
         y[2 * i + 1] = pack_h16<DT>((float) (signed char) (w >> 16), (float) (signed char) (w >> 24));

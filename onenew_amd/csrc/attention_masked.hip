@@ -365,7 +365,7 @@ __global__ __launch_bounds__(RG == 8 ? 512 : 256, HD == 64 ? 3 : 2) void attenti
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const bool far = top > m + p.far;   // each row by itself: its bits do not depend on the rows beside it
+        const bool far = top - m > p.far;   // (m + far would be rounded)  Each row by itself: its bits do not depend on the rows beside it
         if (__any(far)) {
             const float next = far ? top : m, fade = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.0f : next)) * unit);
             m = next;
@@ -376,16 +376,15 @@ __global__ __launch_bounds__(RG == 8 ? 512 : 256, HD == 64 ? 3 : 2) void attenti
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         float shift = m == -INFINITY ? 0.0f : __builtin_fmaf(-m, unit, SHIFT);
-        if constexpr (HOW != GENERAL)
-            if (__any(fabsf(shift) > 65536.0f)) {   // the fused product would count the rounding of m scale2: such rows' scores have m taken off first
-                const bool high = fabsf(shift) > 65536.0f;
-                const float from = high ? m : 0.0f;
+        if (__any(fabsf(shift) > 65536.0f)) {   // the sum would count the rounding of m: such rows' scores have m taken off first
+            const bool high = fabsf(shift) > 65536.0f;
+            const float from = high ? m : 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][r] -= from;
-                shift = high ? SHIFT : shift;
-            }
+                for (int r = 0; r < 16; ++r) s[n][r] -= from;
+            shift = high ? SHIFT : shift;
+        }
         constexpr int PRODUCTS = 2 * DTILES;   // of 32 keys
         auto v_ask = [&](int i) __attribute__((always_inline)) { return v_frag(buf, i / PRODUCTS + kh, i % PRODUCTS / DTILES, i % DTILES); };
 #pragma unroll

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
         for (int j = 1; j < NS; ++j) top = fmaxf(top, s[j]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const bool far = top > m + 8.0f;   // the reference point follows a head's maximum when that is 2^8 above it: most tiles leave the sums alone
+        const bool far = top - m > 8.0f;   // the reference point follows a head's maximum when that is 2^8 above it: most tiles leave the sums alone
         if (__any(far)) {
             const float next = far ? top : m, fade = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
             m = next;
@@ -289,11 +289,11 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[i][r] *= fade;
         }
-        const float shift = m == -INFINITY ? 0.0f : SHIFT - m;
+        const float from = m == -INFINITY ? 0.0f : m;
         float e[NS];
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-            e[j] = __builtin_amdgcn_exp2f(s[j] + shift);
+            e[j] = __builtin_amdgcn_exp2f(s[j] - from + SHIFT);   // SHIFT - m would be rounded
             l += e[j];
         }
         if constexpr (I8)

@@ -160,6 +160,21 @@ def test_scores_of_any_size(dtype, tokens, merged):
         assert bool(((got[0, even + 1].double().cpu() - ref).abs() <= bound).all())
 
 
+def test_scores_a_step_of_fp32_apart():
+    """the next number above a score may be farther away than a probability's room above the reference point"""
+    hip.init(0)
+    q, k, v = (torch.zeros((1, n, 192, 64), dtype=torch.float16) for n in (2, 1, 1))
+    v += torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).half()
+    q[..., 0], q[..., 1] = 2048.0, 8.0
+    k[:, :, 64:128, 1], k[:, :, 128:, 1] = 1.0, 3.0
+    for at in range(30016, 60000, 1504):
+        k[..., 0] = at
+        for slopes in (None, torch.zeros(2).cuda()):
+            got = hip.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=1.0, causal=slopes is not None, slopes=slopes)
+            torch.cuda.synchronize()
+            assert bool((got.abs().cpu() <= v.abs().max()).all()), at
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_many_parts(dtype):
     _run(dtype, 1, 1, 1, 1, 70000, 64)

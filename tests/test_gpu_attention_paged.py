@@ -114,6 +114,22 @@ def test_slopes_that_leave_one_key(dtype):
         assert torch.equal(got[b].double().cpu(), kv_oracle.rows(cache[1], None, table[b], m)[:, -1].repeat_interleave(3, dim=0))
 
 
+def test_scores_a_step_of_fp32_apart():
+    """the next number above a score may be farther away than a probability's room above the reference point"""
+    hip.init(0)
+    q, cache, table, n = _case([1000], 2, 1, 64, 16, torch.float16, False)
+    k, v = _dev(*cache[:2])
+    q.zero_()
+    q[..., 0], q[..., 1] = 2048.0, 8.0
+    for at in range(30016, 60000, 1504):
+        k.zero_()
+        k[..., 0] = at
+        k[..., 1] = torch.arange(k.shape[0], device="cuda")[:, None, None] % 7    # a page's rows alike
+        got = hip.attention_paged(q.cuda(), k, v, table.cuda(), n.cuda(), scale=1.0)
+        torch.cuda.synchronize()
+        assert bool((got.abs() <= v.abs().max() * (1 + 2.0 ** -10)).all()), at   # probabilities rounded to fp16 over a sum that is not
+
+
 def test_no_pages():
     hip.init(0)
     q, cache, _, _ = _case([5, 5], 4, 2, 64, 16, torch.float16, False)

@@ -531,15 +531,33 @@ __global__ __launch_bounds__(RG == 8 ? 512 : 256, HD == 64 ? 3 : 2) void attenti
     }
 }
 
-// Parts of the keys: where row blocks alone leave compute units without work, 256 keys a part at least (one token of 32 heads on 4096 keys 13.5 us, with
-// 512 keys a part 17).
-static int masked_splits(const onhip_masked_attention_desc_t *d, long long blocks) {
-    const long long all = blocks * d->batch * d->kv_heads;
-    if (all >= 256) return 1;
-    long long keys = d->k_tokens;
+// Rows of a workgroup (32 rg), and parts of the keys where row blocks alone leave compute units without work.
+//   256 rows, for which a tile is staged half as often, with head dimension 128: where workgroups, one a compute unit, fill seven eighths of two rounds or more and
+//     blocks are no more than a sixteenth larger than the rows (4096 causal tokens of 32 heads 162 -> 141 us, 4096 on 16384 keys 970 -> 873; 2560 tokens, 320
+//     workgroups in 512 places, 74 and 77, 16 x 260 of 32 heads on 32 46 and 59; 8192 of 16 heads of 64, whose registers give way, 182 and 214); and where as many
+//     parts as fill one round have 640 keys of the middle row each, two parts 1600 (the last 512 of 8000 tokens of 32 heads on 8 126 -> 79 us, of 16000 245 -> 137, 256 of
+//     6000 47 -> 41, 768 of 8000 162 -> 123; 1000 of 3000 62 and 66).
+//   64 rows where 128 give no more than one workgroup a compute unit (4096 causal tokens of 8 heads on one 91 -> 72 us, 2048 of 16 heads of 64 34.5 -> 27, 77 of 12
+//     7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us).  In parts of 256 keys at least where those do not give one
+//     a compute unit either (one token of 32 heads on 4096 keys 13.5 us, with 512 keys a part 17).
+static void masked_shape(const onhip_masked_attention_desc_t *d, int *rg, long long *blocks, int *splits) {
+    const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads), pairs = (long long) d->batch * d->kv_heads;
+    const long long wide = (total + 255) / 256, items = wide * pairs, rounds = (items + 255) / 256;
+    long long keys = d->k_tokens, parts = 1;
     if (d->window > 0 && d->window + 128LL < keys) keys = d->window + 128LL;
-    const long long want = (512 + all - 1) / all, most = (keys + 255) / 256, s = want < most ? want : most;
-    return s < 1 ? 1 : s > 256 ? 256 : (int) s;
+    const long long middle = d->causal ? (long long) d->q_offset + d->q_tokens / 2 : keys, seen = middle < 0 ? 0 : middle < keys ? middle : keys;   // by the middle row
+    if ((total + 127) / 128 * pairs > 256) {
+        *rg = d->head_dim == 128 && rounds > 1 && wide * 256 <= total + total / 16 && items * 8 >= rounds * 256 * 7 ? 8 : 4;
+    } else if (d->head_dim == 128 && items <= 128 && wide * 256 <= 2 * total && seen / (256 / items) >= (items <= 85 ? 640 : 1600)) {
+        *rg = 8;
+        parts = 256 / items;
+    } else {
+        *rg = 2;
+        const long long all = (total + 63) / 64 * pairs, most = (keys + 255) / 256;
+        if (all < 256) parts = (512 + all - 1) / all < most ? (512 + all - 1) / all : most;
+    }
+    *blocks = (total + 32 * *rg - 1) / (32 * *rg);
+    *splits = parts < 1 ? 1 : parts > 256 ? 256 : (int) parts;
 }
 
 static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg, int *blocks, int *splits) {
@@ -555,18 +573,10 @@ static int masked_check(const onhip_masked_attention_desc_t *d, int *dt, int *rg
     if (!cap_fits(d->scale, d->softcap)) return set_error(ONHIP_ERR_ARG, "masked attention: scale and cap must be below 10^30 and finite, the cap not negative, their quotient between 10^-30 and 10^30");
     const long long heads = (long long) d->batch * d->q_heads;
     if (heads >= (1LL << 31) || heads * d->q_tokens >= (1LL << 31)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
-    // 64 rows a workgroup where 128 give no more than one a compute unit (4096 causal tokens of 8 heads on one 91 -> 72 us, 2048 of 16 heads of 64 34.5 -> 27,
-    // 77 of 12 7.0 -> 6.0); above that they stage every tile twice as often (2048 of 32 heads 56 and 66 us).  256 rows, for which a tile is staged half as
-    // often, with head dimension 128 where workgroups, one a compute unit, fill seven eighths of their rounds and blocks are no more than a sixteenth larger than the
-    // rows (4096 causal tokens of 32 heads 162 -> 141 us, 4096 on 16384 keys 970 -> 873; 2560 causal tokens, 320 workgroups in 512 places, 74 and 77, 16 x 260 of 32 heads on 32 46 and 59; 8192 of 16 heads of
-    // 64, whose registers give way, 182 and 214)
-    const long long total = (long long) d->q_tokens * (d->q_heads / d->kv_heads), pairs = (long long) d->batch * d->kv_heads;
-    const long long most = (total + 255) / 256, rounds = (most * pairs + 255) / 256;
-    *rg = (total + 127) / 128 * pairs <= 256 ? 2 : d->head_dim == 128 && most * 256 <= total + total / 16 && most * pairs * 8 >= rounds * 256 * 7 && rounds > 1 ? 8 : 4;
-    const long long n = (total + 32 * *rg - 1) / (32 * *rg);
-    if (n * pairs >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
+    long long n;
+    masked_shape(d, rg, &n, splits);
+    if (n * d->batch * d->kv_heads >= (1LL << 22)) return set_error(ONHIP_ERR_ARG, "masked attention: too many rows");
     *blocks = (int) n;
-    *splits = masked_splits(d, n);
     return ONHIP_OK;
 }
 

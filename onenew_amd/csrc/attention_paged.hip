@@ -405,71 +405,77 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
         reinterpret_cast<unsigned *>(dst)[i / 2] = pack_h16<DT>(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// ---- the parts of a row joined: eight wavefronts a row, a lane HD / 64 channels ------------------------------------------------
-// Bound by its trips to memory: a wavefront asks for eight parts at a time, the first eight before it knows their weights.
-template <int DT, int HD>
+// ---- the parts of a row joined ----------------------------------------------------------------------------------
+// HD / 2 lanes of two channels take a part.  Few rows for their parts (SPREAD): all 8 or 16 groups of a workgroup on one row, joined through LDS, bound by its trips to memory: a
+// group asks for eight parts at a time, the first eight before it knows their weights.  Many rows: a group has its own, bound by memory.
+template <int DT, int HD, bool SPREAD>
 __global__ __launch_bounds__(512) void attention_join_kernel(const JoinParams p) {
-    constexpr int PER = HD / 64, NW = 8, AHEAD = 8;
-    __shared__ float s_acc[NW][HD], s_l[NW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long row = blockIdx.x;
+    constexpr int LANES = HD / 2, GROUPS = 512 / LANES, AHEAD = SPREAD ? 8 : 4, STEP = SPREAD ? GROUPS : 1;
+    __shared__ float2 s_acc[SPREAD ? GROUPS : 1][LANES];
+    __shared__ float s_l[GROUPS];
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const long long row = SPREAD ? (long long) blockIdx.x : (long long) blockIdx.x * GROUPS + group;
+    if (row >= p.rows) return;   // a whole group, and none that others wait for
     const float2 *ml = reinterpret_cast<const float2 *>(p.ml) + row * p.splits;
-    const float *o = p.o + row * p.splits * HD + lane * PER;
-    float part[AHEAD][PER];
-    float2 own[AHEAD];
+    const float2 *o = reinterpret_cast<const float2 *>(p.o + row * p.splits * HD) + lane;
+    const int first = SPREAD ? group : 0;
+    float2 part[AHEAD], own[AHEAD];
     auto ask = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int s = min(s0 + i * NW, p.splits - 1);
+            const int s = min(s0 + i * STEP, p.splits - 1);
             own[i] = ml[s];
-#pragma unroll
-            for (int c = 0; c < PER; ++c) part[i][c] = o[(long long) s * HD + c];
+            part[i] = o[(long long) s * LANES];
         }
     };
-    ask(wave);
+    ask(first);
     float mm = -INFINITY;
-    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[s].x);
+    for (int s = lane; s < p.splits; s += LANES) mm = fmaxf(mm, ml[s].x);
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
+    for (int x = 1; x < LANES; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, LANES));
     const float shift = mm == -INFINITY ? 0.0f : mm;
-    float acc[PER], l = 0.0f;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) acc[c] = 0.0f;
-    for (int s0 = wave; s0 < p.splits; s0 += AHEAD * NW) {
-        if (s0 != wave) ask(s0);
+    float2 acc = make_float2(0.0f, 0.0f);
+    float l = 0.0f;
+    for (int s0 = first; s0 < p.splits; s0 += AHEAD * STEP) {
+        if (s0 != first) ask(s0);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const bool there = s0 + i * NW < p.splits;
+            const bool there = s0 + i * STEP < p.splits;
             const float f = there ? __builtin_amdgcn_exp2f(own[i].x - shift) : 0.0f, ls = own[i].y;
             l += !there || (f == 0.0f && ls == ls) ? 0.0f : ls * f;   // a NaN stays
-#pragma unroll
-            for (int c = 0; c < PER; ++c) acc[c] = f == 0.0f ? acc[c] : __builtin_fmaf(part[i][c], f, acc[c]);   // a part without keys has written nothing
+            acc.x = f == 0.0f ? acc.x : __builtin_fmaf(part[i].x, f, acc.x);   // a part without keys has written nothing
+            acc.y = f == 0.0f ? acc.y : __builtin_fmaf(part[i].y, f, acc.y);
         }
     }
+    if constexpr (SPREAD) {
+        s_acc[group][lane] = acc;
+        if (lane == 0) s_l[group] = l;
+        __syncthreads();
+        if (group) return;
+        l = 0.0f;
+        acc = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int c = 0; c < PER; ++c) s_acc[wave][lane * PER + c] = acc[c];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    if (threadIdx.x >= HD / 2) return;
-    l = 0.0f;
-    float x = 0.0f, y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        l += s_l[w];
-        x += s_acc[w][2 * threadIdx.x];
-        y += s_acc[w][2 * threadIdx.x + 1];
+        for (int g = 0; g < GROUPS; ++g) {
+            l += s_l[g];
+            acc.x += s_acc[g][lane].x;
+            acc.y += s_acc[g][lane].y;
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long token = row % p.tokens, bh = row / p.tokens, h = bh % p.heads, b = bh / p.heads;
-    reinterpret_cast<unsigned *>(p.out + b * p.os[0] + h * p.os[1] + token * p.os[2])[threadIdx.x] = pack_h16<DT>(x * inv, y * inv);
+    reinterpret_cast<unsigned *>(p.out + b * p.os[0] + h * p.os[1] + token * p.os[2])[lane] = pack_h16<DT>(acc.x * inv, acc.y * inv);
+}
+
+// (1024 rows in 64 parts spread 47 us of a call, not 51; in 16 parts 34 and 32.5; 16384 in 4 113 and 63)
+template <int DT, int HD> static void join_launch(const JoinParams &p, hipStream_t stream) {
+    constexpr int GROUPS = 1024 / HD;
+    if (p.rows <= 16LL * p.splits) hipLaunchKernelGGL((attention_join_kernel<DT, HD, true>), dim3((unsigned) p.rows), dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((attention_join_kernel<DT, HD, false>), dim3((unsigned) ((p.rows + GROUPS - 1) / GROUPS)), dim3(512), 0, stream, p);
 }
 
 int attention_join_launch(int dt, int hd, const JoinParams &p, hipStream_t stream) {
-    const dim3 grid((unsigned) p.rows);
-    if (dt == DT_BF16 && hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 64>), grid, dim3(512), 0, stream, p);
-    else if (dt == DT_BF16) hipLaunchKernelGGL((attention_join_kernel<DT_BF16, 128>), grid, dim3(512), 0, stream, p);
-    else if (hd == 64) hipLaunchKernelGGL((attention_join_kernel<DT_F16, 64>), grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((attention_join_kernel<DT_F16, 128>), grid, dim3(512), 0, stream, p);
+    if (dt == DT_BF16) hd == 64 ? join_launch<DT_BF16, 64>(p, stream) : join_launch<DT_BF16, 128>(p, stream);
+    else hd == 64 ? join_launch<DT_F16, 64>(p, stream) : join_launch<DT_F16, 128>(p, stream);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }

@@ -87,6 +87,21 @@ def test_blocks_of_256_rows(dtype, i):
     _run(dtype, b, hq, hkv, tq, tk, 128, causal=i % 2 == 0, ranges=edge, q_offset=tk // 2)
 
 
+# the last tokens of a long prompt: 256 rows a workgroup, keys in parts that a group of lanes joins by itself
+CHUNKS = [(1, 32, 8, 500, 4000), (1, 16, 8, 256, 6000), (2, 8, 1, 130, 11000), (1, 32, 8, 700, 4300)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("i", range(len(CHUNKS)))
+def test_chunks_behind_many_keys(dtype, i):
+    b, hq, hkv, tq, tk = CHUNKS[i]
+    _run(dtype, b, hq, hkv, tq, tk, 128)
+    _run(dtype, b, hq, hkv, tq, tk, 128, bias=True, causal=i % 2 == 0)
+    _run(dtype, b, hq, hkv, tq, tk, 128, window=tk - 600, cap=20.0)
+    edge = torch.randint(-20, tk + 20, (b, tq, 2), generator=torch.Generator().manual_seed(i), dtype=torch.int32)
+    _run(dtype, b, hq, hkv, tq, tk, 128, causal=False, ranges=edge)
+
+
 def test_scores_above_half_of_the_cap():
     """capped by a polynomial below, by an exponential above"""
     for scale in (0.05, 0.3, 1.0, 5.0, -2.0):
@@ -223,7 +238,7 @@ def test_ranges(dtype, tq, tk, causal):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("tq,tk,b", [(100, 100, 1), (20, 2000, 1), (100, 150, 300), (125, 190, 460)])
+@pytest.mark.parametrize("tq,tk,b", [(100, 100, 1), (20, 2000, 1), (100, 150, 300), (125, 190, 460), (125, 5200, 32)])
 def test_unseen_values(dtype, hd, tq, tk, b):
     """what a row does not see leaves its bits alone, infinities and NaN of k and v included; what it sees does not"""
     hip.init(0)

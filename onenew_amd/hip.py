@@ -7,6 +7,7 @@ Tensor arguments are torch CUDA tensors (PyTorch is used for device memory and s
 raw integer device addresses; launches go to torch's current stream.
 """
 import ctypes as C
+import operator
 import os
 
 from . import abi
@@ -705,7 +706,8 @@ def attention(q, k, v, scale=1.0, out=None, merged_out=True):
 #
 # What a call has to check and to describe depends on types, devices, shapes and strides alone, and a step's calls repeat them: the checked
 # descriptions are kept by those (a call that finds its own takes 8 us of host time, with the checks 15 to 24).  Addresses are passed on each call.
-# The last key of an entry point is compared first: a step calls each with the same shapes layer after layer.
+# The last key of an entry point is compared first: a step calls each with the same shapes layer after layer.  A key holds plain numbers alone: a
+# tensor in it would be found again by its identity, whatever it holds by then.
 _plans = {}
 _last = {}
 
@@ -719,6 +721,24 @@ def _plan(what, key, make, *args):
         _plans[what, key] = plan
     _last[what] = (key, plan)
     return plan
+
+
+def _real(what, name, x):
+    """a number, or a tensor of one element as it is now, as a float"""
+    try:
+        if not isinstance(x, (str, bytes)):
+            return float(x)
+    except (TypeError, ValueError, RuntimeError):
+        pass
+    raise OnhipError(f"{what}: {name} is {x!r}, not a number")
+
+
+def _whole(what, name, x):
+    """a whole number, or a tensor of one as it is now, as an int"""
+    try:
+        return operator.index(x)
+    except (TypeError, ValueError, RuntimeError):
+        raise OnhipError(f"{what}: {name} is {x!r}, not a whole number") from None
 
 
 def _meta(t):
@@ -813,6 +833,8 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
     norm of q's and k's heads where there are weights [head_dim] (fp32), rotation by positions [tokens] (int32) times inv_freq [pairs] (fp32)
     where there are frequencies (else positions may be None), q to q_out (returned), k and v into the cache's rows slots [tokens] (int32; -1: none).  The cache is
     [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with fp32 scales [pages, kv_heads, page_tokens]"""
+    eps = eps if type(eps) is float else _real("cache_append", "eps", eps)
+    interleaved = bool(interleaved)
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
            _flat(positions), slots.dtype, slots.get_device(), slots.numel(), slots.is_contiguous(),
            k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
@@ -854,6 +876,7 @@ def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=N
     """rows 0 .. tokens - 1 of every sequence (pages table [sequences, pages], lengths [sequences], int32), zeros behind its length: k and v
     [sequences, kv_heads, tokens, head_dim] in the cache's 16-bit type, or `dtype` for an int8 cache"""
     import torch
+    tokens = tokens if type(tokens) is int else _whole("cache_read", "tokens", tokens)
     dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
     key = (_device(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
            table.dtype, table.get_device(), table.shape, table.stride(), lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(),
@@ -897,6 +920,9 @@ def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, so
     """attention of one new token a sequence, q [sequences, q_heads, head_dim], over the cache's rows table [sequences, pages] / lengths
     [sequences] (int32; the new token's row is the last): scores capped to softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the
     distance, the last `window` rows alone where it is above zero; returns [sequences, q_heads, head_dim]"""
+    scale = scale if type(scale) is float else _real("attention_paged", "scale", scale)
+    softcap = softcap if type(softcap) is float else _real("attention_paged", "softcap", softcap)
+    window = window if type(window) is int else _whole("attention_paged", "window", window)
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(),
            v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(), table.dtype, table.get_device(), table.shape, table.stride(),
            lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(), scale, window, softcap, _flat(slopes), _meta(k_scale), _meta(v_scale), _meta(out))
@@ -944,6 +970,11 @@ def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, sl
     softcap * tanh(s / softcap), minus slopes [q_heads] (fp32) times the distance.  Returns [batch, q_tokens, q_heads * head_dim] (heads merged) or,
     with merged_out=False, [batch, q_heads, q_tokens, head_dim]; `out` may be such a tensor (merged: with a pitch above q_heads * head_dim).  Rows
     that see nothing are zeros"""
+    scale = scale if type(scale) is float else _real("attention_masked", "scale", scale)
+    softcap = softcap if type(softcap) is float else _real("attention_masked", "softcap", softcap)
+    window = window if type(window) is int else _whole("attention_masked", "window", window)
+    q_offset = q_offset if q_offset is None or type(q_offset) is int else _whole("attention_masked", "q_offset", q_offset)
+    causal, merged_out = bool(causal), bool(merged_out)
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
            scale, causal, window, softcap, _flat(slopes), _meta(ranges), q_offset, _meta(out), merged_out)
     last = _last.get("masked")

@@ -746,8 +746,8 @@ def _meta(t):
 
 
 def _flat(t):
-    """_meta of a contiguous array, whose number of elements says as much as its shape"""
-    return t if t is None else (t.dtype, t.get_device(), t.numel(), t.is_contiguous())
+    """_meta of an array that has to be contiguous"""
+    return t if t is None else (t.dtype, t.get_device(), t.shape, t.is_contiguous())
 
 
 def _device():
@@ -836,7 +836,7 @@ def cache_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, q_w
     eps = eps if type(eps) is float else _real("cache_append", "eps", eps)
     interleaved = bool(interleaved)
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k.dtype, k.get_device(), k.shape, k.stride(), v.dtype, v.get_device(), v.shape, v.stride(),
-           _flat(positions), slots.dtype, slots.get_device(), slots.numel(), slots.is_contiguous(),
+           _flat(positions), slots.dtype, slots.get_device(), slots.shape, slots.is_contiguous(),
            k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
            _flat(inv_freq), _flat(q_weight), _flat(k_weight), eps, interleaved, _meta(k_scale), _meta(v_scale), _meta(q_out))
     last = _last.get("append")
@@ -879,7 +879,7 @@ def cache_read(k_cache, v_cache, table, lengths, tokens, k_scale=None, v_scale=N
     tokens = tokens if type(tokens) is int else _whole("cache_read", "tokens", tokens)
     dtype = dtype or (k_out.dtype if k_out is not None else k_cache.dtype)
     key = (_device(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(),
-           table.dtype, table.get_device(), table.shape, table.stride(), lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(),
+           table.dtype, table.get_device(), table.shape, table.stride(), lengths.dtype, lengths.get_device(), lengths.shape, lengths.is_contiguous(),
            tokens, _meta(k_scale), _meta(v_scale), dtype, _meta(k_out), _meta(v_out))
     last = _last.get("read")
     d, shape, step, pages, ks, vs, empty = last[1] if last is not None and last[0] == key else _plan(
@@ -925,7 +925,7 @@ def attention_paged(q, k_cache, v_cache, table, lengths, scale=1.0, window=0, so
     window = window if type(window) is int else _whole("attention_paged", "window", window)
     key = (_device(), q.dtype, q.get_device(), q.shape, q.stride(), k_cache.dtype, k_cache.get_device(), k_cache.shape, k_cache.stride(),
            v_cache.dtype, v_cache.get_device(), v_cache.shape, v_cache.stride(), table.dtype, table.get_device(), table.shape, table.stride(),
-           lengths.dtype, lengths.get_device(), lengths.numel(), lengths.is_contiguous(), scale, window, softcap, _flat(slopes), _meta(k_scale), _meta(v_scale), _meta(out))
+           lengths.dtype, lengths.get_device(), lengths.shape, lengths.is_contiguous(), scale, window, softcap, _flat(slopes), _meta(k_scale), _meta(v_scale), _meta(out))
     last = _last.get("paged")
     c, d, shape, nbytes, empty = last[1] if last is not None and last[0] == key else _plan(
         "paged", key, _paged_plan, q, k_cache, v_cache, table, lengths, scale, window, softcap, slopes, k_scale, v_scale, out)

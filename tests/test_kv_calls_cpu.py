@@ -107,3 +107,30 @@ def test_what_is_no_number(stub, call, field, bad):
             call(**{field: 2 if field in ("window", "q_offset") else 1.0})
         with pytest.raises(hip.OnhipError, match=field):
             call(**{field: bad})
+
+
+def _arrays():
+    """calls by one array's shape: the right one, and the same number of elements in another"""
+    q, cache = torch.zeros((3, 4, 64), dtype=torch.bfloat16), _cache()
+    x = torch.zeros((3, 8, 64), dtype=torch.bfloat16)
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    row = lambda **kw: hip.cache_append(x[:, :4], x[:, 4:6], x[:, 6:], **{**dict(positions=ints(3), slots=ints(3), k_cache=cache[0], v_cache=cache[1], inv_freq=torch.zeros(32)), **kw})  # noqa: E731
+    return {
+        "masked slopes": (lambda s: _masked(slopes=torch.zeros(s)), (4,), (2, 2)),
+        "paged slopes": (lambda s: _paged(slopes=torch.zeros(s)), (4,), (4, 1)),
+        "paged lengths": (lambda s: hip.attention_paged(q, *cache, ints(3, 2), ints(*s)), (3,), (3, 1)),
+        "read lengths": (lambda s: hip.cache_read(*cache, ints(3, 2), ints(*s), 5), (3,), (1, 3)),
+        "positions": (lambda s: row(positions=ints(*s)), (3,), (3, 1)),
+        "slots": (lambda s: row(slots=ints(*s)), (3,), (1, 3)),
+        "q_weight": (lambda s: row(q_weight=torch.zeros(s)), (64,), (8, 8)),
+        "k_weight": (lambda s: row(k_weight=torch.zeros(s)), (64,), (64, 1)),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(_arrays()))
+def test_a_shape_is_refused_whatever_was_called_before(stub, name):
+    call, right, wrong = _arrays()[name]
+    for _ in range(2):
+        with pytest.raises(hip.OnhipError, match="shape"):
+            call(wrong)
+        call(right)

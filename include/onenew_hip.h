@@ -372,7 +372,8 @@ int onhip_attention(const onhip_attention_desc_t *d, const void *q, const void *
  * (`compute`: ONHIP_COMPUTE_BF16 or _F16), the head dimension 64 or 128 and contiguous, everything 16-byte aligned, strides in elements and
  * multiples of 8.  Indices, lengths, tables and ranges are int32 arrays in device memory that the kernels check themselves: nothing outside
  * the cache is read or written whatever they hold.  A stride over a single element is not looked at.  The calls use no shared workspace: calls on different streams may overlap, as long as
- * they are not handed the same workspace, result or cache rows that one of them writes.
+ * they are not handed the same workspace, result or cache rows that one of them writes.  Rows that a call writes, of results or of the cache, may not share memory under their
+ * strides: each stride is at least the span of the extents with smaller ones.
  *
  * The cache: `pages` pages of `page_tokens` rows (a power of two up to 1024) for each of `kv_heads` heads; element (page, head, row, channel)
  * of k at page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + channel, v likewise.  quantised == 0: rows of the 16-bit type.

@@ -21,6 +21,7 @@
 // workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 us (their 67 MB take 13).  Tiles of 32 keys with
 // three workgroups a compute unit, eight operands ahead, a higher wave priority in the products, and 256 rows on four buffers with a barrier every second tile were level.
 #include "attention_join.hpp"
+#include "kv_common.hpp"
 
 namespace onhip {
 
@@ -630,8 +631,7 @@ int onhip_attention_masked(const onhip_masked_attention_desc_t *d, const void *q
             own[t][i] = strides[t][i];
         }
     }
-    for (int i = 0; i < 3; ++i)
-        if (q_extent[i] > 1 && d->out_strides[i] < d->head_dim) return set_error(ONHIP_ERR_ARG, "masked attention: rows of the result overlap");
+    if (!rows_apart(q_extent, d->out_strides, d->head_dim)) return set_error(ONHIP_ERR_ARG, "masked attention: rows of the result overlap");
     if (p.ks[2] >= (1LL << 23) || p.vs[2] >= (1LL << 23)) return set_error(ONHIP_ERR_ARG, "masked attention: token strides of k and v must be below 2^23");
     const long long rows = (long long) d->batch * d->q_heads * d->q_tokens;
     const size_t need = join_bytes(rows, p.splits, d->head_dim);

@@ -543,10 +543,11 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
         if ((i == 0 ? d->batch : d->q_heads) == 1) continue;
         if (d->q_strides[i] < 0 || d->q_strides[i] % 8 || d->out_strides[i] < 0 || d->out_strides[i] % 8)
             return set_error(ONHIP_ERR_ARG, "paged attention: strides must be non-negative multiples of 8");
-        if (d->out_strides[i] < c->head_dim) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
         p.qs[i] = d->q_strides[i];
         p.os[i] = d->out_strides[i];
     }
+    const int extent[2] = {d->batch, d->q_heads};
+    if (!rows_apart(extent, d->out_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
     const long long rows = (long long) d->batch * d->q_heads;
     p.splits = paged_splits(c, d);
     const size_t need = join_bytes(rows, p.splits, c->head_dim);

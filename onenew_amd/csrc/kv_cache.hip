@@ -361,8 +361,10 @@ int onhip_cache_append(const onhip_cache_desc_t *c, void *k_cache, void *v_cache
         }
     }
     if (q_out == q && (p.os[0] != p.qs[0] || p.os[1] != p.qs[1])) return set_error(ONHIP_ERR_ARG, "cache append: a result in q's place has q's strides");
-    if ((r->tokens > 1 && r->out_strides[0] < c->head_dim) || (r->q_heads > 1 && r->out_strides[1] < c->head_dim))
-        return set_error(ONHIP_ERR_ARG, "cache append: rows of the result overlap");
+    const int out_extent[2] = {r->tokens, r->q_heads}, extent[3] = {c->pages, c->kv_heads, c->page_tokens};
+    if (!rows_apart(out_extent, r->out_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache append: rows of the result overlap");
+    if (!rows_apart(extent, c->k_strides, c->head_dim) || !rows_apart(extent, c->v_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache append: rows of the cache overlap");
+    if (c->quantised && !rows_apart(extent, c->scale_strides, 1)) return set_error(ONHIP_ERR_ARG, "cache append: scales of the cache overlap");
     p.q = reinterpret_cast<const unsigned short *>(q);
     p.k = reinterpret_cast<const unsigned short *>(k);
     p.v = reinterpret_cast<const unsigned short *>(v);
@@ -412,6 +414,8 @@ int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const voi
                 return set_error(ONHIP_ERR_ARG, "cache read: strides of the results must be multiples of 8, at least the head dimension");
             p.os[t][i] = strides[t][i];
         }
+    for (int t = 0; t < 2; ++t)
+        if (!rows_apart(extent, strides[t], c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache read: rows of a result overlap");
     p.k_out = reinterpret_cast<unsigned short *>(k_out);
     p.v_out = reinterpret_cast<unsigned short *>(v_out);
     p.table = table;

@@ -18,6 +18,24 @@ int cache_shape(const char *what, const onhip_cache_desc_t *c, CacheView *view, 
 // checks the addresses and fills them in
 int cache_memory(const char *what, const onhip_cache_desc_t *c, const void *k, const void *v, const float *k_scale, const float *v_scale, CacheView *view);
 
+// Whether every row of `row` elements has memory of its own under these extents and strides (in elements, not negative; an extent of one has none):
+// each stride is at least the span of the extents with smaller ones.  Rows that share memory would be written by several wavefronts.
+template <int N> inline bool rows_apart(const int (&extent)[N], const long long *stride, long long row) {
+    int order[N];
+    for (int i = 0; i < N; ++i) {
+        int at = i;
+        for (; at > 0 && stride[order[at - 1]] > stride[i]; --at) order[at] = order[at - 1];
+        order[at] = i;
+    }
+    __int128 span = row;
+    for (int i : order) {
+        if (extent[i] <= 1) continue;
+        if (stride[i] < span) return false;
+        span += (__int128) stride[i] * (extent[i] - 1);
+    }
+    return true;
+}
+
 // lane i's value from lane i ^ 1, i ^ 2, 7 - i (of eight) or 15 - i (of sixteen), through the vector pipe
 enum { DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_REVERSE4 = 0x1B, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140, DPP_ROTATE8 = 0x128 };
 template <int HOW> __device__ __forceinline__ unsigned lane_moved(unsigned x) { return (unsigned) __builtin_amdgcn_update_dpp(0, (int) x, HOW, 0xf, 0xf, true); }

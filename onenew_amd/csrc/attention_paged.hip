@@ -548,6 +548,7 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
     }
     const int extent[2] = {d->batch, d->q_heads};
     if (!rows_apart(extent, d->out_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "paged attention: rows of the result overlap");
+    if (out == k_cache || out == v_cache) return set_error(ONHIP_ERR_ARG, "paged attention: one memory for the result and the cache");
     const long long rows = (long long) d->batch * d->q_heads;
     p.splits = paged_splits(c, d);
     const size_t need = join_bytes(rows, p.splits, c->head_dim);

@@ -365,6 +365,8 @@ int onhip_cache_append(const onhip_cache_desc_t *c, void *k_cache, void *v_cache
     if (!rows_apart(out_extent, r->out_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache append: rows of the result overlap");
     if (!rows_apart(extent, c->k_strides, c->head_dim) || !rows_apart(extent, c->v_strides, c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache append: rows of the cache overlap");
     if (c->quantised && !rows_apart(extent, c->scale_strides, 1)) return set_error(ONHIP_ERR_ARG, "cache append: scales of the cache overlap");
+    if (k_cache == v_cache || (c->quantised && k_scale == v_scale) || q_out == k_cache || q_out == v_cache)
+        return set_error(ONHIP_ERR_ARG, "cache append: one memory for keys and values, or for the result and the cache");
     p.q = reinterpret_cast<const unsigned short *>(q);
     p.k = reinterpret_cast<const unsigned short *>(k);
     p.v = reinterpret_cast<const unsigned short *>(v);
@@ -416,6 +418,7 @@ int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const voi
         }
     for (int t = 0; t < 2; ++t)
         if (!rows_apart(extent, strides[t], c->head_dim)) return set_error(ONHIP_ERR_ARG, "cache read: rows of a result overlap");
+    if (k_out == k_cache || k_out == v_cache || v_out == k_cache || v_out == v_cache) return set_error(ONHIP_ERR_ARG, "cache read: one memory for a result and the cache");
     p.k_out = reinterpret_cast<unsigned short *>(k_out);
     p.v_out = reinterpret_cast<unsigned short *>(v_out);
     p.table = table;

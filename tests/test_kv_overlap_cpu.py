@@ -58,3 +58,17 @@ def test_layouts_that_are_not_refused(strides):
     """any order of the extents, and gaps between them: the next check, of the workspace, is what refuses (2 sequences of 8 tokens, 4 heads; many keys)"""
     d = abi.MaskedAttentionDesc(2, 4, 2, 8, 5000, 64, (2048, 64, 256), (1 << 20, 64, 128), (1 << 20, 64, 128), strides, 1.0, 0.0, 1, 0, 0, abi.COMPUTE_F16)
     _refused(hip.load().onhip_attention_masked(C.byref(d), A, A, A, None, None, B, None, 0, None), "workspace", -3)
+
+
+def test_one_memory_for_two():
+    """keys and values in one place, and results in the cache's"""
+    _refused(_append(_cache(), _rows(), memory=(A, A, None, None)), "one memory")
+    _refused(_append(_cache(quantised=1), _rows(), memory=(A, 2 * A, 3 * A, 3 * A)), "one memory")
+    for memory in ((B, A, None, None), (A, B, None, None)):
+        _refused(_append(_cache(), _rows(), memory=memory), "one memory")
+    c, three = _cache(), (C.c_longlong * 3)(4096, 1024, 64)
+    d = abi.PagedAttentionDesc(1, 4, 4, 0, 4, (256, 64), (256, 64), 1.0, 0.0)
+    for memory in ((B, A), (A, B)):
+        for k, v in ((B, 2 * B), (2 * B, B)):
+            _refused(hip.load().onhip_cache_read(C.byref(c), *memory, None, None, A, 4, 4, A, 2, 5, k, three, v, three, None), "one memory")
+        _refused(hip.load().onhip_attention_paged(C.byref(c), *memory, None, None, C.byref(d), A, A, A, None, B, None, 0, None), "one memory")

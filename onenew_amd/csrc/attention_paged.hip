@@ -440,11 +440,11 @@ __global__ __launch_bounds__(512) void attention_join_kernel(const JoinParams p)
         if (s0 != first) ask(s0);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const bool there = s0 + i * STEP < p.splits;
-            const float f = there ? __builtin_amdgcn_exp2f(own[i].x - shift) : 0.0f, ls = own[i].y;
-            l += !there || (f == 0.0f && ls == ls) ? 0.0f : ls * f;   // a NaN stays
-            acc.x = f == 0.0f ? acc.x : __builtin_fmaf(part[i].x, f, acc.x);   // a part without keys has written nothing
-            acc.y = f == 0.0f ? acc.y : __builtin_fmaf(part[i].y, f, acc.y);
+            const bool there = s0 + i * STEP < p.splits, none = !there || own[i].x == -INFINITY;   // a part without keys has written no values
+            const float f = none ? 0.0f : __builtin_amdgcn_exp2f(own[i].x - shift), ls = own[i].y;
+            l += none ? (there && ls != ls ? ls : 0.0f) : ls * f;
+            acc.x = none ? acc.x : __builtin_fmaf(part[i].x, f, acc.x);   // a weight of 0 as well: what is no number stays
+            acc.y = none ? acc.y : __builtin_fmaf(part[i].y, f, acc.y);
         }
     }
     if constexpr (SPREAD) {

@@ -418,7 +418,7 @@ int onhip_cache_read(const onhip_cache_desc_t *c, const void *k_cache, const voi
  *   out = Softmax(s) v   over j in [0, lengths[b]), or with window > 0 the last `window` of them.
  * scale and softcap are below 10^30, and their quotient (of a scale that is not 0) is between 10^-30 and 10^30.
  * Query head h reads key-value head h / (q_heads / kv_heads).  Strides are (sequence, head).  A sequence of length 0 or less gives zeros; one
- * whose table names a page that does not exist, or is longer than its table, NaN.  out may not be q.  The keys of a sequence may be shared out among
+ * whose table names a page that does not exist for a row that it sees, or is longer than its table, NaN, and so does one whose every score is minus infinity.  out may not be q.  The keys of a sequence may be shared out among
  * workgroups whose parts go through `workspace` (16-byte aligned, onhip_attention_paged_workspace bytes; 0: none needed) and are joined in a
  * fixed order: the same call gives the same bits. */
 typedef struct onhip_paged_attention_desc {
@@ -439,7 +439,7 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
  *   window     P - j < window               (where window > 0)
  *   ranges     begin <= j < end, the pair ranges[(b * q_tokens + i) * 2] (where given: documents of a packed batch, prefixes, padded lengths)
  *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * |P - j| where slopes are given
- *   out = Softmax(s) v over the keys seen, zeros where none is (k_tokens 0 among them).  out may not be q, k or v; scale and softcap as above.
+ *   out = Softmax(s) v over the keys seen, zeros where none is (k_tokens 0 among them), NaN where each one's score is minus infinity.  out may not be q, k or v; scale and softcap as above.
  * Keys and values that a row does not see are kept out of it whatever they hold, infinities and NaN included.  Query head h reads key-value
  * head h / (q_heads / kv_heads).  Strides are (batch, head, token).  workspace as for onhip_attention_paged.  onhip_attention is the form for
  * at most 256 tokens without a mask, and for fp32. */

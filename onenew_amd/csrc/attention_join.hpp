@@ -1,7 +1,8 @@
 // What the attention kernels on long sequences share: the cap of scores, and the join of parts.
 //
 // Attention whose keys were shared out among workgroups: every part leaves its unnormalised result, its largest score m (in units of the
-// exponential base 2) and the sum l of its exponentials; the join is sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// exponential base 2) and the sum l of its exponentials; the join is sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A part without a score above
+// minus infinity leaves no result, and l = 0 where the row sees no key, 1 where it does: where no part has one, zeros and NaN.
 #pragma once
 
 #include "igemm_kernel.hpp"

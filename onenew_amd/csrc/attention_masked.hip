@@ -496,6 +496,7 @@ __global__ __launch_bounds__(RG == 8 ? 512 : 256, HD == 64 ? 3 : 2) void attenti
     }
 
     if (kh) return;
+    if (m == -INFINITY && l == 0.0f && lo < hi) l = p.splits > 1 ? 1.0f : NAN;   // the row sees keys, and every score is minus infinity: no number, unless another part has one
     if (p.splits > 1) {
         unsigned again = row0;   // the row's token and head anew, not kept through the loop
         asm volatile("" : "+s"(again));

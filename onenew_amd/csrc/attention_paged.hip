@@ -390,6 +390,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
         for (int i = 0; i < PER; ++i) acc[i] = __builtin_fmaf(s_o[w][oh][d0 + i], f, acc[i]);
         if (s_l[w][oh] != s_l[w][oh]) ll = NAN;   // a page that does not exist
     }
+    if (mm == -INFINITY && ll == 0.0f && t_begin < t_end) ll = p.splits > 1 ? 1.0f : NAN;   // keys, and every score minus infinity: no number, unless another part has one
     const int row = b * p.q_heads + kvh * p.group + hb * 16 + oh;
     if (p.splits > 1) {
         float *po = p.part_o + ((long long) row * p.splits + split) * HD + d0;
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(512) void attention_join_kernel(const JoinParams p)
         for (int i = 0; i < AHEAD; ++i) {
             const bool there = s0 + i * STEP < p.splits, none = !there || own[i].x == -INFINITY;   // a part without keys has written no values
             const float f = none ? 0.0f : __builtin_amdgcn_exp2f(own[i].x - shift), ls = own[i].y;
-            l += none ? (there && ls != ls ? ls : 0.0f) : ls * f;
+            l += !none ? ls * f : there && (mm == -INFINITY ? ls != 0.0f : ls != ls) ? NAN : 0.0f;   // (a sum without a score: one of the row's keys, all of them minus infinity)
             acc.x = none ? acc.x : __builtin_fmaf(part[i].x, f, acc.x);   // a weight of 0 as well: what is no number stays
             acc.y = none ? acc.y : __builtin_fmaf(part[i].y, f, acc.y);
         }

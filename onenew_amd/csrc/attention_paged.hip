@@ -14,8 +14,8 @@
 // (sequence, head) pairs alone would leave compute units idle.
 //
 // int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
-// probability.  Before the second product 2^(s - m) (times a constant, and the scale) is rounded to fp16 with fp16 and int8 values, half of one of its eleven bits; with
-// bf16's it goes in as two bf16 parts, sixteen bits: the cache's trip leaves the matrix cores time for both.  Scores, maximum, sum and
+// probability.  Before the second product 2^(s - m) (times a constant, and the scale) is rounded to fp16 with fp16 and int8 values, half of one of its eleven bits (fp16 values:
+// what is summed is the rounded one); with bf16's it goes in as two bf16 parts, sixteen bits: the cache's trip leaves the matrix cores time for both.  Scores, maximum, sum and
 // products' sums are fp32.
 #include "attention_join.hpp"
 #include "kv_common.hpp"
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             e[j] = __builtin_amdgcn_exp2f(s[j] - from + SHIFT);   // SHIFT - m would be rounded
-            l += e[j];
+            if constexpr (I8 || DT == DT_BF16) l += e[j];
         }
         if constexpr (I8)
 #pragma unroll
@@ -311,6 +311,8 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             } else {
                 hi[i] = pack_h16<PT>(e[2 * i], e[2 * i + 1]);
                 lo[i] = 0u;
+                // the sum is of the rounded ones: the weights of equal values sum to one
+                if constexpr (!I8) l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi[i]), f16x2{(_Float16) 1.0f, (_Float16) 1.0f}, l, false);
             }
         }
 #pragma unroll

@@ -14,9 +14,10 @@
 // (sequence, head) pairs alone would leave compute units idle.
 //
 // int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
-// probability.  Before the second product 2^(s - m) (times a constant, and the scale) is rounded to fp16 with fp16 and int8 values, half of one of its eleven bits (fp16 values:
-// what is summed is the rounded one); with bf16's it goes in as two bf16 parts, sixteen bits: the cache's trip leaves the matrix cores time for both.  Scores, maximum, sum and
-// products' sums are fp32.
+// probability.  Before the second product 2^(s - m) (times a constant) is rounded to fp16 with fp16 values, half of one of its eleven bits, and what is summed is the
+// rounded one; with bf16 values, and with int8's times the scale, it goes in as two bf16 parts, sixteen bits: the cache's trip leaves the matrix cores time for both.
+// (int8 in fp16, which has not the range for scales, needs a unit for them: in units of the largest one so far, one of 10^9 times the others took their
+// bits although its key had no weight.)  Scores, maximum, sum and products' sums are fp32.
 #include "attention_join.hpp"
 #include "kv_common.hpp"
 
@@ -48,7 +49,8 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
     constexpr int VB = (I8 ? 1 : 2) * HD / 16;        // bytes of a lane's part of a value: 4, 8 or 16
     constexpr int VW = VB / 4;
     // probabilities are 2^(s - m + SHIFT): fp16's stay clear of its smallest numbers, a sum of bf16's largest values of fp32's largest
-    constexpr int PT = I8 ? DT_F16 : DT;   // type of the second product
+    // (values below 2^-94, which are 2^-118 there, lose bits)
+    constexpr int PT = I8 ? DT_BF16 : DT;   // type of the second product: a probability times a value's scale needs fp32's range
     constexpr float SHIFT = PT == DT_BF16 ? -24.0f : 7.0f;
     // a wavefront's tile of keys on its way into operands, in the end the wavefronts' results
     constexpr int KEY_BYTES = NW * KT * UNITS * 16, OUT_BYTES = NW * 16 * (HD + 4) * 4;
@@ -98,7 +100,6 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
     for (int t = 0; t < TILES; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    int unit = -1000;   // int8: o is in units of 2^unit
     bool bad = false;
     const int *table = p.table + b * p.table_stride;
     const char *kb = p.c.k + kvh * p.c.ks[1], *vb = p.c.v + kvh * p.c.vs[1];
@@ -202,23 +203,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             const int key = key0 + (lane & (KT - 1));
             const bool seen = key >= begin && key < len;
             const float x = seen ? tile.k_scale : 0.0f;
-            float y = seen ? tile.v_scale : 0.0f;
-            // fp16's range is short: the probabilities below are times a scale in units of the largest one so far
-            unsigned most = __float_as_uint(y) & 0x7fffffffu;   // as whole numbers, an infinity is above every number and a NaN above that
-            most = max(most, lane_moved<DPP_XOR1>(most));
-            most = max(most, lane_moved<DPP_XOR2>(most));
-            most = max(most, lane_moved<DPP_MIRROR8>(most));
-            most = max(most, lane_moved<DPP_MIRROR16>(most));
-            most = max((unsigned) __builtin_amdgcn_readlane((int) most, 0), (unsigned) __builtin_amdgcn_readlane((int) most, 16));
-            const int e = most != 0u && most < 0x7f800000u ? (int) (most >> 23) - 126 : -1000;
-            if (e > unit) {   // uniform
-#pragma unroll
-                for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit - e);
-                unit = e;
-            }
-            y = ldexpf(y, -unit);
+            const float y = seen ? tile.v_scale : 0.0f;
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 const int from_lane = 16 * (j / 4) + 4 * lg + j % 4;
@@ -294,7 +279,7 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             e[j] = __builtin_amdgcn_exp2f(s[j] - from + SHIFT);   // SHIFT - m would be rounded
-            if constexpr (I8 || DT == DT_BF16) l += e[j];
+            if constexpr (PT == DT_BF16) l += e[j];
         }
         if constexpr (I8)
 #pragma unroll
@@ -304,15 +289,16 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (PT == DT_BF16) {
-                // a bf16 below the probability, and the rest in a product of its own: of one sign both, so that an infinity stays one
-                const unsigned x = __float_as_uint(e[2 * i]), y = __float_as_uint(e[2 * i + 1]), x1 = x - (x != 0u), y1 = y - (y != 0u);
+                // a bf16 below the probability (or its size times a scale's), and the rest in a product of its own: of one sign both, so that an infinity stays one
+                constexpr unsigned SIZE = I8 ? 0x7fffffffu : 0xffffffffu;   // a scale may have a sign
+                const unsigned x = __float_as_uint(e[2 * i]), y = __float_as_uint(e[2 * i + 1]), x1 = x - ((x & SIZE) != 0u), y1 = y - ((y & SIZE) != 0u);
                 hi[i] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
                 lo[i] = pack_h16<PT>(e[2 * i] - __uint_as_float(x1 & 0xffff0000u), e[2 * i + 1] - __uint_as_float(y1 & 0xffff0000u));
             } else {
                 hi[i] = pack_h16<PT>(e[2 * i], e[2 * i + 1]);
                 lo[i] = 0u;
                 // the sum is of the rounded ones: the weights of equal values sum to one
-                if constexpr (!I8) l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi[i]), f16x2{(_Float16) 1.0f, (_Float16) 1.0f}, l, false);
+                l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi[i]), f16x2{(_Float16) 1.0f, (_Float16) 1.0f}, l, false);
             }
         }
 #pragma unroll
@@ -354,11 +340,6 @@ __global__ __launch_bounds__(512, 2) void attention_paged_kernel(const PagedPara
             if (t >= t_end) break;
         }
     }
-    if constexpr (I8)
-#pragma unroll
-        for (int i = 0; i < TILES; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[i][r] = ldexpf(o[i][r], unit);
     // the eight wavefronts' parts
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);

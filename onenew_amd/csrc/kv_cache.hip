@@ -217,11 +217,16 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= up;
             }
-            const float inv = top > 0.0f && fine ? 127.0f * __builtin_amdgcn_rcpf(top * up) : 0.0f;   // a unit and a half unit off: a value 1 / 60000 of a step
+            // x 127 / max by the reciprocal, which is a unit off, and one step of the division's remainder: a quotient that fp32 holds comes out as it is, so that one in the
+            // middle of two whole numbers goes to the even one (by the reciprocal alone half of the largest value of some rows was 63 and not 64)
+            const float size = top * up, inv = top > 0.0f && fine ? __builtin_amdgcn_rcpf(size) : 0.0f;
             // to the nearest whole number by adding 1.5 2^23, whose sum has it in its lowest byte
             unsigned b[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(x[j] * inv + 12582912.0f);
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[j] * 127.0f, z = y * inv;
+                b[j] = __float_as_uint(__builtin_fmaf(__builtin_fmaf(-z, size, y), inv, z) + 12582912.0f);
+            }
             unsigned q8[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j)

@@ -379,7 +379,7 @@ int onhip_attention(const onhip_attention_desc_t *d, const void *q, const void *
  * of k at page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + channel, v likewise.  quantised == 0: rows of the 16-bit type.
  * quantised == 1: int8 rows (strides multiples of 16) and one fp32 scale a row at page * scale_strides[0] + head * scale_strides[1] +
  * row * scale_strides[2] of k_scale / v_scale (else ignored); a value is int8 * scale. */
-typedef struct onhip_cache_desc {
+typedef struct onhip_cache_desc {   /* page_tokens times a row stride, of scales too, is below 2^30 */
     int32_t pages, page_tokens, kv_heads, head_dim;
     int32_t compute, quantised;
     long long k_strides[3], v_strides[3], scale_strides[3];
@@ -441,7 +441,7 @@ int onhip_attention_paged(const onhip_cache_desc_t *c, const void *k_cache, cons
  *   s_j = scale * q.k_j, capped to softcap * tanh(s_j / softcap) where softcap > 0, minus slopes[head] * |P - j| where slopes are given
  *   out = Softmax(s) v over the keys seen, zeros where none is (k_tokens 0 among them), NaN where each one's score is minus infinity.  out may not be q, k or v; scale and softcap as above.
  * Keys and values that a row does not see are kept out of it whatever they hold, infinities and NaN included.  Query head h reads key-value
- * head h / (q_heads / kv_heads).  Strides are (batch, head, token).  workspace as for onhip_attention_paged.  onhip_attention is the form for
+ * head h / (q_heads / kv_heads).  Strides are (batch, head, token), those of k's and v's tokens below 2^23.  workspace as for onhip_attention_paged.  onhip_attention is the form for
  * at most 256 tokens without a mask, and for fp32. */
 typedef struct onhip_masked_attention_desc {
     int32_t batch, q_heads, kv_heads, q_tokens, k_tokens, head_dim;

@@ -17,8 +17,8 @@
 // What bounds it: per tile of 64 keys the matrix instructions take 1024 cycles of a SIMD, the softmax's vector instructions as many (half of the exponentials run
 // between the second product's matrix instructions), LDS 1300 for operands and staging; two wavefronts a SIMD overlap them to half of the
 // time, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 500 to 535 us, 1.02 to 1.10 PFLOP/s where a large library
-// product reaches 1.2 (540 to 565 with a tile staged for 128 rows, not 256).  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 99 us.  Short rows are bound by a
-// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 us (their 67 MB take 13).  Tiles of 32 keys with
+// product reaches 1.2 (540 to 565 with a tile staged for 128 rows, not 256).  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 98 to 102 us.  Short rows are bound by a
+// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 to 46 us (their 67 MB take 13).  Tiles of 32 keys with
 // three workgroups a compute unit, eight operands ahead, a higher wave priority in the products, and 256 rows on four buffers with a barrier every second tile were level.
 #include "attention_join.hpp"
 #include "kv_common.hpp"
@@ -61,7 +61,7 @@ template <int DT> __device__ __forceinline__ unsigned finite_of(unsigned w) {
 // HOW the scores become exponents.  PLAIN: one fused product takes them there.  BIASED: as that, where every key that counts lies behind its query, so that the
 // bias is slope / scale times (the key's number - the row's place): one more matrix instruction, of the number in the tile of 64 (a whole number) and of one
 // with the quotient and the rest in three bf16 parts each, all of their 24 bits (documents of 16 heads 40 us, as GENERAL 43).  GENERAL: capped, a
-// bias on keys on both sides, or a scale of (nearly) zero.
+// bias on keys on both sides, or a scale of (nearly) zero; with 64 channels and 128 rows three of its registers are spilled.
 enum { PLAIN, BIASED, GENERAL };
 // RG: groups of 32 rows of a workgroup.  4 and 8: a wavefront has all keys of a tile for its rows.  2: two wavefronts share the rows, one has the first 32 keys of
 // every tile, one the others, and their results are joined in the end.

@@ -9,8 +9,8 @@
 // (HD 128) of 8 keys, and channel 8 li + t of them is its operand for channel tile t, put together from the halves (or bytes) of those registers.
 //
 // Bound by memory: a byte of the cache takes part in 2 to 16 operations.  Measured against a large copy's 5.1 TB/s: 32 sequences of 2048 to 4096 keys, 8
-// key-value heads of 128 in bf16, 407 MB in 80 us; 4 of up to 65536 in int8 450 MB in 93 us; one of 65536 in bf16 268 MB in 55 us; one of 777 10 us, its chain of
-// trips to memory.  A sequence's tiles are shared out among `splits` workgroups of eight wavefronts, whose parts a second launch joins, where
+// key-value heads of 128 in bf16, 407 MB in 76 to 80 us; 4 of up to 65536 in int8 450 MB in 91 to 94 us; one of 65536 in bf16 268 MB in 55 us; one of 777 10 us, its chain of
+// trips to memory.  Workgroups a compute unit: two with head dimension 64 and int8 (128 registers), one else (16-bit rows of 64 channels 132 registers, four past two).  A sequence's tiles are shared out among `splits` workgroups of eight wavefronts, whose parts a second launch joins, where
 // (sequence, head) pairs alone would leave compute units idle.
 //
 // int8: an int8 is a bf16 and an fp16, so the products are exact in it; the scale of a key multiplies its score, the scale of a value its
@@ -464,8 +464,10 @@ int attention_join_launch(int dt, int hd, const JoinParams &p, hipStream_t strea
     return ONHIP_OK;
 }
 
-// Workgroups that a sequence's head is cut into: one a compute unit (two were 6 to 46 % behind: 32 sequences of 4096 keys 80 and 86 us, 2 of 30000 with
-// one key-value head 15.1 and 22.1), 256 keys each at least.  Up to 1024 keys one, without a second launch (one sequence of 300 keys 7.3 us, in two parts
+// Workgroups that a sequence's head is cut into: as many that all of them are one a compute unit (two were 6 to 46 % behind: 32 sequences of 4096 keys 80 and 86 us, 2
+// of 30000 with one key-value head 15.1 and 22.1), rounded up, and no more than the 256s of keys, rounded up as well (1025 keys: five parts of 205).  Where the heads do not divide
+// 256, the rest is a second round of a few workgroups: of 4096 keys and eight heads 8 sequences take 25 us, 9 (288 workgroups) 33, 12 (288) 43, 17 (272) 56, 24 (384) 67, 32 78 and 33
+// (264) 93.  Up to 1024 keys one, without a second launch (one sequence of 300 keys 7.3 us, in two parts
 // 9.7; of 777 10.1 and in four 9.7, with a launch more to queue).  int8, whose tiles are half the bytes in flight: two a compute unit where each still has
 // 4096 keys (4 of 65536 99 and 93 us; 32 of 4000 50 and 58).
 static int paged_splits(const onhip_cache_desc_t *c, const onhip_paged_attention_desc_t *d) {

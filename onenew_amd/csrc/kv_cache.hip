@@ -12,7 +12,7 @@
 // 49.9 us of the int8 case below).
 //
 // Bound by memory, and by the vector pipe next to it: 8191 tokens of 32 + 8 + 8 heads of 128 in bf16 201 MB in 41 us with norms and a full rotation, 38 without
-// norms (a large copy of as many bytes 40); into an int8 cache 184 MB in 44; a step of 32 tokens 3.3 us, a launch.  Read back: 8 sequences of up to 8192, 8 heads of 128,
+// norms (a large copy of as many bytes 40); into an int8 cache 184 MB in 44 (37 of them repeated over one input, part of which the last-level cache holds); a step of 32 tokens 3.3 us, a launch.  Read back: 8 sequences of up to 8192, 8 heads of 128,
 // 377 MB of int8 and its values in 75 us, 480 MB of bf16 in 93.
 #include "kv_common.hpp"
 

@@ -728,7 +728,7 @@ def _real(what, name, x):
     try:
         if not isinstance(x, (str, bytes)):
             return float(x)
-    except (TypeError, ValueError, RuntimeError):
+    except (TypeError, ValueError, RuntimeError, OverflowError):
         pass
     raise OnhipError(f"{what}: {name} is {x!r}, not a number")
 
@@ -790,6 +790,13 @@ def _dims(what, n, **tensors):
             raise OnhipError(f"{what}: {name} has {t.dim()} dimensions, not {n}")
 
 
+def _int32(what, **sizes):
+    """what goes into 32 bits of a description, where ctypes would cut it"""
+    for name, x in sizes.items():
+        if not -(1 << 31) <= x < 1 << 31:
+            raise OnhipError(f"{what}: {name} is {x}, past 2^31")
+
+
 def _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype):
     """k_cache, v_cache [pages, kv_heads, page_tokens, head_dim], 16-bit or int8 with scales [pages, kv_heads, page_tokens]"""
     import torch
@@ -798,6 +805,7 @@ def _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype):
     _dims(what, 4, k_cache=k_cache)
     _need(what, torch.int8 if quantised else dtype, k_cache.shape, last=True, k_cache=k_cache, v_cache=v_cache)
     pages, heads, rows, hd = k_cache.shape
+    _int32(what, pages=pages, heads=heads, page_tokens=rows, head_dim=hd)
     d = abi.CacheDesc(pages, rows, heads, hd, compute, int(quantised), k_cache.stride()[:3], v_cache.stride()[:3])
     if (k_scale is None) != (not quantised) or (v_scale is None) != (not quantised):
         raise OnhipError(f"{what}: scales go with an int8 cache, and an int8 cache with scales")
@@ -815,6 +823,7 @@ def _append_plan(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_weight
     d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, q.dtype)
     _dims(what, 3, q=q)
     tokens, q_heads, hd = q.shape
+    _int32(what, tokens=tokens, q_heads=q_heads, pairs=0 if inv_freq is None else inv_freq.numel())
     if hd != d.head_dim:
         raise OnhipError(f"{what}: heads of {hd} channels for a cache of {d.head_dim}")
     _need(what, q.dtype, q.shape, last=True, q=q, q_out=q_out)
@@ -865,6 +874,7 @@ def _read_plan(k_cache, v_cache, table, lengths, tokens, k_scale, v_scale, dtype
     what = "cache_read"
     d = _cache_desc(what, k_cache, v_cache, k_scale, v_scale, dtype)
     _table(what, table, lengths)
+    _int32(what, tokens=tokens, sequences=table.shape[0], table_pages=table.shape[1])
     shape = (table.shape[0], d.kv_heads, tokens, d.head_dim)
     _need(what, dtype, shape, last=True, k_out=k_out, v_out=v_out)
     flat = (d.kv_heads * tokens * d.head_dim, tokens * d.head_dim, d.head_dim)
@@ -908,6 +918,7 @@ def _paged_plan(q, k_cache, v_cache, table, lengths, scale, window, softcap, slo
     _table(what, table, lengths)
     _dims(what, 3, q=q)
     batch, q_heads, hd = q.shape
+    _int32(what, batch=batch, q_heads=q_heads, table_pages=table.shape[1], window=window)
     _need(what, q.dtype, (table.shape[0], q_heads, c.head_dim), last=True, q=q)
     _need(what, q.dtype, q.shape, last=True, out=out)
     _need(what, torch.float32, (q_heads,), flat=True, slopes=slopes)
@@ -947,6 +958,8 @@ def _masked_plan(q, k, v, scale, causal, window, softcap, slopes, ranges, q_offs
     _dims(what, 4, q=q, k=k)
     b, hq, tq, hd = q.shape
     hkv, tk = k.shape[1], k.shape[2]
+    q_offset = tk - tq if q_offset is None else q_offset
+    _int32(what, batch=b, q_heads=hq, kv_heads=hkv, q_tokens=tq, k_tokens=tk, head_dim=hd, window=window, q_offset=q_offset)
     _need(what, q.dtype, last=True, q=q, out=out)
     _need(what, q.dtype, (b, hkv, tk, hd), last=True, k=k, v=v)
     _need(what, torch.float32, (hq,), flat=True, slopes=slopes)
@@ -959,7 +972,7 @@ def _masked_plan(q, k, v, scale, causal, window, softcap, slopes, ranges, q_offs
             raise OnhipError(f"{what}: a result of the shape {tuple(out.shape)}, not {shape}")
         o_strides = (out.stride(0), hd, out.stride(1)) if merged_out else out.stride()[:3]
     d = abi.MaskedAttentionDesc(b, hq, hkv, tq, tk, hd, q.stride()[:3], k.stride()[:3], v.stride()[:3], o_strides, scale, softcap, int(causal), window,
-                                tk - tq if q_offset is None else q_offset, compute)
+                                q_offset, compute)
     return C.byref(d), shape, load().onhip_attention_masked_workspace(C.byref(d)), b == 0 or tq == 0
 
 

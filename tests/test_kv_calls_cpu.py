@@ -134,3 +134,35 @@ def test_a_shape_is_refused_whatever_was_called_before(stub, name):
         with pytest.raises(hip.OnhipError, match="shape"):
             call(wrong)
         call(right)
+
+
+BIG = 1 << 32
+
+
+@pytest.mark.parametrize("call,field", [(_masked, "window"), (_masked, "q_offset"), (_paged, "window")])
+@pytest.mark.parametrize("value", [BIG + 5, -BIG + 3, 1 << 31, -(1 << 31) - 1, 10 ** 30])
+def test_numbers_past_32_bits(stub, call, field, value):
+    """are refused, not cut to their lower half"""
+    for _ in range(2):
+        with pytest.raises(hip.OnhipError, match=field):
+            call(**{field: value})
+    assert not stub.got
+
+
+def test_extents_past_32_bits(stub):
+    """views may have them"""
+    one = torch.zeros((1, 1, 1, 64), dtype=torch.bfloat16)
+    long = one.expand(1, 1, BIG + 1, 64)
+    for args in ((one, long, long), (long, one, one), (one.expand(BIG + 1, 1, 1, 64),) * 3, (one.expand(1, BIG + 1, 1, 64), one, one)):
+        with pytest.raises(hip.OnhipError, match="2\\^31"):
+            hip.attention_masked(*args, out=torch.zeros((1, 1, 64), dtype=torch.bfloat16))
+    table, n = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    many = one.expand(BIG + 1, 1, 1, 64)
+    with pytest.raises(hip.OnhipError, match="contiguous rows"):
+        hip.attention_paged(one[0], one, one, table.expand(1, BIG + 1), n)
+    for call in (lambda: hip.attention_paged(one[0], many, many, table, n),
+                 lambda: hip.cache_read(many, many, table, n, 1), lambda: hip.cache_read(one, one, table, n, BIG + 1, k_out=one, v_out=one),
+                 lambda: hip.cache_append(one[0], one[0], one[0], None, n, many, many), lambda: hip.cache_append(one[0].expand(1, BIG + 1, 64), one[0], one[0], None, n, one, one.clone())):
+        with pytest.raises(hip.OnhipError, match="2\\^31"):
+            call()
+    assert not stub.got

@@ -18,7 +18,7 @@
 // between the second product's matrix instructions), LDS 1300 for operands and staging; two wavefronts a SIMD overlap them to half of the
 // time, at a clock that falls under them (1.74 GHz): 8192 causal tokens of 32 heads of 128 on 8 in bf16 500 to 535 us, 1.02 to 1.10 PFLOP/s where a large library
 // product reaches 1.2 (540 to 565 with a tile staged for 128 rows, not 256).  Capped scores add a third to the vector work: 2 x 4001 tokens of 16 heads on 8 in a window of 1024, fp16, 98 to 102 us.  Short rows are bound by a
-// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 40 to 46 us (their 67 MB take 13).  Tiles of 32 keys with
+// workgroup's chain of tiles: 2 x 4096 tokens of 16 heads of 64 in documents of about 450, with a bias, 38 to 47 us (their 67 MB take 13).  Tiles of 32 keys with
 // three workgroups a compute unit, eight operands ahead, a higher wave priority in the products, and 256 rows on four buffers with a barrier every second tile were level.
 #include "attention_join.hpp"
 #include "kv_common.hpp"

@@ -478,6 +478,57 @@ int onhip_add_f32(const onhip_add_desc_t *d, const float *large, const float *sm
  * including its two rules: the first n - n % 32 elements keep a NaN or a negative zero. */
 int onhip_relu_f32(const float *x, float *y, long long n, void *stream);
 
+/* ---- the linear layers of a generating transformer in 8-bit floating point ---------------------------------------------------------
+ *
+ * e4m3 rows (one sign, four exponent and three fraction bits, largest value 448, a NaN, no infinity): a byte a channel, the rows
+ * 16-byte aligned and a multiple of 16 bytes apart, and an fp32 scale for every 128 channels of a row (the last of them may have fewer) or, for weights
+ * [output][channel], for every 128 channels of 128 outputs: value = byte * scale.  What lies behind a row's last channel is neither read into a
+ * result nor written.  Scales have strides (row or 128 outputs, block of channels) in floats.
+ *   scale = max(max|y| / 448, 2^-126),  byte = e4m3(y / scale), the quotient rounded to fp32, then to the nearest e4m3, ties to even
+ * The maximum passes over NaN, which stays NaN in its place; an infinity makes its block's scale infinite and its values NaN.
+ *
+ * Element types are ONHIP_COMPUTE_F32 / _BF16 / _F16.  Strides count elements; a stride over a single row or block is not looked at.  Tensors are aligned to their
+ * elements (fast where 16-byte aligned, rows a multiple of 16 bytes apart).  The calls use no shared workspace: calls on different streams may
+ * overlap, as long as they are not handed the same results or workspace.  Results lie apart from each other and from the operands, but for what is said below. */
+
+/* h = x + residual (NULL: none) in fp32; sum (NULL: not wanted) = h rounded to x's type; y = h / sqrt(mean(h^2) + eps) * weight (fp32; NULL: none);
+ * out = y in x's type, or (f8 != 0) as e4m3 rows with out_scale.  A sum or result in x's type may take the place of x or residual, with its stride. */
+typedef struct onhip_norm_desc {
+    int32_t rows, channels;
+    int32_t compute;             /* type of x, residual and sum, and of a result that is not e4m3 */
+    int32_t f8;
+    long long x_stride, residual_stride, sum_stride, out_stride;   /* out_stride: bytes for e4m3 */
+    long long scale_strides[2];
+    float eps;
+} onhip_norm_desc_t;
+int onhip_rms_norm(const onhip_norm_desc_t *d, const void *x, const void *residual, const float *weight, void *out, float *out_scale,
+                   void *sum, void *stream);
+
+/* rows to e4m3: y = x (ONHIP_F8_ROWS); y[c] = silu(x[c]) * x[channels + c], rows of 2 * channels elements (ONHIP_F8_GATED: what lies between the products of a gated
+ * feed-forward layer); y = x with a scale for 128 x 128 (ONHIP_F8_WEIGHTS: rows are outputs).  silu(g) = g / (1 + e^-g). */
+#define ONHIP_F8_ROWS 0
+#define ONHIP_F8_GATED 1
+#define ONHIP_F8_WEIGHTS 2
+typedef struct onhip_f8_rows_desc {
+    int32_t rows, channels;      /* of the result */
+    int32_t compute, form;
+    long long x_stride, q_stride;
+    long long scale_strides[2];
+} onhip_f8_rows_desc_t;
+int onhip_f8_from_rows(const onhip_f8_rows_desc_t *d, const void *x, void *q, float *scale, void *stream);
+
+/* out[m][n] = sum over blocks b of 128 channels of a_scale[m][b] * w_scale[n / 128][b] * (sum of a[m][k] w[n][k] over the block), + bias[n] (fp32; NULL: none).
+ * The product of the two scales and the sums are fp32; out is rounded once to its type. */
+typedef struct onhip_f8_linear_desc {
+    int32_t rows, outputs, channels;
+    int32_t compute;             /* type of out */
+    long long a_stride, w_stride;  /* bytes, at most 2^22 */
+    long long out_stride;
+    long long a_scale_strides[2], w_scale_strides[2];
+} onhip_f8_linear_desc_t;
+int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float *a_scale, const void *w, const float *w_scale,
+                    const float *bias, void *out, void *stream);
+
 /* Max pooling over NCHW planes, every side padded by `pad`; oh x ow is the extent of the output
  * operand (at most the floor-mode shape onhip_maxpool_out_shape reports).  Replaces
  * device/x86/MaxPool/maxpool.c eval (:7-92) with pad_maxpool.h; the running maximum starts at

@@ -250,6 +250,29 @@ class MaskedAttentionDesc(C.Structure):
                 ("causal", C.c_int32), ("window", C.c_int32), ("q_offset", C.c_int32), ("compute", C.c_int32)]
 
 
+class NormDesc(C.Structure):
+    """onhip_norm_desc_t"""
+    _fields_ = [("rows", C.c_int32), ("channels", C.c_int32), ("compute", C.c_int32), ("f8", C.c_int32),
+                ("x_stride", C.c_longlong), ("residual_stride", C.c_longlong), ("sum_stride", C.c_longlong), ("out_stride", C.c_longlong),
+                ("scale_strides", C.c_longlong * 2), ("eps", C.c_float)]
+
+
+F8_ROWS, F8_GATED, F8_WEIGHTS = 0, 1, 2
+
+
+class F8RowsDesc(C.Structure):
+    """onhip_f8_rows_desc_t"""
+    _fields_ = [("rows", C.c_int32), ("channels", C.c_int32), ("compute", C.c_int32), ("form", C.c_int32),
+                ("x_stride", C.c_longlong), ("q_stride", C.c_longlong), ("scale_strides", C.c_longlong * 2)]
+
+
+class F8LinearDesc(C.Structure):
+    """onhip_f8_linear_desc_t"""
+    _fields_ = [("rows", C.c_int32), ("outputs", C.c_int32), ("channels", C.c_int32), ("compute", C.c_int32),
+                ("a_stride", C.c_longlong), ("w_stride", C.c_longlong), ("out_stride", C.c_longlong),
+                ("a_scale_strides", C.c_longlong * 2), ("w_scale_strides", C.c_longlong * 2)]
+
+
 def check_layout():
     assert C.sizeof(BUFFER_INFO_S) == 16
     assert C.sizeof(OPERAND_S) == 312 and OPERAND_S.shapes.offset == 276 and OPERAND_S.data_type.offset == 308

@@ -42,6 +42,7 @@ EXPORTS = ["onhip_init", "onhip_last_error", "onhip_set_tuning", "onhip_split_ta
            "onhip_h16_from_nchw_f32", "onhip_h16_to_nchw_f32", "onhip_h16_from_rows_f32", "onhip_h16_to_rows_f32",
            "onhip_conv2d_h16", "onhip_h16_first_width", "onhip_h16_first_channels", "onhip_h16_first_input_bytes", "onhip_h16_first_weight_bytes", "onhip_h16_first_from_nchw_f32", "onhip_h16_first_pack_weights", "onhip_conv2d_h16_first", "onhip_linear_h16", "onhip_attention",
            "onhip_cache_append", "onhip_cache_read", "onhip_attention_paged_workspace", "onhip_attention_paged", "onhip_attention_masked_workspace", "onhip_attention_masked",
+           "onhip_rms_norm", "onhip_f8_from_rows", "onhip_linear_f8",
            "onhip_ir_block_supported", "onhip_ir_block_packed_weight_bytes", "onhip_ir_block_pack_weights", "onhip_ir_block_f32",
            "onhip_conv2d_pw_supported", "onhip_conv2d_pw_packed_weight_bytes", "onhip_conv2d_pw_pack_weights", "onhip_conv2d_pw_f32",
            "onhip_add_f32", "onhip_relu_f32", "onhip_maxpool_out_shape", "onhip_maxpool_f32", "onhip_maxpool_s8_nhwc", "onhip_maxpool_s8_eval", "onhip_global_avgpool_f32",
@@ -138,6 +139,9 @@ def load():
     L.onhip_attention_masked_workspace.argtypes = [C.POINTER(abi.MaskedAttentionDesc)]
     L.onhip_attention_masked_workspace.restype = C.c_size_t
     L.onhip_attention_masked.argtypes = [C.POINTER(abi.MaskedAttentionDesc)] + [vp] * 7 + [C.c_size_t, vp]
+    L.onhip_rms_norm.argtypes = [C.POINTER(abi.NormDesc)] + [vp] * 7
+    L.onhip_f8_from_rows.argtypes = [C.POINTER(abi.F8RowsDesc)] + [vp] * 4
+    L.onhip_linear_f8.argtypes = [C.POINTER(abi.F8LinearDesc)] + [vp] * 7
     L.onhip_ir_block_supported.argtypes = [C.POINTER(ConvDesc)] * 3
     L.onhip_ir_block_packed_weight_bytes.argtypes = [i32, i32, i32]
     L.onhip_ir_block_packed_weight_bytes.restype = C.c_size_t
@@ -1000,6 +1004,185 @@ def attention_masked(q, k, v, scale=1.0, causal=False, window=0, softcap=0.0, sl
         rc = (_lib or load()).onhip_attention_masked(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges), _ptr(slopes), out.data_ptr(), _ptr(ws), nbytes, _stream())
         if rc:
             _check(rc, "onhip_attention_masked")
+    return out
+
+
+# ---- the linear layers of a generating transformer in 8-bit floating point: e4m3 rows with fp32 scales for blocks of 128 channels ----
+
+F8_BLOCK = 128
+
+
+def _f8_compute(what, dtype):
+    import torch
+    if dtype == torch.float32:
+        return abi.COMPUTE_F32
+    if dtype == torch.bfloat16:
+        return abi.COMPUTE_BF16
+    if dtype == torch.float16:
+        return abi.COMPUTE_F16
+    raise OnhipError(f"{what}: {dtype} is none of float32, bfloat16 and float16")
+
+
+def _rows_of(what, dtype, shape=None, **tensors):
+    """checks matrices whose rows are contiguous, None left out"""
+    _need(what, dtype, shape, **tensors)
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dim() != 2:
+            raise OnhipError(f"{what}: {name} has {t.dim()} dimensions, not 2")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise OnhipError(f"{what}: the rows of {name} must be contiguous")
+
+
+def _f8_blocks(n):
+    return -(-n // F8_BLOCK)
+
+
+def _f8_empty(like, rows, n):
+    """e4m3 rows that lie a multiple of 16 bytes apart"""
+    import torch
+    if n % 16 == 0:
+        return like.new_empty((rows, n), dtype=torch.float8_e4m3fn)
+    return like.new_empty((rows, (n + 15) // 16 * 16), dtype=torch.float8_e4m3fn)[:, :n]
+
+
+def _f8_results(what, rows, n, scale_rows, q, scale):
+    """checks e4m3 rows and their scales as results; their strides"""
+    import torch
+    _rows_of(what, torch.float8_e4m3fn, (rows, n), out=q)
+    _need(what, torch.float32, (scale_rows, _f8_blocks(n)), scale=scale)
+    return (n + 15) // 16 * 16 if q is None else q.stride(0), (_f8_blocks(n), 1) if scale is None else scale.stride()
+
+
+def _norm_plan(x, weight, eps, residual, f8, out, sum_out, scale_out):
+    import torch
+    what = "rms_norm"
+    compute = _f8_compute(what, x.dtype)
+    _rows_of(what, x.dtype, x=x)
+    rows, n = x.shape
+    if n < 1:
+        raise OnhipError(f"{what}: rows without channels")
+    _int32(what, rows=rows, channels=n)
+    _rows_of(what, x.dtype, (rows, n), residual=residual, sum_out=sum_out)
+    _need(what, torch.float32, (n,), flat=True, weight=weight)
+    if sum_out is not None and residual is None:
+        raise OnhipError(f"{what}: sum_out without a residual")
+    if f8:
+        out_stride, scale_strides = _f8_results(what, rows, n, rows, out, scale_out)
+    else:
+        if scale_out is not None:
+            raise OnhipError(f"{what}: scales of a result in {x.dtype}")
+        _rows_of(what, x.dtype, (rows, n), out=out)
+        out_stride, scale_strides = n if out is None else out.stride(0), (0, 0)
+    d = abi.NormDesc(rows, n, compute, int(f8), x.stride(0), 0 if residual is None else residual.stride(0), n if sum_out is None else sum_out.stride(0), out_stride, scale_strides, eps)
+    return C.byref(d), rows, n, _f8_blocks(n), rows == 0
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None, f8=False, out=None, sum_out=None, scale_out=None):
+    """y = h / sqrt(mean(h^2) + eps) * weight of h = x + residual: x and residual [rows, channels] in bfloat16, float16 or float32 (any row stride), weight [channels] in
+    float32.  Returns y in x's type or, with f8, e4m3 rows and scales [rows, blocks of 128]; and behind them, where there is a residual, h rounded to
+    x's type (sum_out, which may be x or residual; so may `out` where it is of their type)"""
+    eps = eps if type(eps) is float else _real("rms_norm", "eps", eps)
+    f8 = bool(f8)
+    key = (_device(), x.dtype, x.get_device(), x.shape, x.stride(), _flat(weight), eps, _meta(residual), f8, _meta(out), _meta(sum_out), _meta(scale_out))
+    last = _last.get("norm")
+    d, rows, n, blocks, empty = last[1] if last is not None and last[0] == key else _plan("norm", key, _norm_plan, x, weight, eps, residual, f8, out, sum_out, scale_out)
+    if out is None:
+        out = _f8_empty(x, rows, n) if f8 else x.new_empty((rows, n))
+    if f8 and scale_out is None:
+        scale_out = _scales(x, rows, blocks)
+    if residual is not None and sum_out is None:
+        sum_out = x.new_empty((rows, n))
+    if not empty:
+        rc = (_lib or load()).onhip_rms_norm(d, x.data_ptr(), _ptr(residual), _ptr(weight), out.data_ptr(), _ptr(scale_out), _ptr(sum_out), _stream())
+        if rc:
+            _check(rc, "onhip_rms_norm")
+    if f8:
+        return (out, scale_out) if residual is None else (out, scale_out, sum_out)
+    return out if residual is None else (out, sum_out)
+
+
+def _scales(like, rows, blocks):
+    import torch
+    return like.new_empty((rows, blocks), dtype=torch.float32)
+
+
+def _f8_rows_plan(what, form, x, q, scale):
+    compute = _f8_compute(what, x.dtype)
+    _rows_of(what, x.dtype, x=x)
+    rows, n = x.shape
+    if form == abi.F8_GATED:
+        if n % 2:
+            raise OnhipError(f"{what}: gated rows of {n} channels, not two halves")
+        n //= 2
+    if n < 1:
+        raise OnhipError(f"{what}: rows without channels")
+    _int32(what, rows=rows, channels=n)
+    scale_rows = _f8_blocks(rows) if form == abi.F8_WEIGHTS else rows
+    q_stride, scale_strides = _f8_results(what, rows, n, scale_rows, q, scale)
+    d = abi.F8RowsDesc(rows, n, compute, form, x.stride(0), q_stride, scale_strides)
+    return C.byref(d), rows, n, scale_rows, _f8_blocks(n), rows == 0
+
+
+def _f8_rows(what, form, x, q, scale):
+    key = (_device(), form, x.dtype, x.get_device(), x.shape, x.stride(), _meta(q), _meta(scale))
+    last = _last.get("f8 rows")
+    d, rows, n, scale_rows, blocks, empty = last[1] if last is not None and last[0] == key else _plan("f8 rows", key, _f8_rows_plan, what, form, x, q, scale)
+    if q is None:
+        q = _f8_empty(x, rows, n)
+    if scale is None:
+        scale = _scales(x, scale_rows, blocks)
+    if not empty:
+        rc = (_lib or load()).onhip_f8_from_rows(d, x.data_ptr(), q.data_ptr(), scale.data_ptr(), _stream())
+        if rc:
+            _check(rc, "onhip_f8_from_rows")
+    return q, scale
+
+
+def f8_from_rows(x, gated=False, out=None, scale_out=None):
+    """rows [rows, channels] in bfloat16, float16 or float32 (any row stride) to e4m3 rows and their scales [rows, blocks of 128]; gated: rows of twice as many
+    channels, of which silu(first half) * second half is taken"""
+    return _f8_rows("f8_from_rows", abi.F8_GATED if gated else abi.F8_ROWS, x, out, scale_out)
+
+
+def f8_from_weights(w, out=None, scale_out=None):
+    """weights [outputs, channels] to e4m3 rows and scales [blocks of 128 outputs, blocks of 128 channels]: linear_f8's second operand"""
+    return _f8_rows("f8_from_weights", abi.F8_WEIGHTS, w, out, scale_out)
+
+
+def _linear_f8_plan(a, a_scale, w, w_scale, bias, dtype, out):
+    import torch
+    what = "linear_f8"
+    compute = _f8_compute(what, dtype)
+    _rows_of(what, torch.float8_e4m3fn, a=a, w=w)
+    (rows, n), outputs = a.shape, w.shape[0]
+    if w.shape[1] != n or n < 1:
+        raise OnhipError(f"{what}: rows of {n} channels and weights of {w.shape[1]}")
+    _int32(what, rows=rows, outputs=outputs, channels=n)
+    _need(what, torch.float32, (rows, _f8_blocks(n)), a_scale=a_scale)
+    _need(what, torch.float32, (_f8_blocks(outputs), _f8_blocks(n)), w_scale=w_scale)
+    _need(what, torch.float32, (outputs,), flat=True, bias=bias)
+    _rows_of(what, dtype, (rows, outputs), out=out)
+    d = abi.F8LinearDesc(rows, outputs, n, compute, a.stride(0), w.stride(0), outputs if out is None else out.stride(0), a_scale.stride(), w_scale.stride())
+    return C.byref(d), (rows, outputs), rows == 0 or outputs == 0
+
+
+def linear_f8(a, a_scale, w, w_scale, bias=None, dtype=None, out=None):
+    """a [rows, channels] times w [outputs, channels], both e4m3 rows with fp32 scales ([rows, blocks of 128 channels] and [blocks of 128 outputs, blocks of 128
+    channels], any strides), plus bias [outputs] (float32): [rows, outputs] in `dtype` (float32, float16 or bfloat16, which it is unless given)"""
+    import torch
+    dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
+    key = (_device(), a.dtype, a.get_device(), a.shape, a.stride(), a_scale.dtype, a_scale.get_device(), a_scale.shape, a_scale.stride(),
+           w.dtype, w.get_device(), w.shape, w.stride(), w_scale.dtype, w_scale.get_device(), w_scale.shape, w_scale.stride(), _flat(bias), dtype, _meta(out))
+    last = _last.get("linear f8")
+    d, shape, empty = last[1] if last is not None and last[0] == key else _plan("linear f8", key, _linear_f8_plan, a, a_scale, w, w_scale, bias, dtype, out)
+    if out is None:
+        out = a.new_empty(shape, dtype=dtype)
+    if not empty:
+        rc = (_lib or load()).onhip_linear_f8(d, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), out.data_ptr(), _stream())
+        if rc:
+            _check(rc, "onhip_linear_f8")
     return out
 
 

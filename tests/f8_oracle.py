@@ -63,14 +63,23 @@ def norm(x, residual, weight, eps):
     return h, y, ((n / 64 + 22 + 2) / 2 + 10) * 2.0 ** -24 * y.abs()
 
 
-def linear(a, a_scale, w, w_scale, bias=None):
+def linear(a, a_scale, w, w_scale, bias=None, cut=False):
     """the product and what it may be off in fp32: the scales' product, a block's 128 additions (each off by a unit of the magnitudes' sum at most, however the matrix
-    instruction orders and cuts them), the fused sums over blocks, the bias"""
+    instruction orders and cuts them), the fused sums over blocks, the bias.
+
+    cut: sums of eight products with 13 bits below the power of two of the largest: a product of two e4m3 has 8 bits, so the largest is whole, and each of the seven others loses
+    less than 2^-13 of the largest, which is at most the eight magnitudes' sum: 7 2^-13 of the magnitudes' sum over all channels."""
     x, y = values(a, a_scale), values(w, w_scale, True)
     out, mass = x @ y.t(), x.abs() @ y.abs().t()
+    far = (128 + blocks(a.shape[1]) + 4) * 2.0 ** -23 * mass + (7 * 2.0 ** -13 * mass if cut else 0)
     if bias is not None:
-        out, mass = out + bias.double(), mass + bias.double().abs()
-    return out, (128 + blocks(a.shape[1]) + 4) * 2.0 ** -23 * mass
+        out, far = out + bias.double(), far + 2.0 ** -23 * (mass + bias.double().abs())
+    return out, far
+
+
+def cuts(m, dtype):
+    """whether a product of m rows may sum with 13 bits: more than 64 rows with a result in 16 bits"""
+    return m > 64 and dtype != torch.float32
 
 
 def check(got, ref, off):

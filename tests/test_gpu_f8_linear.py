@@ -34,7 +34,7 @@ def test_product(dtype, m, n, k):
     for b in (None, bias):
         got = hip.linear_f8(a, sa, w, sw, bias=b, dtype=DT[dtype])
         torch.cuda.synchronize()
-        o.check(got, *o.linear(a, sa, w, sw, b))
+        o.check(got, *o.linear(a, sa, w, sw, b, o.cuts(m, DT[dtype])))
 
 
 @pytest.mark.parametrize("m", [1, 20, 70, 300])
@@ -43,7 +43,7 @@ def test_strides(m):
     hip.init(0)
     n, k = 300, 520
     (a, sa), (w, sw) = operand(m, k, 1, pad=48), operand(n, k, 2, True, pad=32)
-    ref, off = o.linear(a, sa, w, sw)
+    ref, off = o.linear(a, sa, w, sw, cut=o.cuts(m, torch.bfloat16))
     turned = [t.t().contiguous().t() for t in (sa, sw)]
     for first in (0, 1, 4):
         wide = torch.full((m, n + 12), 3.0, dtype=torch.bfloat16, device="cuda")
@@ -89,14 +89,14 @@ def test_far_results():
     (a, sa), (w, sw) = operand(m, k, 1), operand(n, k, 2, True)
     got = hip.linear_f8(a, sa, w, sw)
     for rows in (slice(0, 130), slice(65500, 65600), slice(m - 130, m)):
-        o.check(got[rows], *o.linear(a[rows], sa[rows], w, sw))
+        o.check(got[rows], *o.linear(a[rows], sa[rows], w, sw, cut=True))
     del got
     n, k = 1100, 300
     (a, sa), (w, sw) = operand(150, k, 1), operand(n, k, 2, True)
     far = torch.zeros((n - 1 << 22) + 4096, dtype=torch.uint8, device="cuda").view(o.F8).as_strided((n, k), (1 << 22, 1))
     far.copy_(w)
     for rows in (1, 30, 150):
-        o.check(hip.linear_f8(a[:rows], sa[:rows], far, sw), *o.linear(a[:rows], sa[:rows], w, sw))
+        o.check(hip.linear_f8(a[:rows], sa[:rows], far, sw), *o.linear(a[:rows], sa[:rows], w, sw, cut=o.cuts(rows, torch.bfloat16)))
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (32, 4096, 4096), (300, 4096, 11008), (1024, 4096, 4096)])
@@ -105,6 +105,6 @@ def test_repeats(m, n, k):
     hip.init(0)
     (a, sa), (w, sw) = operand(m, k, 1), operand(n, k, 2, True)
     want = hip.linear_f8(a, sa, w, sw)
-    o.check(want, *o.linear(a, sa, w, sw))
+    o.check(want, *o.linear(a, sa, w, sw, cut=o.cuts(m, torch.bfloat16)))
     for _ in range(5):
         assert torch.equal(hip.linear_f8(a, sa, w, sw), want)

@@ -23,7 +23,7 @@ struct F8LinearParams {
     long long a_ss[2], w_ss[2];      // floats between rows and blocks
     int m, n, k;
     int tiles_m, tiles_n;
-    Div31 by_group, by_last;         // tiles in eight rows of them; rows of tiles in the last such group
+    Div31 by_group, by_last;         // tiles in HIGH rows of them; rows of tiles in the last such group
     bool vec, wide;                  // four results are one aligned store; eight, in rows up to 2^22 bytes apart
     bool quads;                      // scales of a row's blocks lie side by side, four of them at least
 };
@@ -94,14 +94,13 @@ template <int DT> __device__ __forceinline__ void store4(const F8LinearParams &p
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
-// A workgroup has 16 NT outputs of AM rows, its eight wavefronts every eighth block of channels each.  A wavefront has a ring of DEPTH blocks in LDS of its own,
-// which nobody else waits for; whole lines come in (a load of matrix operands straight into registers takes sixteen rows at once, a line each:
+// A workgroup has 16 NT outputs of AM rows, its wavefronts a run of the blocks of channels each.  A wavefront has a place for a block in LDS of its own,
+// which nobody else waits for, and takes the next one when it has read the last; whole lines come in (a load of matrix operands straight into registers takes sixteen rows at once, a line each:
 // 10 bytes a cycle and compute unit were measured so).  The wavefronts' sums meet in LDS, in one order.
-template <int DT, int AM, int NT, int DEPTH, int WAVES>
+template <int DT, int AM, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int MT = AM < 16 ? 1 : AM / 16, SLOT = NT * 2048 + AM * 128 + 256, LOADS = NT * 2 + AM / 8 + 1;
-    constexpr int RING = WAVES * DEPTH * SLOT, JOIN = WAVES * NT * MT * 1024;
+    constexpr int MT = AM < 16 ? 1 : AM / 16, CHUNK = 1024, SLOT = NT * 2048 + AM * 128 + 2 * CHUNK, RING = WAVES * SLOT, JOIN = WAVES * NT * MT * 1024;
     static_assert(AM < 64, "a lane for each row's scale, and for the weights'");
     __shared__ __attribute__((aligned(1024))) char lds[RING > JOIN ? RING : JOIN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -125,79 +124,76 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
     // a lane's scale: of row `lane`, of the weights behind the rows
     const float *scales = lane < AM ? p.a_scale + (m0 + min(lane, rows_m - 1)) * p.a_ss[0] : p.w_scale + n0 / 128 * p.w_ss[0];
     const long long scale_step = lane < AM ? p.a_ss[1] : p.w_ss[1];
-    const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds + wave * DEPTH * SLOT;
-    auto ask = [&](int kb, int d) __attribute__((always_inline)) {
-        const bool live = kb < k_blocks;   // one that is not there is not fetched
-        const i32x4 rw = descriptor(w_base, live ? w_bytes : 0u), ra = descriptor(a_base, live ? a_bytes : 0u);
-        const int at = live ? kb : 0;
-        const unsigned to = lds0 + d * SLOT;
+    const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds + wave * SLOT;
+    const i32x4 rw = descriptor(w_base, w_bytes), ra = descriptor(a_base, a_bytes);
+    const int share = (k_blocks + WAVES - 1) / WAVES, begin = wave * share, end = min(begin + share, k_blocks);
+    auto ask = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < NT * 2; ++t) load_to_lds(rw, w_off[t], (unsigned) at * 128u, to + t * 1024);
+        for (int t = 0; t < NT * 2; ++t) load_to_lds(rw, w_off[t], (unsigned) kb * 128u, lds0 + t * 1024);
 #pragma unroll
-        for (int t = 0; t < AM / 8; ++t) load_to_lds(ra, a_off[t], (unsigned) at * 128u, to + NT * 2048 + t * 1024);
-        word_to_lds(scales + at * scale_step, to + NT * 2048 + AM * 128);
+        for (int t = 0; t < AM / 8; ++t) load_to_lds(ra, a_off[t], (unsigned) kb * 128u, lds0 + NT * 2048 + t * 1024);
+        const int i = kb - begin;
+        const unsigned to = lds0 + NT * 2048 + AM * 128 + (i / 4 & 1) * CHUNK;
+        if (!p.quads) word_to_lds(scales + kb * scale_step, to + i % 4 * 256);
+        else if (i % 4 == 0) quad_to_lds(scales + min(kb, k_blocks - 4), to);   // of four blocks, the last four as they are
     };
+    const int row_step = p.quads ? 16 : 4;
     f32x4 acc[NT][MT] = {};
+    if (begin < end) ask(begin);
+    const char *slot = lds + wave * SLOT;
+    for (int kb = begin; kb < end; ++kb) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        i32x4 w[NT][2], a[MT][2];
+        float s[MT];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) ask(wave + WAVES * d, d);
-    for (int first = wave; first < k_blocks; first += WAVES * DEPTH) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int kb = first + WAVES * d;
-            if (kb >= k_blocks) break;
-            const char *slot = lds + (wave * DEPTH + d) * SLOT;
-            asm volatile("s_waitcnt vmcnt(%0)" :: "n"((DEPTH - 1) * LOADS) : "memory");
-            i32x4 w[NT][2], a[MT][2];
-            float s[MT];
+            for (int u = 0; u < NT; ++u) w[u][h] = *reinterpret_cast<const i32x4 *>(slot + (u * 16 + li) * 128 + (lane_unit(lq, h) ^ (li / 2)) * 16);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int row = AM < 16 ? li % AM : t * 16 + li;   // columns past the last row are not stored
+                a[t][h] = *reinterpret_cast<const i32x4 *>(slot + NT * 2048 + row * 128 + (lane_unit(lq, h) ^ (row / 2 % 8)) * 16);
+            }
+        }
+        const int i = kb - begin, first = kb - i % 4;
+        const char *factor = slot + NT * 2048 + AM * 128 + (i / 4 & 1) * CHUNK + (p.quads ? (kb - min(first, k_blocks - 4)) * 4 : i % 4 * 256);
+        const float sw = *reinterpret_cast<const float *>(factor + AM * row_step);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) s[t] = *reinterpret_cast<const float *>(factor + (AM < 16 ? li % AM : t * 16 + li) * row_step) * sw;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read, so that the place can take another block
+        if (kb + 1 < end) ask(kb + 1);
+        if (kb * 128 + 128 > p.k) {   // the last block: nothing behind a row's end takes part
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                const int keep = p.k - (kb * 128 + lane_unit(lq, h) * 16);
 #pragma unroll
-                for (int u = 0; u < NT; ++u) w[u][h] = *reinterpret_cast<const i32x4 *>(slot + (u * 16 + li) * 128 + (lane_unit(lq, h) ^ (li / 2)) * 16);
+                for (int u = 0; u < NT; ++u) w[u][h] = f8_kept(w[u][h], keep);
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int row = AM < 16 ? li % AM : t * 16 + li;   // columns past the last row are not stored
-                    a[t][h] = *reinterpret_cast<const i32x4 *>(slot + NT * 2048 + row * 128 + (lane_unit(lq, h) ^ (row / 2 % 8)) * 16);
-                }
+                for (int t = 0; t < MT; ++t) a[t][h] = f8_kept(a[t][h], keep);
             }
-            const float *factor = reinterpret_cast<const float *>(slot + NT * 2048 + AM * 128);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) s[t] = factor[AM < 16 ? li % AM : t * 16 + li] * factor[AM];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read, so that the slot can take another block
-            ask(kb + WAVES * DEPTH, d);
-            if (kb * 128 + 128 > p.k) {   // the last block: nothing behind a row's end takes part
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int keep = p.k - (kb * 128 + lane_unit(lq, h) * 16);
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) w[u][h] = f8_kept(w[u][h], keep);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) a[t][h] = f8_kept(a[t][h], keep);
-                }
-            }
-            f32x4 part[NT][MT] = {};
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    bf16x8 y[MT];
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) y[t] = f8_widened(a[t][h][2 * e], a[t][h][2 * e + 1]);
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) {
-                        const bf16x8 x = f8_widened(w[u][h][2 * e], w[u][h][2 * e + 1]);
-#pragma unroll
-                        for (int t = 0; t < MT; ++t) part[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y[t], part[u][t], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[u][t][i] = __builtin_fmaf(part[u][t][i], s[t], acc[u][t][i]);
         }
+        f32x4 part[NT][MT] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                bf16x8 y[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) y[t] = f8_widened(a[t][h][2 * e], a[t][h][2 * e + 1]);
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+                    const bf16x8 x = f8_widened(w[u][h][2 * e], w[u][h][2 * e + 1]);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) part[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y[t], part[u][t], 0, 0, 0);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[u][t][i] = __builtin_fmaf(part[u][t][i], s[t], acc[u][t][i]);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads that wrote nothing but zeros are still on their way to LDS
     __syncthreads();
     f32x4 *parts = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
@@ -219,124 +215,6 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
 #endif
 }
 
-// BN weight rows x BM rows a workgroup, WN x WM wavefronts
-template <int DT, int BN, int BM, int WN, int WM>
-__global__ __launch_bounds__(64 * WN * WM) void f8_linear_kernel(const F8LinearParams p) {
-    constexpr int WAVES = WN * WM, TN = BN / WN / 32, TM = BM / WM / 32, STAGE = (BN + BM) * 128;
-    constexpr int LOADS_N = BN / 8 / WAVES, LOADS_M = BM / 8 / WAVES;   // eight rows a load
-    static_assert(BN / WN <= 128 && LOADS_N >= 1 && LOADS_M >= 1, "a wavefront's weights share a scale, and every wavefront loads");
-    __shared__ __attribute__((aligned(1024))) char lds[2][STAGE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int li = lane & 31, lh = lane >> 5, wn = wave / WM, wm = wave % WM;
-    // tiles: an XCD has a run of them, eight rows of tiles by columns
-    int tn, tm;
-    {
-        const int bid = blockIdx.x, nb = (int) gridDim.x, q = nb >> 3, rem = nb & 7, xcd = bid & 7;
-        const int lid = xcd * q + (xcd < rem ? xcd : rem) + (bid >> 3);
-        const int group = lid / (8 * p.tiles_n), left = lid - group * 8 * p.tiles_n, high = min(8, p.tiles_m - group * 8);
-        tn = left / high;
-        tm = group * 8 + left - tn * high;
-    }
-    const int n0 = tn * BN, m0 = tm * BM;
-    const int k_blocks = (p.k + 127) / 128;
-
-    const int rows_n = min(BN, p.n - n0), rows_m = min(BM, p.m - m0), k16 = (p.k + 15) & ~15;
-    const char *w_base = p.w + (long long) n0 * p.ws, *a_base = p.a + (long long) m0 * p.as;
-    const unsigned w_bytes = (unsigned) ((rows_n - 1) * p.ws + k16), a_bytes = (unsigned) ((rows_m - 1) * p.as + k16);
-    unsigned w_off[LOADS_N], a_off[LOADS_M];
-    const int lrow = lane / 8;
-#pragma unroll
-    for (int t = 0; t < LOADS_N; ++t) {
-        const int row = (wave * LOADS_N + t) * 8 + lrow;
-        w_off[t] = row < rows_n ? (unsigned) (row * p.ws) + ((lane % 8) ^ (row / 2 % 8)) * 16 : OOB;
-    }
-#pragma unroll
-    for (int t = 0; t < LOADS_M; ++t) {
-        const int row = (wave * LOADS_M + t) * 8 + lrow;
-        a_off[t] = row < rows_m ? (unsigned) (row * p.as) + ((lane % 8) ^ (row / 2 % 8)) * 16 : OOB;
-    }
-    const i32x4 rw = descriptor(w_base, w_bytes), ra = descriptor(a_base, a_bytes);
-    const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) &lds[0][0];
-    auto issue = [&](int kb, int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int t = 0; t < LOADS_N; ++t) load_to_lds(rw, w_off[t], (unsigned) kb * 128u, lds0 + buf * STAGE + (wave * LOADS_N + t) * 1024);
-#pragma unroll
-        for (int t = 0; t < LOADS_M; ++t) load_to_lds(ra, a_off[t], (unsigned) kb * 128u, lds0 + buf * STAGE + BN * 128 + (wave * LOADS_M + t) * 1024);
-    };
-
-    // factors of a block: this lane's rows m, and the wavefront's weights
-    const int m_wave = m0 + wm * (BM / WM), n_wave = n0 + wn * (BN / WN);
-    const float *sw = p.w_scale + (n_wave < p.n ? n_wave / 128 : 0) * p.w_ss[0];
-    const float *sa[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) sa[t] = p.a_scale + (long long) min(m_wave + t * 32 + li, p.m - 1) * p.a_ss[0];
-
-    f32x16 acc[TN][TM] = {};
-    issue(0, 0);
-    for (int kb = 0; kb < k_blocks; ++kb) {
-        const int buf = kb & 1;
-        float s[TM];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) s[t] = sa[t][kb * p.a_ss[1]] * sw[kb * p.w_ss[1]];
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this stage is there, and everybody has read the other one
-        __syncthreads();
-        char *stage = lds[buf];
-        const int there = p.k - kb * 128;
-        if (there < 128) {   // the last block: nothing behind a row's end takes part
-            for (int i = threadIdx.x; i < (BN + BM) * 8; i += 64 * WAVES) {
-                const int row = i / 8, unit = (i % 8) ^ (row / 2 % 8), keep = there - unit * 16;
-                if (keep >= 16) continue;
-                unsigned *at = reinterpret_cast<unsigned *>(stage + i * 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int bytes = keep - 4 * j;
-                    at[j] = bytes >= 4 ? at[j] : bytes <= 0 ? 0u : at[j] & (0xffffffffu >> (32 - 8 * bytes));
-                }
-            }
-            __syncthreads();
-        }
-        if (kb + 1 < k_blocks) issue(kb + 1, buf ^ 1);
-        // this lane's 16 bytes of a row: units 2 i and 2 i + 1 are the two halves of the wavefront's
-        auto operand = [&](int row, int i, bf16x8 (&x)[2]) __attribute__((always_inline)) {
-            const i32x4 q = *reinterpret_cast<const i32x4 *>(stage + row * 128 + ((2 * i + lh) ^ (row / 2 % 8)) * 16);
-            x[0] = f8_widened(q[0], q[1]);
-            x[1] = f8_widened(q[2], q[3]);
-        };
-        f32x16 part[TN][TM] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bf16x8 a[TN][2], b[TM][2];
-#pragma unroll
-            for (int t = 0; t < TM; ++t) operand(BN + wm * (BM / WM) + t * 32 + li, i, b[t]);
-#pragma unroll
-            for (int u = 0; u < TN; ++u) operand(wn * (BN / WN) + u * 32 + li, i, a[u]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int u = 0; u < TN; ++u)
-#pragma unroll
-                    for (int t = 0; t < TM; ++t) part[u][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[u][h], b[t][h], part[u][t], 0, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < TN; ++u)
-#pragma unroll
-            for (int t = 0; t < TM; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[u][t][r] = __builtin_fmaf(part[u][t][r], s[t], acc[u][t][r]);
-    }
-
-    // a lane has 4 consecutive n in each of four groups of eight, of row m
-#pragma unroll
-    for (int u = 0; u < TN; ++u)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const int m = m_wave + t * 32 + li, n = n_wave + u * 32 + g * 8 + lh * 4;
-                if (m < p.m && n < p.n) store4<DT>(p, m, n, f32x4{acc[u][t][g * 4], acc[u][t][g * 4 + 1], acc[u][t][g * 4 + 2], acc[u][t][g * 4 + 3]});
-            }
-}
-
 // ---- many rows -----------------------------------------------------------------------------------------------------
 // A workgroup a compute unit walks over tiles of 256 weights x 256 rows, eight wavefronts of 128 x 64: 2048 cycles of matrix instructions a block of channels, whose tiles come in during the
 // block before, across the ends of tiles.  Matrix instructions on e4m3 itself: they take half the time of those in bf16 and sum eight products at a time with 13 bits below the largest
@@ -349,6 +227,8 @@ __device__ __forceinline__ f32x4 f8_mma(i32x8 a, i32x8 b) {
 #endif
 }
 
+constexpr int HIGH = 4;   // rows of tiles that go together: 32 workgroups of an XCD share 4 x 8 panels at a time
+
 template <int DT>
 __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -358,7 +238,7 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
     const int li = lane & 15, lq = lane >> 4, wn = wave / WM, wm = wave % WM;
     const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds;
     const int k_blocks = (p.k + 127) / 128, k16 = (p.k + 15) & ~15, blocks_n = (p.n + 127) / 128;
-    // an XCD has a run of the tiles, eight rows of tiles by columns; its workgroups take them in turn
+    // an XCD has a run of the tiles, HIGH rows of tiles by columns; its workgroups take them in turn
     const int tiles = p.tiles_m * p.tiles_n, xcd = (int) blockIdx.x & 7, each = tiles >> 3, over = tiles & 7;
     const int begin = xcd * each + min(xcd, over), end = begin + each + (xcd < over), step = ((int) gridDim.x - xcd + 7) >> 3;
 
@@ -376,13 +256,13 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
     const long long scale_step = of_rows ? p.a_ss[1] : p.w_ss[1];
     auto set_tile = [&](int lid) __attribute__((always_inline)) {
         const bool live = lid < end;   // behind the last one nothing is fetched
-        const int at = live ? lid : begin, group = (int) div31((unsigned) at, p.by_group), left = at - group * 8 * p.tiles_n;
-        const bool whole = group * 8 + 8 <= p.tiles_m;
-        const int high = whole ? 8 : p.tiles_m - group * 8, tn = whole ? left >> 3 : (int) div31((unsigned) left, p.by_last);
+        const int at = live ? lid : begin, group = (int) div31((unsigned) at, p.by_group), left = at - group * HIGH * p.tiles_n;
+        const bool whole = group * HIGH + HIGH <= p.tiles_m;
+        const int high = whole ? HIGH : p.tiles_m - group * HIGH, tn = whole ? left / HIGH : (int) div31((unsigned) left, p.by_last);
         next.lid = lid;
         next.kb = 0;
         next.n0 = tn * BN;
-        next.m0 = (group * 8 + left - tn * high) * BM;
+        next.m0 = (group * HIGH + left - tn * high) * BM;
         const int rows_n = min(BN, p.n - next.n0), rows_m = min(BM, p.m - next.m0);
         next.w = descriptor(p.w + (long long) next.n0 * p.ws, live ? (unsigned) ((rows_n - 1) * p.ws + k16) : 0u);
         next.a = descriptor(p.a + (long long) next.m0 * p.as, live ? (unsigned) ((rows_m - 1) * p.as + k16) : 0u);
@@ -439,10 +319,6 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
             const int first = p.quads ? min(kb & ~3, k_blocks - 4) : kb & ~3;   // of the chunk
             const char *factors = lds + 2 * TILES + chunk * CHUNK + (kb - first) * (p.quads ? 4 : (BM + 64) * 4);
             const int row_step = p.quads ? 16 : 4;
-            const float sw = *reinterpret_cast<const float *>(factors + (BM + wn) * row_step);
-            float s[TM];
-#pragma unroll
-            for (int t = 0; t < TM; ++t) s[t] = *reinterpret_cast<const float *>(factors + (wm * 64 + t * 16 + li) * row_step) * sw;
             auto operand = [&](int row) __attribute__((always_inline)) {
                 const int swz = row / 2 % 8;
                 const i32x4 x = *reinterpret_cast<const i32x4 *>(stage + row * 128 + (lane_unit(lq, 0) ^ swz) * 16), y = *reinterpret_cast<const i32x4 *>(stage + row * 128 + (lane_unit(lq, 1) ^ swz) * 16);
@@ -450,26 +326,34 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
             };
             // multiply-adds of a tile three matrix instructions behind it: its result is there, and the vector pipe works next to the matrix cores
             constexpr int BACK = 3;
-            i32x8 a[2], b[TM];
+            i32x8 a[3], b[TM];
             f32x4 part[BACK + 1];
+            float s[TM];
             auto add = [&](int j) __attribute__((always_inline)) {
                 const int u = j / TM, t = j % TM;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[u][t][r] = __builtin_fmaf(part[j % (BACK + 1)][r], s[t], acc[u][t][r]);
             };
+            advance();
+            load_scales();
+            __builtin_amdgcn_sched_barrier(0);
             a[0] = operand(wn * 128 + li);
 #pragma unroll
             for (int t = 0; t < TM; ++t) b[t] = operand(BN + wm * 64 + t * 16 + li);
-            advance();
-            load_scales();
+            __builtin_amdgcn_sched_barrier(0);
+            const float sw = *reinterpret_cast<const float *>(factors + (BM + wn) * row_step);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) s[t] = *reinterpret_cast<const float *>(factors + (wm * 64 + t * 16 + li) * row_step);
+            a[1] = operand(wn * 128 + 16 + li);
 #pragma unroll
             for (int u = 0; u < TN; ++u) {   // one basic block: across branches the multiply-adds would be put off
-                if (u + 1 < TN) a[(u + 1) & 1] = operand(wn * 128 + (u + 1) * 16 + li);
+                if (u + 2 < TN) a[(u + 2) % 3] = operand(wn * 128 + (u + 2) * 16 + li);
 #pragma unroll
                 for (int t = 0; t < TM; ++t) {
                     const int j = u * TM + t;
                     __builtin_amdgcn_sched_barrier(0);
-                    part[j % (BACK + 1)] = f8_mma(a[u & 1], b[t]);
+                    part[j % (BACK + 1)] = f8_mma(a[u % 3], b[t]);
+                    if (j < TM) s[j] *= sw;
                     if (j >= BACK) add(j - BACK);
                     if (j < 16 && j % 2 == 1) load_tiles(j / 2, buf ^ 1);
                 }
@@ -511,7 +395,7 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
                         x[i] = z[0];
                         y[i] = z[1];
                     }
-                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, n_wide + u * 16 + 8 <= p.n ? off + u * 32 : OOB, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, n_wide + u * 16 + 8 <= p.n ? off + u * 32 : OOB, 0, 2);   // not kept in the caches
                 }
             }
             stored = true;
@@ -536,16 +420,183 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
 #endif
 }
 
-template <int DT, int AM, int NT, int DEPTH, int WAVES> static int few_launch(const F8LinearParams &p, hipStream_t stream) {
-    hipLaunchKernelGGL((f8_few_kernel<DT, AM, NT, DEPTH, WAVES>), dim3((unsigned) ((p.n + 16 * NT - 1) / (16 * NT)), (unsigned) ((p.m + AM - 1) / AM)), dim3(64 * WAVES), 0, stream, p);
-    ONHIP_CHECK_HIP(hipGetLastError());
-    return ONHIP_OK;
+// ---- some rows -----------------------------------------------------------------------------------------------------
+// A workgroup has BN weights x BM rows, its wavefronts WN x WM parts of them in each of KG groups, and a group a run of the blocks of channels, in a ring of DEPTH blocks: tiles
+// enough for the compute units, and wavefronts enough for a unit, where there are few rows.  The groups' sums meet in LDS, in one order.
+// EXACT: matrix instructions in bf16, which sum in fp32.
+template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
+__global__ __launch_bounds__(64 * KG * WN * WM) void f8_tile_kernel(const F8LinearParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int GW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16, LN = BN / 8 / GW, LM = BM / 8 / GW, LOADS = LN + LM;
+    constexpr int SLOT = (BN + BM) * 128, CHUNK = (BM + 64) * 16, RING = KG * (DEPTH * SLOT + 2 * CHUNK), JOIN = KG * GW * TN * TM * 1024;
+    static_assert(BN / WN <= 128 && BM % 64 == 0 && BM / 64 < GW && LN >= 1 && LM >= 1, "a wavefront's weights share a scale, 64 rows' scales are a wavefront's load, those of the weights another's, and every wavefront loads");
+    __shared__ __attribute__((aligned(1024))) char lds[RING > JOIN ? RING : JOIN];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, lq = lane >> 4, kg = wave / GW, gw = wave % GW, wn = gw / WM, wm = gw % WM;
+    int n0, m0;
+    {   // an XCD has a run of the tiles, all rows of a column of them by the next
+        const int bid = blockIdx.x, nb = (int) gridDim.x, q = nb >> 3, rem = nb & 7, xcd = bid & 7;
+        const unsigned lid = (unsigned) (xcd * q + min(xcd, rem) + (bid >> 3)), tn = div31(lid, p.by_last);
+        n0 = (int) tn * BN;
+        m0 = (int) (lid - tn * (unsigned) p.tiles_m) * BM;
+    }
+    const int k_blocks = (p.k + 127) / 128, k16 = (p.k + 15) & ~15, rows_n = min(BN, p.n - n0), rows_m = min(BM, p.m - m0);
+    const char *w_base = p.w + (long long) n0 * p.ws, *a_base = p.a + (long long) m0 * p.as;
+    const unsigned w_bytes = (unsigned) ((rows_n - 1) * p.ws + k16), a_bytes = (unsigned) ((rows_m - 1) * p.as + k16);
+    unsigned w_off[LN], a_off[LM];
+    const int lrow = lane / 8;
+#pragma unroll
+    for (int t = 0; t < LN; ++t) {
+        const int row = (gw * LN + t) * 8 + lrow;
+        w_off[t] = row < rows_n ? (unsigned) (row * p.ws) + ((lane % 8) ^ (row / 2 % 8)) * 16 : OOB;
+    }
+#pragma unroll
+    for (int t = 0; t < LM; ++t) {
+        const int row = (gw * LM + t) * 8 + lrow;
+        a_off[t] = row < rows_m ? (unsigned) (row * p.as) + ((lane % 8) ^ (row / 2 % 8)) * 16 : OOB;
+    }
+    // a lane's scale: of 64 rows a wavefront, of the weights' blocks of 128 in the one behind those
+    constexpr int OWN = BM / WM;
+    const int n_wave = n0 + wn * (BN / WN), m_wave = m0 + wm * OWN, blocks_n = (p.n + 127) / 128;
+    const bool of_rows = gw < BM / 64;
+    const float *scales = of_rows ? p.a_scale + (m0 + min(gw * 64 + lane, rows_m - 1)) * p.a_ss[0] : p.w_scale + min(n0 / 128 + lane, blocks_n - 1) * p.w_ss[0];
+    const long long scale_step = of_rows ? p.a_ss[1] : p.w_ss[1];
+    const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds + kg * DEPTH * SLOT;
+    const unsigned scales0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds + KG * DEPTH * SLOT + kg * 2 * CHUNK;
+    const int share = (k_blocks + KG - 1) / KG, begin = kg * share, end = min(begin + share, k_blocks);
+    auto ask_scales = [&](int i) __attribute__((always_inline)) {   // in front of the block's others: a wait for those is one for it
+        const int kb = begin + i;
+        if (kb >= end || gw > BM / 64) return;
+        const unsigned chunk = scales0 + (i / 4 & 1) * CHUNK;
+        if (!p.quads) word_to_lds(scales + kb * scale_step, chunk + i % 4 * (CHUNK / 4) + gw * 256);
+        else if (i % 4 == 0) quad_to_lds(scales + min(kb, k_blocks - 4), chunk + gw * 1024);
+    };
+    auto ask = [&](int j, int i, int d) __attribute__((always_inline)) {   // j = 0 .. LOADS - 1
+        const bool live = begin + i < end;   // one that is not there is not fetched
+        const unsigned from = live ? (unsigned) (begin + i) * 128u : 0u, to = lds0 + d * SLOT;
+        if (j < LN) load_to_lds(descriptor(w_base, live ? w_bytes : 0u), w_off[j], from, to + (gw * LN + j) * 1024);
+        else load_to_lds(descriptor(a_base, live ? a_bytes : 0u), a_off[j - LN], from, to + BN * 128 + (gw * LM + j - LN) * 1024);
+    };
+    const int row_step = p.quads ? 16 : 4;
+    f32x4 acc[TN][TM] = {};
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) {
+        ask_scales(d);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) ask(j, d, d);
+    }
+    for (int first = 0; first < share; first += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int i = first + d, kb = begin + i;
+            if (i >= share) break;   // uniform over the workgroup
+            // this block is there, and everybody has read the one before it
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((DEPTH - 2) * LOADS) : "memory");
+            const int then = i + DEPTH - 1;
+            ask_scales(then);
+            if (kb >= end) {
+#pragma unroll
+                for (int j = 0; j < LOADS; ++j) ask(j, then, (d + DEPTH - 1) % DEPTH);
+                continue;
+            }
+            const char *slot = lds + (kg * DEPTH + d) * SLOT;
+            const char *factor = lds + KG * DEPTH * SLOT + (kg * 2 + (i / 4 & 1)) * CHUNK + (p.quads ? (kb - min(kb - i % 4, k_blocks - 4)) * 4 : i % 4 * (CHUNK / 4));
+            const float sw = *reinterpret_cast<const float *>(factor + (BM + wn * (BN / WN) / 128) * row_step);
+            float s[TM];
+#pragma unroll
+            for (int t = 0; t < TM; ++t) s[t] = *reinterpret_cast<const float *>(factor + (wm * OWN + t * 16 + li) * row_step) * sw;
+            i32x4 a[TN][2], b[TM][2];
+            auto operand = [&](int row, i32x4 (&x)[2]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[h] = *reinterpret_cast<const i32x4 *>(slot + row * 128 + (lane_unit(lq, h) ^ (row / 2 % 8)) * 16);
+            };
+#pragma unroll
+            for (int t = 0; t < TM; ++t) operand(BN + wm * OWN + t * 16 + li, b[t]);
+#pragma unroll
+            for (int u = 0; u < TN; ++u) operand(wn * (BN / WN) + u * 16 + li, a[u]);
+            if (kb * 128 + 128 > p.k) {   // the last block: nothing behind a row's end takes part
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int keep = p.k - (kb * 128 + lane_unit(lq, h) * 16);
+#pragma unroll
+                    for (int u = 0; u < TN; ++u) a[u][h] = f8_kept(a[u][h], keep);
+#pragma unroll
+                    for (int t = 0; t < TM; ++t) b[t][h] = f8_kept(b[t][h], keep);
+                }
+            }
+            // loads between the matrix instructions: a wavefront stands still where it asks for more than the memory pipe takes at once
+            f32x4 part[TN][TM] = {};
+            auto step = [&](int j) __attribute__((always_inline)) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j < LOADS) ask(j, then, (d + DEPTH - 1) % DEPTH);
+            };
+            static_assert(LOADS <= TN * TM, "a load behind each product");
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        bf16x8 y[TM];
+#pragma unroll
+                        for (int t = 0; t < TM; ++t) y[t] = f8_widened(b[t][h][2 * e], b[t][h][2 * e + 1]);
+#pragma unroll
+                        for (int u = 0; u < TN; ++u) {
+                            const bf16x8 x = f8_widened(a[u][h][2 * e], a[u][h][2 * e + 1]);
+#pragma unroll
+                            for (int t = 0; t < TM; ++t) {
+                                part[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y[t], part[u][t], 0, 0, 0);
+                                if (h == 0 && e == 0) step(u * TM + t);
+                            }
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int u = 0; u < TN; ++u)
+#pragma unroll
+                    for (int t = 0; t < TM; ++t) {
+                        part[u][t] = f8_mma(__builtin_shufflevector(a[u][0], a[u][1], 0, 1, 2, 3, 4, 5, 6, 7), __builtin_shufflevector(b[t][0], b[t][1], 0, 1, 2, 3, 4, 5, 6, 7));
+                        step(u * TM + t);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < TN; ++u)
+#pragma unroll
+                for (int t = 0; t < TM; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[u][t][i] = __builtin_fmaf(part[u][t][i], s[t], acc[u][t][i]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads that wrote nothing but zeros are still on their way to LDS
+    __syncthreads();
+    f32x4 *parts = reinterpret_cast<f32x4 *>(lds);
+    if constexpr (KG > 1) {
+#pragma unroll
+        for (int u = 0; u < TN; ++u)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) parts[(wave * TN * TM + u * TM + t) * 64 + lane] = acc[u][t];
+        __syncthreads();
+    }
+    // a lane has four consecutive outputs of a row; the groups share the tiles out
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int j = u * TM + t;
+            if (KG > 1 && j % KG != kg) continue;   // uniform
+            f32x4 v = acc[u][t];
+            if constexpr (KG > 1) {
+                v = parts[(gw * TN * TM + j) * 64 + lane];
+#pragma unroll
+                for (int g = 1; g < KG; ++g) v += parts[((g * GW + gw) * TN * TM + j) * 64 + lane];
+            }
+            const int m = m_wave + t * 16 + li, n = n_wave + u * 16 + lq * 4;
+            if (m < p.m && n < p.n) store4<DT>(p, m, n, v);
+        }
+#endif
 }
 
-template <int DT, int BN, int BM, int WN, int WM> static int linear_launch(F8LinearParams p, hipStream_t stream) {
-    p.tiles_n = (p.n + BN - 1) / BN;
-    p.tiles_m = (p.m + BM - 1) / BM;
-    hipLaunchKernelGGL((f8_linear_kernel<DT, BN, BM, WN, WM>), dim3((unsigned) p.tiles_n * p.tiles_m), dim3(64 * WN * WM), 0, stream, p);
+template <int DT, int AM, int NT, int WAVES> static int few_launch(const F8LinearParams &p, hipStream_t stream) {
+    hipLaunchKernelGGL((f8_few_kernel<DT, AM, NT, WAVES>), dim3((unsigned) ((p.n + 16 * NT - 1) / (16 * NT)), (unsigned) ((p.m + AM - 1) / AM)), dim3(64 * WAVES), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
@@ -554,9 +605,18 @@ template <int DT> static int many_launch(F8LinearParams p, hipStream_t stream) {
     p.tiles_n = (p.n + 255) / 256;
     p.tiles_m = (p.m + 255) / 256;
     const long long tiles = (long long) p.tiles_n * p.tiles_m;
-    p.by_group = make_div31((unsigned) (8 * p.tiles_n));
-    p.by_last = make_div31((unsigned) (p.tiles_m % 8 ? p.tiles_m % 8 : 8));
+    p.by_group = make_div31((unsigned) (HIGH * p.tiles_n));
+    p.by_last = make_div31((unsigned) (p.tiles_m % HIGH ? p.tiles_m % HIGH : HIGH));
     hipLaunchKernelGGL((f8_many_kernel<DT>), dim3((unsigned) (tiles < 256 ? tiles : 256)), dim3(512), 0, stream, p);
+    ONHIP_CHECK_HIP(hipGetLastError());
+    return ONHIP_OK;
+}
+
+template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH> static int tile_launch(F8LinearParams p, hipStream_t stream) {
+    p.tiles_n = (p.n + BN - 1) / BN;
+    p.tiles_m = (p.m + BM - 1) / BM;
+    p.by_last = make_div31((unsigned) p.tiles_m);
+    hipLaunchKernelGGL((f8_tile_kernel<DT, EXACT, BN, BM, KG, WN, WM, DEPTH>), dim3((unsigned) p.tiles_n * p.tiles_m), dim3(64 * KG * WN * WM), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
@@ -611,22 +671,22 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
         p.w_ss[i] = d->w_scale_strides[i];
     }
     p.vec = !off(out, 4 * (uintptr_t) size) && p.os % (4 * size) == 0;
-    p.wide = !off(out, 16) && p.os % 16 == 0;
     p.quads = p.a_ss[1] == 1 && p.w_ss[1] == 1 && p.k > 3 * 128;
+    p.wide = !off(out, 16) && p.os % 16 == 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     // up to 64 rows: 16 outputs a workgroup, 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and 27.6 us;
     // 4096 of 4096, 16 rows: 5.7 and 7.1), and 32 with all eight for more rows, which come in once for them
     auto few = [&]<int DT>() {
         const bool wide = p.n > 16384;
-        if (p.m <= 8) return wide ? few_launch<DT, 8, 2, 1, 4>(p, st) : few_launch<DT, 8, 1, 1, 8>(p, st);
-        if (p.m <= 16) return wide ? few_launch<DT, 16, 2, 1, 4>(p, st) : few_launch<DT, 16, 1, 1, 8>(p, st);
-        return wide ? few_launch<DT, 32, 2, 1, 4>(p, st) : few_launch<DT, 32, 2, 1, 8>(p, st);
+        if (p.m <= 8) return wide ? few_launch<DT, 8, 2, 4>(p, st) : few_launch<DT, 8, 1, 8>(p, st);
+        if (p.m <= 16) return wide ? few_launch<DT, 16, 2, 4>(p, st) : few_launch<DT, 16, 1, 8>(p, st);
+        return wide ? few_launch<DT, 32, 2, 4>(p, st) : few_launch<DT, 32, 2, 8>(p, st);
     };
     auto go = [&]<int DT>() {
         if (p.m <= 64) return few.template operator()<DT>();
         if constexpr (DT != DT_F32)
             if (p.os <= (1 << 22)) return many_launch<DT>(p, st);
-        return linear_launch<DT, 128, 128, 2, 2>(p, st);
+        return tile_launch<DT, true, 128, 64, 2, 2, 2, 3>(p, st);
     };
     return dt == DT_F32 ? go.template operator()<DT_F32>() : dt == DT_BF16 ? go.template operator()<DT_BF16>() : go.template operator()<DT_F16>();
 }

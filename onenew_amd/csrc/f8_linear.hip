@@ -126,22 +126,24 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
     const long long scale_step = lane < AM ? p.a_ss[1] : p.w_ss[1];
     const unsigned lds0 = (unsigned) (size_t) (__attribute__((address_space(3))) char *) lds + wave * SLOT;
     const i32x4 rw = descriptor(w_base, w_bytes), ra = descriptor(a_base, a_bytes);
-    const int share = (k_blocks + WAVES - 1) / WAVES, begin = wave * share, end = min(begin + share, k_blocks);
-    auto ask = [&](int kb) __attribute__((always_inline)) {
+    // a run of the blocks a wavefront; every WAVESth one where rows are not whole lines apart: two blocks then share a line, which wavefronts take at the same time (32003 outputs of
+    // 4000 channels, 5 rows: 26.2 and 28.9 us; of 4096 channels 10% the other way)
+    const bool spread = p.ws % 128 != 0, quads = p.quads && !spread;
+    const int share = (k_blocks + WAVES - 1) / WAVES, begin = spread ? wave : wave * share, end = spread ? k_blocks : min(begin + share, k_blocks), stride = spread ? WAVES : 1;
+    auto ask = [&](int i, int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < NT * 2; ++t) load_to_lds(rw, w_off[t], (unsigned) kb * 128u, lds0 + t * 1024);
 #pragma unroll
         for (int t = 0; t < AM / 8; ++t) load_to_lds(ra, a_off[t], (unsigned) kb * 128u, lds0 + NT * 2048 + t * 1024);
-        const int i = kb - begin;
         const unsigned to = lds0 + NT * 2048 + AM * 128 + (i / 4 & 1) * CHUNK;
-        if (!p.quads) word_to_lds(scales + kb * scale_step, to + i % 4 * 256);
+        if (!quads) word_to_lds(scales + kb * scale_step, to + i % 4 * 256);
         else if (i % 4 == 0) quad_to_lds(scales + min(kb, k_blocks - 4), to);   // of four blocks, the last four as they are
     };
-    const int row_step = p.quads ? 16 : 4;
+    const int row_step = quads ? 16 : 4;
     f32x4 acc[NT][MT] = {};
-    if (begin < end) ask(begin);
+    if (begin < end) ask(0, begin);
     const char *slot = lds + wave * SLOT;
-    for (int kb = begin; kb < end; ++kb) {
+    for (int i = 0, kb = begin; kb < end; ++i, kb += stride) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         i32x4 w[NT][2], a[MT][2];
         float s[MT];
@@ -155,13 +157,13 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
                 a[t][h] = *reinterpret_cast<const i32x4 *>(slot + NT * 2048 + row * 128 + (lane_unit(lq, h) ^ (row / 2 % 8)) * 16);
             }
         }
-        const int i = kb - begin, first = kb - i % 4;
-        const char *factor = slot + NT * 2048 + AM * 128 + (i / 4 & 1) * CHUNK + (p.quads ? (kb - min(first, k_blocks - 4)) * 4 : i % 4 * 256);
+        const int first = kb - i % 4;
+        const char *factor = slot + NT * 2048 + AM * 128 + (i / 4 & 1) * CHUNK + (quads ? (kb - min(first, k_blocks - 4)) * 4 : i % 4 * 256);
         const float sw = *reinterpret_cast<const float *>(factor + AM * row_step);
 #pragma unroll
         for (int t = 0; t < MT; ++t) s[t] = *reinterpret_cast<const float *>(factor + (AM < 16 ? li % AM : t * 16 + li) * row_step) * sw;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read, so that the place can take another block
-        if (kb + 1 < end) ask(kb + 1);
+        if (kb + stride < end) ask(i + 1, kb + stride);
         if (kb * 128 + 128 > p.k) {   // the last block: nothing behind a row's end takes part
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -227,7 +229,7 @@ __device__ __forceinline__ f32x4 f8_mma(i32x8 a, i32x8 b) {
 #endif
 }
 
-constexpr int HIGH = 4;   // rows of tiles that go together: 32 workgroups of an XCD share 4 x 8 panels at a time
+constexpr int HIGH = 6;   // rows of tiles that go together: 32 workgroups of an XCD share 6 + 6 panels at a time
 
 template <int DT>
 __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
@@ -395,7 +397,7 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
                         x[i] = z[0];
                         y[i] = z[1];
                     }
-                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, n_wide + u * 16 + 8 <= p.n ? off + u * 32 : OOB, 0, 2);   // not kept in the caches
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, n_wide + u * 16 + 8 <= p.n ? off + u * 32 : OOB, 0, 0);
                 }
             }
             stored = true;
@@ -621,6 +623,32 @@ template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
     return ONHIP_OK;
 }
 
+// What a product of more than 32 rows runs on: the least expected time, as rounds of tiles over the 256 compute units (PAIR: two workgroups a unit) times what a block of channels was
+// measured to take there, in us, at 4096 outputs of 4096 channels and 64 to 8192 rows (within a tenth for 22016 outputs and 11008 channels).  300 rows of 11008 channels, 4096 outputs: 50,
+// 45, 33, 41, 69 and 121 us in this order, 2048 rows of 4096 channels: 114, 88, 61, 49, 39 and 50
+enum { BY_FEW, BY_64, BY_128, BY_128_PAIR, BY_SQUARE_PAIR, BY_MANY };
+static int linear_choice(const F8LinearParams &p, bool exact) {
+    static constexpr struct {
+        int n, m, slots;
+        float one, full, exact_one, exact_full, round;   // a block: of a round of up to 256 workgroups, of a full one; in bf16; once a round
+    } ways[] = {{32, 32, 512, 0.14f, 0.25f, 0.14f, 0.26f, 1.0f}, {64, 64, 256, 0.27f, 0.27f, 0.40f, 0.40f, 1.0f}, {128, 64, 256, 0.38f, 0.38f, 0.62f, 0.62f, 1.0f},
+                {128, 64, 512, 0.47f, 0.69f, 0.75f, 1.22f, 1.5f}, {128, 128, 512, 0.78f, 1.10f, 1.15f, 2.05f, 1.5f}, {256, 256, 256, 1.45f, 1.45f, 1e9f, 1e9f, 6.0f}};
+    const float blocks = (float) ((p.k + 127) / 128);
+    int best = BY_FEW;
+    float least = 0.0f;
+    for (int i = 0; i <= BY_MANY; ++i) {
+        if (i == BY_MANY && (exact || p.os > (1 << 22))) break;   // a tile's results within 2^30 bytes
+        const long long tiles = ((long long) (p.n + ways[i].n - 1) / ways[i].n) * ((p.m + ways[i].m - 1) / ways[i].m), rounds = tiles / ways[i].slots, rest = tiles % ways[i].slots;
+        const float one = exact ? ways[i].exact_one : ways[i].one, full = exact ? ways[i].exact_full : ways[i].full;
+        const float t = (float) rounds * (full * blocks + ways[i].round) + (rest == 0 ? 0.0f : (rest <= 256 ? one : full) * blocks + ways[i].round);
+        if (i == 0 || t < least) {
+            best = i;
+            least = t;
+        }
+    }
+    return best;
+}
+
 static bool off(const void *at, uintptr_t to) { return reinterpret_cast<uintptr_t>(at) % to != 0; }
 
 static int linear_check(const onhip_f8_linear_desc_t *d, int *dt) {
@@ -674,19 +702,28 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
     p.quads = p.a_ss[1] == 1 && p.w_ss[1] == 1 && p.k > 3 * 128;
     p.wide = !off(out, 16) && p.os % 16 == 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    // up to 64 rows: 16 outputs a workgroup, 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and 27.6 us;
-    // 4096 of 4096, 16 rows: 5.7 and 7.1), and 32 with all eight for more rows, which come in once for them
+    // up to 32 rows: 16 outputs a workgroup, or 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and
+    // 27.6 us; 4096 of 4096, 16 rows: 5.6 and 7.1)
     auto few = [&]<int DT>() {
         const bool wide = p.n > 16384;
         if (p.m <= 8) return wide ? few_launch<DT, 8, 2, 4>(p, st) : few_launch<DT, 8, 1, 8>(p, st);
         if (p.m <= 16) return wide ? few_launch<DT, 16, 2, 4>(p, st) : few_launch<DT, 16, 1, 8>(p, st);
-        return wide ? few_launch<DT, 32, 2, 4>(p, st) : few_launch<DT, 32, 2, 8>(p, st);
+        if (p.m <= 32 && p.n <= 4096) return few_launch<DT, 32, 1, 8>(p, st);   // 32 rows of 11008 channels, 4096 outputs: 14.0 us, 17.2 with 32 outputs a workgroup
+        return wide && p.m <= 32 ? few_launch<DT, 32, 2, 4>(p, st) : few_launch<DT, 32, 2, 8>(p, st);
     };
     auto go = [&]<int DT>() {
-        if (p.m <= 64) return few.template operator()<DT>();
-        if constexpr (DT != DT_F32)
-            if (p.os <= (1 << 22)) return many_launch<DT>(p, st);
-        return tile_launch<DT, true, 128, 64, 2, 2, 2, 3>(p, st);
+        constexpr bool EXACT = DT == DT_F32;
+        if (p.m <= 32) return few.template operator()<DT>();
+        switch (linear_choice(p, EXACT)) {
+        case BY_FEW: return few.template operator()<DT>();
+        case BY_64: return tile_launch<DT, EXACT, 64, 64, 2, 2, 2, 3>(p, st);
+        case BY_128: return tile_launch<DT, EXACT, 128, 64, 2, 2, 2, 3>(p, st);
+        case BY_128_PAIR: return tile_launch<DT, EXACT, 128, 64, 1, 2, 2, 3>(p, st);
+        case BY_SQUARE_PAIR: return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 2>(p, st);
+        default: break;
+        }
+        if constexpr (!EXACT) return many_launch<DT>(p, st);
+        else return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 2>(p, st);
     };
     return dt == DT_F32 ? go.template operator()<DT_F32>() : dt == DT_BF16 ? go.template operator()<DT_BF16>() : go.template operator()<DT_F16>();
 }

@@ -78,8 +78,8 @@ def linear(a, a_scale, w, w_scale, bias=None, cut=False):
 
 
 def cuts(m, dtype):
-    """whether a product of m rows may sum with 13 bits: more than 64 rows with a result in 16 bits"""
-    return m > 64 and dtype != torch.float32
+    """whether a product of m rows may sum with 13 bits: more than 32 rows with a result in 16 bits"""
+    return m > 32 and dtype != torch.float32
 
 
 def check(got, ref, off):

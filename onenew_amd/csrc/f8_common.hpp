@@ -123,4 +123,28 @@ __device__ __forceinline__ void f8_store(char *at, int left, uint2 q) {
         if (j < left) at[j] = (char) ((j < 4 ? q.x : q.y) >> (j % 4 * 8));
 }
 
+inline bool misaligned(const void *at, uintptr_t to) { return reinterpret_cast<uintptr_t>(at) % to != 0; }
+
+// rows of bytes as a call names them, and whether two of them have no byte in common: spans behind each other, or columns of one matrix
+struct Span {
+    const char *at;
+    long long step, row;   // bytes
+    int rows;
+};
+inline bool apart(const Span &a, const Span &b) {
+    if (!a.at || !b.at) return true;
+    auto last = [](const Span &x) { return x.at + (x.rows - 1) * x.step + x.row; };
+    if (last(a) <= b.at || last(b) <= a.at) return true;
+    const long long step = a.rows > 1 ? a.step : b.step;
+    if ((a.rows > 1 && b.rows > 1 && a.step != b.step) || step == 0) return false;
+    long long off = (b.at - a.at) % step;
+    off = off < 0 ? off + step : off;
+    return off >= a.row && off + b.row <= step;
+}
+// scales as one span of bytes
+inline Span scale_span(const float *scale, const long long *ss, int rows, int blocks) {
+    return {reinterpret_cast<const char *>(scale), 0, 4 * ((rows - 1) * ss[0] + (blocks - 1) * ss[1] + 1), 1};
+}
+inline bool same(const Span &a, const Span &b) { return a.at == b.at && a.step == b.step && a.row == b.row; }
+
 }  // namespace onhip

@@ -634,14 +634,15 @@ static int linear_choice(const F8LinearParams &p, bool exact) {
     } ways[] = {{32, 32, 512, 0.14f, 0.25f, 0.14f, 0.26f, 1.0f}, {64, 64, 256, 0.27f, 0.27f, 0.40f, 0.40f, 1.0f}, {128, 64, 256, 0.38f, 0.38f, 0.62f, 0.62f, 1.0f},
                 {128, 64, 512, 0.47f, 0.69f, 0.75f, 1.22f, 1.5f}, {128, 128, 512, 0.78f, 1.10f, 1.15f, 2.05f, 1.5f}, {256, 256, 256, 1.45f, 1.45f, 1e9f, 1e9f, 6.0f}};
     const float blocks = (float) ((p.k + 127) / 128);
-    int best = BY_FEW;
-    float least = 0.0f;
+    int best = BY_SQUARE_PAIR;
+    float least = INFINITY;
     for (int i = 0; i <= BY_MANY; ++i) {
         if (i == BY_MANY && (exact || p.os > (1 << 22))) break;   // a tile's results within 2^30 bytes
+        if (i == BY_FEW && p.m > 32 * 65535) continue;             // groups of rows are the grid's second dimension
         const long long tiles = ((long long) (p.n + ways[i].n - 1) / ways[i].n) * ((p.m + ways[i].m - 1) / ways[i].m), rounds = tiles / ways[i].slots, rest = tiles % ways[i].slots;
         const float one = exact ? ways[i].exact_one : ways[i].one, full = exact ? ways[i].exact_full : ways[i].full;
         const float t = (float) rounds * (full * blocks + ways[i].round) + (rest == 0 ? 0.0f : (rest <= 256 ? one : full) * blocks + ways[i].round);
-        if (i == 0 || t < least) {
+        if (t < least) {
             best = i;
             least = t;
         }
@@ -649,22 +650,41 @@ static int linear_choice(const F8LinearParams &p, bool exact) {
     return best;
 }
 
-static bool off(const void *at, uintptr_t to) { return reinterpret_cast<uintptr_t>(at) % to != 0; }
-
 static int linear_check(const onhip_f8_linear_desc_t *d, int *dt) {
     const char *what = "e4m3 product";
+    constexpr int MOST = 1 << 30;
     if (!d || d->rows < 1 || d->outputs < 1 || d->channels < 1) return set_error(ONHIP_ERR_ARG, "%s: bad shape", what);
     if (!element_type(d->compute, dt)) return set_error(ONHIP_ERR_ARG, "%s: unknown type %d", what, d->compute);
-    if (d->channels > (1 << 22)) return set_error(ONHIP_ERR_ARG, "%s: %d channels (up to 2^22)", what, d->channels);
+    if (d->rows > MOST || d->outputs > MOST || d->channels > (1 << 22)) return set_error(ONHIP_ERR_ARG, "%s: %d rows, %d outputs, %d channels (up to 2^30, 2^30, 2^22)", what, d->rows, d->outputs, d->channels);
     // byte offsets within a tile stay below 2^31
     const long long most = 1LL << 22;
     if (d->rows > 1 && (d->a_stride < d->channels || d->a_stride > most || d->a_stride % 16)) return set_error(ONHIP_ERR_ARG, "%s: rows %lld bytes apart (a multiple of 16, up to 2^22)", what, d->a_stride);
     if (d->outputs > 1 && (d->w_stride < d->channels || d->w_stride > most || d->w_stride % 16)) return set_error(ONHIP_ERR_ARG, "%s: weights %lld bytes apart (a multiple of 16, up to 2^22)", what, d->w_stride);
     if (d->rows > 1 && (d->out_stride < d->outputs || d->out_stride > (1LL << 40))) return set_error(ONHIP_ERR_ARG, "%s: results %lld elements apart", what, d->out_stride);
-    for (int i = 0; i < 2; ++i)
-        if (d->a_scale_strides[i] < 0 || d->a_scale_strides[i] > (1LL << 31) || d->w_scale_strides[i] < 0 || d->w_scale_strides[i] > (1LL << 31))
-            return set_error(ONHIP_ERR_ARG, "%s: bad scale strides", what);
+    const int blocks = (d->channels + F8_BLOCK - 1) / F8_BLOCK, blocks_n = (d->outputs + F8_BLOCK - 1) / F8_BLOCK, extent[4] = {d->rows, blocks, blocks_n, blocks};
+    for (int i = 0; i < 4; ++i) {
+        const long long stride = i < 2 ? d->a_scale_strides[i] : d->w_scale_strides[i - 2];
+        if (extent[i] > 1 && (stride < 0 || stride > (1LL << 40))) return set_error(ONHIP_ERR_ARG, "%s: bad scale strides", what);
+    }
     return ONHIP_OK;
+}
+
+// sizes and strides; 0 for a stride that is never stepped over
+static F8LinearParams linear_shape(const onhip_f8_linear_desc_t *d, int size) {
+    F8LinearParams p = {};
+    p.m = d->rows;
+    p.n = d->outputs;
+    p.k = d->channels;
+    p.as = d->rows > 1 ? (int) d->a_stride : 0;
+    p.ws = d->outputs > 1 ? (int) d->w_stride : 0;
+    p.os = d->rows > 1 ? d->out_stride * size : 0;
+    const int blocks = (p.k + F8_BLOCK - 1) / F8_BLOCK;
+    p.a_ss[0] = p.m > 1 ? d->a_scale_strides[0] : 0;
+    p.a_ss[1] = blocks > 1 ? d->a_scale_strides[1] : 0;
+    p.w_ss[0] = p.n > F8_BLOCK ? d->w_scale_strides[0] : 0;
+    p.w_ss[1] = blocks > 1 ? d->w_scale_strides[1] : 0;
+    p.quads = blocks >= 4 && p.a_ss[1] == 1 && p.w_ss[1] == 1;
+    return p;
 }
 
 }  // namespace onhip
@@ -673,34 +693,34 @@ using namespace onhip;
 
 extern "C" {
 
+int onhip_linear_f8_way(const onhip_f8_linear_desc_t *d) {
+    int dt;
+    if (int rc = linear_check(d, &dt)) return rc;
+    return d->rows <= 32 ? (int) BY_FEW : linear_choice(linear_shape(d, bytes_of(dt)), dt == DT_F32);
+}
+
 int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float *a_scale, const void *w, const float *w_scale, const float *bias, void *out, void *stream) {
     const char *what = "e4m3 product";
     int dt;
     if (int rc = linear_check(d, &dt)) return rc;
     if (!a || !a_scale || !w || !w_scale || !out) return set_error(ONHIP_ERR_ARG, "%s: null pointer", what);
-    if (off(a, 16) || off(w, 16)) return set_error(ONHIP_ERR_ARG, "%s: rows and weights must be 16-byte aligned", what);
+    if (misaligned(a, 16) || misaligned(w, 16)) return set_error(ONHIP_ERR_ARG, "%s: rows and weights must be 16-byte aligned", what);
     const int size = bytes_of(dt);
-    if (off(a_scale, 4) || off(w_scale, 4) || off(bias, 4) || off(out, (uintptr_t) size)) return set_error(ONHIP_ERR_ARG, "%s: misaligned scales, bias or result", what);
-    F8LinearParams p = {};
+    if (misaligned(a_scale, 4) || misaligned(w_scale, 4) || misaligned(bias, 4) || misaligned(out, (uintptr_t) size)) return set_error(ONHIP_ERR_ARG, "%s: misaligned scales, bias or result", what);
+    F8LinearParams p = linear_shape(d, size);
+    const int blocks = (p.k + F8_BLOCK - 1) / F8_BLOCK, blocks_n = (p.n + F8_BLOCK - 1) / F8_BLOCK;
+    const Span of_out = {static_cast<const char *>(out), p.os, (long long) p.n * size, p.m};
+    for (const Span &from : {Span{static_cast<const char *>(a), p.as, p.k, p.m}, Span{static_cast<const char *>(w), p.ws, p.k, p.n}, scale_span(a_scale, p.a_ss, p.m, blocks), scale_span(w_scale, p.w_ss, blocks_n, blocks),
+                             Span{reinterpret_cast<const char *>(bias), 0, 4LL * p.n, 1}})
+        if (!apart(of_out, from)) return set_error(ONHIP_ERR_ARG, "%s: the result lies over an operand", what);
     p.a = static_cast<const char *>(a);
     p.w = static_cast<const char *>(w);
     p.a_scale = a_scale;
     p.w_scale = w_scale;
     p.bias = bias;
     p.out = static_cast<char *>(out);
-    p.m = d->rows;
-    p.n = d->outputs;
-    p.k = d->channels;
-    p.as = d->rows > 1 ? (int) d->a_stride : 0;
-    p.ws = d->outputs > 1 ? (int) d->w_stride : 0;
-    p.os = d->rows > 1 ? d->out_stride * size : 0;
-    for (int i = 0; i < 2; ++i) {
-        p.a_ss[i] = d->a_scale_strides[i];
-        p.w_ss[i] = d->w_scale_strides[i];
-    }
-    p.vec = !off(out, 4 * (uintptr_t) size) && p.os % (4 * size) == 0;
-    p.quads = p.a_ss[1] == 1 && p.w_ss[1] == 1 && p.k > 3 * 128;
-    p.wide = !off(out, 16) && p.os % 16 == 0;
+    p.vec = !misaligned(out, 4 * (uintptr_t) size) && p.os % (4 * size) == 0;
+    p.wide = !misaligned(out, 16) && p.os % 16 == 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     // up to 32 rows: 16 outputs a workgroup, or 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and
     // 27.6 us; 4096 of 4096, 16 rows: 5.6 and 7.1)

@@ -189,8 +189,6 @@ __global__ __launch_bounds__(256) void f8_weights_kernel(const WeightsParams p) 
 
 // ---- checks and launches -------------------------------------------------------------------------------------------
 
-static bool misaligned(const void *at, uintptr_t to) { return reinterpret_cast<uintptr_t>(at) % to != 0; }
-
 // a matrix of `rows` rows of `n` elements of `size` bytes: its row stride in bytes, 0 where there is one row
 static int row_step(const char *what, const char *name, const void *at, int rows, long long n, long long stride, int size, bool written, long long *step) {
     *step = 0;
@@ -201,28 +199,6 @@ static int row_step(const char *what, const char *name, const void *at, int rows
     *step = stride * size;
     return ONHIP_OK;
 }
-
-// rows of bytes as a call names them, and whether two of them have no byte in common: spans behind each other, or columns of one matrix
-struct Span {
-    const char *at;
-    long long step, row;   // bytes
-    int rows;
-};
-static bool apart(const Span &a, const Span &b) {
-    if (!a.at || !b.at) return true;
-    auto last = [](const Span &x) { return x.at + (x.rows - 1) * x.step + x.row; };
-    if (last(a) <= b.at || last(b) <= a.at) return true;
-    const long long step = a.rows > 1 ? a.step : b.step;
-    if ((a.rows > 1 && b.rows > 1 && a.step != b.step) || step == 0) return false;
-    long long off = (b.at - a.at) % step;
-    off = off < 0 ? off + step : off;
-    return off >= a.row && off + b.row <= step;
-}
-// scales as one span of bytes
-static Span scale_span(const float *scale, const long long *ss, int rows, int blocks) {
-    return {reinterpret_cast<const char *>(scale), 0, 4 * ((rows - 1) * ss[0] + (blocks - 1) * ss[1] + 1), 1};
-}
-static bool same(const Span &a, const Span &b) { return a.at == b.at && a.step == b.step && a.row == b.row; }
 
 // e4m3 rows and scales as results
 static int f8_result(const char *what, void *q, long long q_stride, float *scale, const long long *scale_strides, int rows, int scale_rows, int n, long long *os, long long *ss) {

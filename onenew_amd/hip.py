@@ -42,7 +42,7 @@ EXPORTS = ["onhip_init", "onhip_last_error", "onhip_set_tuning", "onhip_split_ta
            "onhip_h16_from_nchw_f32", "onhip_h16_to_nchw_f32", "onhip_h16_from_rows_f32", "onhip_h16_to_rows_f32",
            "onhip_conv2d_h16", "onhip_h16_first_width", "onhip_h16_first_channels", "onhip_h16_first_input_bytes", "onhip_h16_first_weight_bytes", "onhip_h16_first_from_nchw_f32", "onhip_h16_first_pack_weights", "onhip_conv2d_h16_first", "onhip_linear_h16", "onhip_attention",
            "onhip_cache_append", "onhip_cache_read", "onhip_attention_paged_workspace", "onhip_attention_paged", "onhip_attention_masked_workspace", "onhip_attention_masked",
-           "onhip_rms_norm", "onhip_f8_from_rows", "onhip_linear_f8",
+           "onhip_rms_norm", "onhip_f8_from_rows", "onhip_linear_f8", "onhip_linear_f8_way",
            "onhip_ir_block_supported", "onhip_ir_block_packed_weight_bytes", "onhip_ir_block_pack_weights", "onhip_ir_block_f32",
            "onhip_conv2d_pw_supported", "onhip_conv2d_pw_packed_weight_bytes", "onhip_conv2d_pw_pack_weights", "onhip_conv2d_pw_f32",
            "onhip_add_f32", "onhip_relu_f32", "onhip_maxpool_out_shape", "onhip_maxpool_f32", "onhip_maxpool_s8_nhwc", "onhip_maxpool_s8_eval", "onhip_global_avgpool_f32",
@@ -141,6 +141,7 @@ def load():
     L.onhip_attention_masked.argtypes = [C.POINTER(abi.MaskedAttentionDesc)] + [vp] * 7 + [C.c_size_t, vp]
     L.onhip_rms_norm.argtypes = [C.POINTER(abi.NormDesc)] + [vp] * 7
     L.onhip_f8_from_rows.argtypes = [C.POINTER(abi.F8RowsDesc)] + [vp] * 4
+    L.onhip_linear_f8_way.argtypes = [C.POINTER(abi.F8LinearDesc)]
     L.onhip_linear_f8.argtypes = [C.POINTER(abi.F8LinearDesc)] + [vp] * 7
     L.onhip_ir_block_supported.argtypes = [C.POINTER(ConvDesc)] * 3
     L.onhip_ir_block_packed_weight_bytes.argtypes = [i32, i32, i32]

@@ -1,9 +1,11 @@
 """The product of e4m3 rows and weights with scales for blocks of 128 against 64 bits."""
+import ctypes as C
+
 import pytest
 import torch
 
 import f8_oracle as o
-from onenew_amd import hip
+from onenew_amd import abi, hip
 
 pytestmark = pytest.mark.gpu
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
@@ -35,6 +37,52 @@ def test_product(dtype, m, n, k):
         got = hip.linear_f8(a, sa, w, sw, bias=b, dtype=DT[dtype])
         torch.cuda.synchronize()
         o.check(got, *o.linear(a, sa, w, sw, b, o.cuts(m, DT[dtype])))
+
+
+# one and more of every kernel, whole and ragged at each edge, one block of channels and several, an odd number of workgroups for the XCDs
+WAYS = [(0, 40, 500, 900), (0, 64, 2048, 128), (0, 100, 300, 2056), (1, 200, 4090, 1500), (1, 130, 4096, 4096), (1, 200, 3000, 1000), (2, 400, 4096, 1025), (2, 512, 4000, 700), (3, 128, 20000, 520), (3, 1000, 4096, 640),
+        (4, 600, 10000, 300), (4, 1999, 4090, 1100), (5, 4000, 4096, 4104), (5, 4090, 4090, 1030), (5, 8170, 8150, 640), (5, 8161, 4085, 777)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("i", range(len(WAYS)))
+def test_every_kernel(dtype, i):
+    """the kernel that onhip_linear_f8_way names, for bf16 results (fp32 ones take none of 256 x 256)"""
+    hip.init(0)
+    way, m, n, k = WAYS[i]
+    print(dtype, WAYS[i], flush=True)
+    pitch = (k + 15) // 16 * 16
+    d = abi.F8LinearDesc(m, n, k, abi.COMPUTE_BF16, pitch, pitch, n)
+    assert hip.load().onhip_linear_f8_way(C.byref(d)) == way
+    (a, sa), (w, sw) = operand(m, k, i), operand(n, k, i + 1, True)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(4)).cuda() if i % 2 else None
+    got = hip.linear_f8(a, sa, w, sw, bias=bias, dtype=DT[dtype])
+    o.check(got, *o.linear(a, sa, w, sw, bias, o.cuts(m, DT[dtype])))
+    # scales with the blocks first, which do not lie side by side; results at an odd element; nothing beside them
+    wide = torch.full((m, n + 5), 3.0, dtype=DT[dtype], device="cuda")
+    hip.linear_f8(a, sa.t().contiguous().t(), w, sw.t().contiguous().t(), bias=bias, out=wide[:, 3:3 + n])
+    assert torch.equal(wide[:, 3:3 + n], got) and bool((wide[:, :3] == 3.0).all()) and bool((wide[:, 3 + n:] == 3.0).all())
+    # rows at a multiple of 16 bytes, behind whose ends nothing is written
+    wide = torch.full((m, (n + 7) // 8 * 8 + 16), 3.0, dtype=DT[dtype], device="cuda")
+    hip.linear_f8(a, sa, w, sw, bias=bias, out=wide[:, 8:8 + n])
+    assert torch.equal(wide[:, 8:8 + n], got) and bool((wide[:, :8] == 3.0).all()) and bool((wide[:, 8 + n:] == 3.0).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(200, 4096, 4096), (512, 4096, 4096), (2048, 4096, 4096), (8192, 8192, 1024)])
+def test_how_exact(m, n, k):
+    """ordinary rows, results in fp16: what sums of eight with 13 bits leave out is small next to the result's own rounding.
+
+    A product's cut is uniform in 0 .. 2^-13 of the power of two of the largest of eight, at most a third of the eight's root of summed squares on average, towards zero: with
+    signs as they come, its variance is at most 2^-26 / 3 / 2 of the eight products' summed squares' mean largest, for each of 7: below (2^-13)^2 of the summed squares.  So the error's root
+    mean square is below 2^-13 of the results' (sums of products with random signs have the summed squares as their variance), on top of 2^-11 / sqrt(12) 2 of the rounding."""
+    hip.init(0)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    a, sa = hip.f8_from_rows(torch.randn((m, k), generator=g, device="cuda"))
+    w, sw = hip.f8_from_weights(torch.randn((n, k), generator=g, device="cuda"))
+    ref, _ = o.linear(a, sa, w, sw)
+    size = float(ref.square().mean().sqrt())
+    off = [float((hip.linear_f8(a, sa, w, sw, dtype=t).double() - ref).square().mean().sqrt()) / size for t in (torch.float16, torch.float32)]
+    assert off[0] <= 2.0 ** -13 + 2.0 ** -11 and off[1] <= 2.0 ** -20, off
 
 
 @pytest.mark.parametrize("m", [1, 20, 70, 300])

@@ -123,6 +123,10 @@ __device__ __forceinline__ void f8_store(char *at, int left, uint2 q) {
         if (j < left) at[j] = (char) ((j < 4 ? q.x : q.y) >> (j % 4 * 8));
 }
 
+// workgroups in rows of 2^21, for a row's threads are counted in 32 bits; what is behind the last one returns
+inline dim3 f8_grid(long long groups) { return dim3((unsigned) (groups < (1 << 21) ? groups : 1 << 21), (unsigned) ((groups + (1 << 21) - 1) >> 21)); }
+__device__ __forceinline__ long long f8_group() { return (long long) blockIdx.y * (1 << 21) + blockIdx.x; }
+
 inline bool misaligned(const void *at, uintptr_t to) { return reinterpret_cast<uintptr_t>(at) % to != 0; }
 
 // rows of bytes as a call names them, and whether two of them have no byte in common: spans behind each other, or columns of one matrix

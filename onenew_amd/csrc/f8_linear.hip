@@ -13,7 +13,6 @@ namespace onhip {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-
 struct F8LinearParams {
     const char *a, *w;
     const float *a_scale, *w_scale, *bias;
@@ -607,6 +606,7 @@ template <int DT> static int many_launch(F8LinearParams p, hipStream_t stream) {
     p.tiles_n = (p.n + 255) / 256;
     p.tiles_m = (p.m + 255) / 256;
     const long long tiles = (long long) p.tiles_n * p.tiles_m;
+    if (tiles >= 1LL << 31) return set_error(ONHIP_ERR_ARG, "e4m3 product: %lld tiles", tiles);
     p.by_group = make_div31((unsigned) (HIGH * p.tiles_n));
     p.by_last = make_div31((unsigned) (p.tiles_m % HIGH ? p.tiles_m % HIGH : HIGH));
     hipLaunchKernelGGL((f8_many_kernel<DT>), dim3((unsigned) (tiles < 256 ? tiles : 256)), dim3(512), 0, stream, p);
@@ -618,26 +618,33 @@ template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
     p.tiles_n = (p.n + BN - 1) / BN;
     p.tiles_m = (p.m + BM - 1) / BM;
     p.by_last = make_div31((unsigned) p.tiles_m);
-    hipLaunchKernelGGL((f8_tile_kernel<DT, EXACT, BN, BM, KG, WN, WM, DEPTH>), dim3((unsigned) p.tiles_n * p.tiles_m), dim3(64 * KG * WN * WM), 0, stream, p);
+    const long long tiles = (long long) p.tiles_n * p.tiles_m;
+    constexpr int THREADS = 64 * KG * WN * WM;
+    if (tiles * THREADS >= 1LL << 32) return set_error(ONHIP_ERR_ARG, "e4m3 product: %lld tiles", tiles);   // a launch's threads
+    hipLaunchKernelGGL((f8_tile_kernel<DT, EXACT, BN, BM, KG, WN, WM, DEPTH>), dim3((unsigned) tiles), dim3(THREADS), 0, stream, p);
     ONHIP_CHECK_HIP(hipGetLastError());
     return ONHIP_OK;
 }
 
 // What a product of more than 32 rows runs on: the least expected time, as rounds of tiles over the 256 compute units (PAIR: two workgroups a unit) times what a block of channels was
-// measured to take there, in us, at 4096 outputs of 4096 channels and 64 to 8192 rows (within a tenth for 22016 outputs and 11008 channels).  300 rows of 11008 channels, 4096 outputs: 50,
-// 45, 33, 41, 69 and 121 us in this order, 2048 rows of 4096 channels: 114, 88, 61, 49, 39 and 50
-enum { BY_FEW, BY_64, BY_128, BY_128_PAIR, BY_SQUARE_PAIR, BY_MANY };
+// measured to take there, in us, with weights that come from memory, at 4096 outputs of 4096 channels and 33 to 2048 rows (mostly within a tenth for 22016 outputs and 11008 channels).
+// bf16 results, in this order: 256 rows of 4096 channels, 4096 outputs 21, 14, 18, 21, 28, 38 and 61 us; 1024 rows 67, 50, 36, 32, 29, 38 and 61; 2048 rows 126, 110, 78, 61, 56, 46
+// and 62; 300 rows of 11008 channels 58, 57, 44, 47, 66, 90 and 143; 512 rows of 4096, 22016 outputs 208, 148, 117, 96, 83, 84 and 65
+enum { BY_FEW, BY_64, BY_128, BY_128_PAIR, BY_SQUARE, BY_SQUARE_PAIR, BY_MANY };
 static int linear_choice(const F8LinearParams &p, bool exact) {
+    constexpr float never = 1e9f;                                     // 128 x 128 in bf16 takes alone what it takes in pairs, up to 256 of them
     static constexpr struct {
         int n, m, slots;
         float one, full, exact_one, exact_full, round;   // a block: of a round of up to 256 workgroups, of a full one; in bf16; once a round
-    } ways[] = {{32, 32, 512, 0.14f, 0.25f, 0.14f, 0.26f, 1.0f}, {64, 64, 256, 0.27f, 0.27f, 0.40f, 0.40f, 1.0f}, {128, 64, 256, 0.38f, 0.38f, 0.62f, 0.62f, 1.0f},
-                {128, 64, 512, 0.47f, 0.69f, 0.75f, 1.22f, 1.5f}, {128, 128, 512, 0.78f, 1.10f, 1.15f, 2.05f, 1.5f}, {256, 256, 256, 1.45f, 1.45f, 1e9f, 1e9f, 6.0f}};
+    } ways[] = {{32, 32, 512, 0.15f, 0.26f, 0.15f, 0.27f, 1.0f}, {64, 64, 256, 0.32f, 0.32f, 0.40f, 0.40f, 1.0f}, {128, 64, 256, 0.46f, 0.46f, 0.62f, 0.62f, 1.0f},
+                {128, 64, 512, 0.50f, 0.85f, 0.68f, 1.15f, 1.5f}, {128, 128, 256, 0.73f, 0.73f, never, never, 1.5f}, {128, 128, 512, 1.00f, 1.30f, 1.12f, 1.95f, 1.5f},
+                {256, 256, 256, 1.65f, 1.65f, never, never, 6.0f}};
     const float blocks = (float) ((p.k + 127) / 128);
     int best = BY_SQUARE_PAIR;
     float least = INFINITY;
     for (int i = 0; i <= BY_MANY; ++i) {
-        if (i == BY_MANY && (exact || p.os > (1 << 22))) break;   // a tile's results within 2^30 bytes
+        if (exact && ways[i].exact_one == never) continue;
+        if (i == BY_MANY && p.os > (1 << 22)) break;               // a tile's results within 2^30 bytes
         if (i == BY_FEW && p.m > 32 * 65535) continue;             // groups of rows are the grid's second dimension
         const long long tiles = ((long long) (p.n + ways[i].n - 1) / ways[i].n) * ((p.m + ways[i].m - 1) / ways[i].m), rounds = tiles / ways[i].slots, rest = tiles % ways[i].slots;
         const float one = exact ? ways[i].exact_one : ways[i].one, full = exact ? ways[i].exact_full : ways[i].full;
@@ -652,10 +659,10 @@ static int linear_choice(const F8LinearParams &p, bool exact) {
 
 static int linear_check(const onhip_f8_linear_desc_t *d, int *dt) {
     const char *what = "e4m3 product";
-    constexpr int MOST = 1 << 30;
+    constexpr int MOST = 1 << 27;
     if (!d || d->rows < 1 || d->outputs < 1 || d->channels < 1) return set_error(ONHIP_ERR_ARG, "%s: bad shape", what);
     if (!element_type(d->compute, dt)) return set_error(ONHIP_ERR_ARG, "%s: unknown type %d", what, d->compute);
-    if (d->rows > MOST || d->outputs > MOST || d->channels > (1 << 22)) return set_error(ONHIP_ERR_ARG, "%s: %d rows, %d outputs, %d channels (up to 2^30, 2^30, 2^22)", what, d->rows, d->outputs, d->channels);
+    if (d->rows > MOST || d->outputs > MOST || d->channels > (1 << 22)) return set_error(ONHIP_ERR_ARG, "%s: %d rows, %d outputs, %d channels (up to 2^27, 2^27, 2^22)", what, d->rows, d->outputs, d->channels);
     // byte offsets within a tile stay below 2^31
     const long long most = 1LL << 22;
     if (d->rows > 1 && (d->a_stride < d->channels || d->a_stride > most || d->a_stride % 16)) return set_error(ONHIP_ERR_ARG, "%s: rows %lld bytes apart (a multiple of 16, up to 2^22)", what, d->a_stride);
@@ -740,10 +747,10 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
         case BY_128: return tile_launch<DT, EXACT, 128, 64, 2, 2, 2, 3>(p, st);
         case BY_128_PAIR: return tile_launch<DT, EXACT, 128, 64, 1, 2, 2, 3>(p, st);
         case BY_SQUARE_PAIR: return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 2>(p, st);
-        default: break;
+        case BY_SQUARE: if constexpr (!EXACT) return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 3>(p, st); break;
+        case BY_MANY: if constexpr (!EXACT) return many_launch<DT>(p, st); break;
         }
-        if constexpr (!EXACT) return many_launch<DT>(p, st);
-        else return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 2>(p, st);
+        return set_error(ONHIP_ERR_ARG, "%s: no kernel", what);
     };
     return dt == DT_F32 ? go.template operator()<DT_F32>() : dt == DT_BF16 ? go.template operator()<DT_BF16>() : go.template operator()<DT_F16>();
 }

@@ -28,8 +28,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
     constexpr int SIZE = element_bytes<DT>, STEP = 512 * WAVES;
     __shared__ float part[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long row = WAVES == 1 ? (long long) blockIdx.x * 4 + wave : (long long) blockIdx.x;
-    if (row >= p.rows) return;   // WAVES == 1 alone, where nothing below synchronises
+    const long long row = WAVES == 1 ? f8_group() * 4 + wave : f8_group();
+    if (row >= p.rows) return;   // all of a workgroup, or WAVES == 1, where nothing below synchronises
     const char *x = p.x + row * p.xs, *res = p.res ? p.res + row * p.rs : nullptr;
     const int first = (WAVES == 1 ? 0 : wave) * 512 + lane * 8;
 
@@ -127,7 +127,7 @@ struct RowsParams {
 template <int DT, bool GATED, bool VEC>
 __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsParams p) {
     constexpr int SIZE = element_bytes<DT>;
-    const unsigned item = blockIdx.x * 16 + threadIdx.x / 16;
+    const unsigned item = (unsigned) f8_group() * 16 + threadIdx.x / 16;
     if (item >= p.items) return;   // sixteen lanes at a time, and what follows is between those
     const long long row = div31(item, p.by_blocks);
     const int block = (int) (item - (unsigned) row * p.blocks), at = block * F8_BLOCK + (threadIdx.x & 15) * 8, left = p.n - at;
@@ -156,14 +156,16 @@ struct WeightsParams {
     float *scale;
     long long xs, os;
     long long ss[2];
-    int rows, n, blocks;
+    int rows, n, blocks, scale_rows;
 };
 
 // a workgroup a block of 128 x 128: sixteen lanes have 128 channels of eight of its rows
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void f8_weights_kernel(const WeightsParams p) {
     __shared__ float part[4];
-    const int tile = (int) (blockIdx.x / (unsigned) p.blocks), block = (int) (blockIdx.x % (unsigned) p.blocks);
+    const unsigned group = (unsigned) f8_group();
+    const int tile = (int) (group / (unsigned) p.blocks), block = (int) (group % (unsigned) p.blocks);
+    if (tile >= p.scale_rows) return;
     const int at = block * F8_BLOCK + (threadIdx.x & 15) * 8, left = p.n - at;
     const long long first = (long long) tile * F8_BLOCK + threadIdx.x / 16;
     float y[8][8], top = 0.0f;
@@ -219,7 +221,7 @@ template <int DT, bool F8, bool VEC>
 static int norm_launch(const NormParams &p, hipStream_t stream) {
     const unsigned rows = (unsigned) p.rows;
     auto go = [&]<int WAVES, int NI, bool LONG>() {
-        hipLaunchKernelGGL((rms_norm_kernel<DT, F8, WAVES, NI, LONG, VEC>), dim3(WAVES == 1 ? (rows + 3) / 4 : rows), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, p);
+        hipLaunchKernelGGL((rms_norm_kernel<DT, F8, WAVES, NI, LONG, VEC>), f8_grid(WAVES == 1 ? (rows + 3) / 4 : rows), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, p);
     };
     if (p.n <= 512) go.template operator()<1, 1, false>();
     else if (p.n <= 2048) go.template operator()<4, 1, false>();
@@ -307,11 +309,11 @@ int onhip_f8_from_rows(const onhip_f8_rows_desc_t *d, const void *x, void *q, fl
     if (items >= (1LL << 31) - 16) return set_error(ONHIP_ERR_ARG, "%s: too many rows", what);
     const bool vec = !misaligned(x, 16) && xs % 16 == 0 && (!gated || (long long) d->channels * size % 16 == 0);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned) groups);
+    const dim3 grid = f8_grid(groups);
     const char *from = static_cast<const char *>(x);
     char *to = static_cast<char *>(q);
     if (weights) {
-        const WeightsParams p = {from, to, scale, xs, os, {ss[0], ss[1]}, d->rows, d->channels, blocks};
+        const WeightsParams p = {from, to, scale, xs, os, {ss[0], ss[1]}, d->rows, d->channels, blocks, scale_rows};
         auto go = [&]<int DT>() {
             if (vec) hipLaunchKernelGGL((f8_weights_kernel<DT, true>), grid, dim3(256), 0, st, p);
             else hipLaunchKernelGGL((f8_weights_kernel<DT, false>), grid, dim3(256), 0, st, p);

@@ -40,14 +40,15 @@ def test_product(dtype, m, n, k):
 
 
 # one and more of every kernel, whole and ragged at each edge, one block of channels and several, an odd number of workgroups for the XCDs
-WAYS = [(0, 40, 500, 900), (0, 64, 2048, 128), (0, 100, 300, 2056), (1, 200, 4090, 1500), (1, 130, 4096, 4096), (1, 200, 3000, 1000), (2, 400, 4096, 1025), (2, 512, 4000, 700), (3, 128, 20000, 520), (3, 1000, 4096, 640),
-        (4, 600, 10000, 300), (4, 1999, 4090, 1100), (5, 4000, 4096, 4104), (5, 4090, 4090, 1030), (5, 8170, 8150, 640), (5, 8161, 4085, 777)]
+WAYS = [(0, 40, 500, 900), (0, 64, 2048, 128), (0, 100, 300, 2056), (1, 200, 4090, 1500), (1, 130, 4096, 4096), (1, 200, 3000, 1000), (2, 400, 4096, 1025), (2, 512, 4000, 700), (3, 64, 40000, 520), (3, 50, 33000, 1000),
+        (4, 128, 20000, 520), (4, 1000, 4096, 640), (4, 333, 10007, 130), (5, 600, 10000, 300), (5, 1999, 4090, 1100), (6, 4000, 4096, 4104), (6, 4090, 4090, 1030), (6, 8170, 8150, 640),
+        (6, 8161, 4085, 777)]
 
 
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("i", range(len(WAYS)))
 def test_every_kernel(dtype, i):
-    """the kernel that onhip_linear_f8_way names, for bf16 results (fp32 ones take none of 256 x 256)"""
+    """the kernel that onhip_linear_f8_way names, for bf16 results (fp32 ones take none of 256 x 256, and 128 x 128 in pairs alone)"""
     hip.init(0)
     way, m, n, k = WAYS[i]
     print(dtype, WAYS[i], flush=True)

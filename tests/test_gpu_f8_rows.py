@@ -127,3 +127,23 @@ def test_far_rows():
     q, scale = hip.f8_from_rows(x, out=far)
     want, want_scale = o.to_f8(x.float().cpu())
     assert torch.equal(scale.cpu(), want_scale) and torch.equal(q.cpu().contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("form", ["rows", "weights", "norm"])
+def test_many_rows(form):
+    """more workgroups than a launch's first dimension takes: every row, all alike, is written"""
+    hip.init(0)
+    rows, n = {"rows": ((1 << 25) + 40, 16), "weights": ((1 << 28) + 130, 16), "norm": ((1 << 21) + 3, 528)}[form]
+    x = _rows(1, n, torch.bfloat16, 7).expand(rows, n)
+    q = torch.full((rows, n), 0x55, dtype=torch.uint8, device="cuda").view(o.F8)
+    print(form, rows, n, flush=True)
+    if form == "norm":
+        q, scale = hip.rms_norm(x, f8=True, out=q)
+        first = hip.rms_norm(x[:1], f8=True)
+    else:
+        q, scale = (hip.f8_from_weights if form == "weights" else hip.f8_from_rows)(x, out=q)
+        first = (hip.f8_from_weights if form == "weights" else hip.f8_from_rows)(x[:1])
+    q = q.view(torch.uint8)
+    assert scale.shape[0] == (-(-rows // 128) if form == "weights" else rows) and bool((scale == first[1]).all())
+    for at in range(0, rows, 1 << 24):
+        assert bool((q[at:at + (1 << 24)] == first[0].view(torch.uint8)).all())

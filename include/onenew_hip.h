@@ -529,7 +529,7 @@ typedef struct onhip_f8_linear_desc {
     long long out_stride;
     long long a_scale_strides[2], w_scale_strides[2];
 } onhip_f8_linear_desc_t;
-/* Diagnostic: the kernel that a product of these sizes runs on: 0 few rows, 1 to 5 tiles of 64 x 64 to 128 x 128, 6 tiles of 256 x 256; negative for what onhip_linear_f8 refuses. */
+/* Diagnostic: the kernel that a product of these sizes runs on: 0 few rows, 1 to 6 tiles of 64 x 64 to 128 x 128, 7 tiles of 256 x 256; negative for what onhip_linear_f8 refuses. */
 int onhip_linear_f8_way(const onhip_f8_linear_desc_t *d);
 int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float *a_scale, const void *w, const float *w_scale,
                     const float *bias, void *out, void *stream);

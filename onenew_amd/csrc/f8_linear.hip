@@ -1,12 +1,16 @@
 // Product of rows and weights in 8-bit floating point:
 //   out[m][n] = sum over blocks b of 128 channels  sa[m][b] sw[n / 128][b] (sum_k a[m][k] w[n][k])  + bias[n]
 //
-// The inner sums are matrix instructions in bf16, which holds every e4m3, that start at zero; sums over blocks are fp32, a fused multiply-add a
-// value.  (The instructions on e4m3 itself sum eight products at a time with 13 bits below the largest of them.)  Weights are the instruction's rows, so that a
-// lane's values belong to one row m: a block has one factor a lane, sa[m] times the wavefront's sw.
+// A block's inner sums are matrix instructions that start at zero, sums over blocks fp32, a fused multiply-add a value.  Up to 32 rows, and for fp32 results, the instructions are those in bf16,
+// which holds every e4m3: they wait for the weights there.  For 16-bit results of more rows they are those on e4m3 itself, in half the time: these add eight products at a time with 13 bits below the
+// power of two of the largest one (what is below is cut), each eight joined in fp32.
+// Weights are the instruction's rows, so that a lane's values belong to one row m and a lane has one factor a block and tile of sixteen rows, sa[m] times sw.
 //
-// Tiles of both operands go from memory straight into LDS, a block of 128 channels of every row a stage, two stages; a row's 16-byte units are exchanged
-// as (unit ^ row / 2 % 8), which puts the sixteen rows that are read together on different banks.
+// Operands go from memory straight into LDS, a block of 128 channels of a row at a time; a row's 16-byte units are exchanged as (unit ^ row / 2 % 8), which puts the sixteen units that are
+// read together on different banks.
+//
+// Three kernels: up to 32 rows a wavefront's own ring, bound by the weights' bytes; more rows tiles for a compute unit, bound by what goes into its LDS (48 to 56 bytes a cycle and unit are the
+// most that direct loads reached); many rows tiles of 256 x 256, bound by matrix instructions and the multiply-adds of the scales beside them.
 #include "f8_common.hpp"
 
 namespace onhip {
@@ -95,7 +99,9 @@ template <int DT> __device__ __forceinline__ void store4(const F8LinearParams &p
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // A workgroup has 16 NT outputs of AM rows, its wavefronts a run of the blocks of channels each.  A wavefront has a place for a block in LDS of its own,
 // which nobody else waits for, and takes the next one when it has read the last; whole lines come in (a load of matrix operands straight into registers takes sixteen rows at once, a line each:
-// 10 bytes a cycle and compute unit were measured so).  The wavefronts' sums meet in LDS, in one order.
+// 10 bytes a cycle and compute unit were measured so).  The wavefronts' sums meet in LDS, in one order.  Deeper rings cost wavefronts a unit and were level or behind.
+// Bound by the weights' bytes: 32 rows of 4096 channels, 22016 outputs 18.3 us (92 MB at 5.0 TB/s; a large copy reaches 4.9 to 5.4), 5 rows of 4000, 32003 fp32 outputs 26.5 us (129 MB, 4.9 TB/s);
+// one row of 4096, 6144 outputs 6.4 us, of which half are the launch and a wavefront's first loads.
 template <int DT, int AM, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -218,8 +224,10 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
 // A workgroup a compute unit walks over tiles of 256 weights x 256 rows, eight wavefronts of 128 x 64: 2048 cycles of matrix instructions a block of channels, whose tiles come in during the
-// block before, across the ends of tiles.  Matrix instructions on e4m3 itself: they take half the time of those in bf16 and sum eight products at a time with 13 bits below the largest
-// of them (cut), each eight joined in fp32; the result's own rounding is 2^-9 of it in bf16, 2^-12 in fp16.
+// block before, across the ends of tiles.  A matrix instruction has four multiply-adds beside it, which a SIMD with two wavefronts issues in its time but for a seventh (37 cycles for 32).
+// 8192 rows of 4096 channels, 22016 outputs: 680 us, 2.17 PFLOP/s; 8192 of 8192, 8192 outputs 452 us, 2.43 PFLOP/s.  (Instructions alone reach 4.3 to 4.9 in a loop; the clock falls to some 2 GHz.)
+// Measured and not kept: a block's last products held back over the barrier, loads a block and a half ahead with two barriers a block (8192^3 486 us), lines asked for ahead of time, stores past the
+// caches (650 us with operands in the last-level cache, 701 with operands from memory).
 __device__ __forceinline__ f32x4 f8_mma(i32x8 a, i32x8 b) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{}, 0, 0, 0, 0, 0, 0);
@@ -228,7 +236,7 @@ __device__ __forceinline__ f32x4 f8_mma(i32x8 a, i32x8 b) {
 #endif
 }
 
-constexpr int HIGH = 6;   // rows of tiles that go together: 32 workgroups of an XCD share 6 + 6 panels at a time
+constexpr int HIGH = 6;   // rows of tiles that go together: 32 workgroups of an XCD share 6 + 6 panels at a time (2 or 8 some percent slower, 16 and 32 much)
 
 template <int DT>
 __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
@@ -425,12 +433,15 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
 // A workgroup has BN weights x BM rows, its wavefronts WN x WM parts of them in each of KG groups, and a group a run of the blocks of channels, in a ring of DEPTH blocks: tiles
 // enough for the compute units, and wavefronts enough for a unit, where there are few rows.  The groups' sums meet in LDS, in one order.
 // EXACT: matrix instructions in bf16, which sum in fp32.
+// Bound by what goes into LDS: a block of 96 x 64 is 20 KB for 192 cycles of matrix instructions, and takes some 800.  300 rows of 11008 channels, 4096 outputs 38 us with weights from memory (0.7 PFLOP/s,
+// 215 tiles on 256 units), 26 to 30 from the last-level cache.  Measured and not kept: operands of the next block read ahead into registers, lines asked for ahead of time (2 to 15% behind).
 template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
 __global__ __launch_bounds__(64 * KG * WN * WM) void f8_tile_kernel(const F8LinearParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int GW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16, LN = BN / 8 / GW, LM = BM / 8 / GW, LOADS = LN + LM;
     constexpr int SLOT = (BN + BM) * 128, CHUNK = (BM + 64) * 16, RING = KG * (DEPTH * SLOT + 2 * CHUNK), JOIN = KG * GW * TN * TM * 1024;
-    static_assert(BN / WN <= 128 && BM % 64 == 0 && BM / 64 < GW && LN >= 1 && LM >= 1, "a wavefront's weights share a scale, 64 rows' scales are a wavefront's load, those of the weights another's, and every wavefront loads");
+    constexpr bool ONE = 128 % (BN / WN) == 0;   // a wavefront's weights share a scale; else sixteen of them do
+    static_assert(BN % (16 * WN) == 0 && BM % 64 == 0 && BM / 64 < GW && LN >= 1 && LM >= 1, "64 rows' scales are a wavefront's load, those of the weights another's, and every wavefront loads");
     __shared__ __attribute__((aligned(1024))) char lds[RING > JOIN ? RING : JOIN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, lq = lane >> 4, kg = wave / GW, gw = wave % GW, wn = gw / WM, wm = gw % WM;
@@ -502,10 +513,11 @@ __global__ __launch_bounds__(64 * KG * WN * WM) void f8_tile_kernel(const F8Line
             }
             const char *slot = lds + (kg * DEPTH + d) * SLOT;
             const char *factor = lds + KG * DEPTH * SLOT + (kg * 2 + (i / 4 & 1)) * CHUNK + (p.quads ? (kb - min(kb - i % 4, k_blocks - 4)) * 4 : i % 4 * (CHUNK / 4));
-            const float sw = *reinterpret_cast<const float *>(factor + (BM + wn * (BN / WN) / 128) * row_step);
-            float s[TM];
+            float s[TM], sw[TN];
 #pragma unroll
-            for (int t = 0; t < TM; ++t) s[t] = *reinterpret_cast<const float *>(factor + (wm * OWN + t * 16 + li) * row_step) * sw;
+            for (int u = 0; u < (ONE ? 1 : TN); ++u) sw[u] = *reinterpret_cast<const float *>(factor + (BM + (n_wave + u * 16) / 128 - n0 / 128) * row_step);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) s[t] = *reinterpret_cast<const float *>(factor + (wm * OWN + t * 16 + li) * row_step) * (ONE ? sw[0] : 1.0f);
             i32x4 a[TN][2], b[TM][2];
             auto operand = [&](int row, i32x4 (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -562,9 +574,11 @@ __global__ __launch_bounds__(64 * KG * WN * WM) void f8_tile_kernel(const F8Line
 #pragma unroll
             for (int u = 0; u < TN; ++u)
 #pragma unroll
-                for (int t = 0; t < TM; ++t)
+                for (int t = 0; t < TM; ++t) {
+                    const float by = ONE ? s[t] : s[t] * sw[u];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[u][t][i] = __builtin_fmaf(part[u][t][i], s[t], acc[u][t][i]);
+                    for (int i = 0; i < 4; ++i) acc[u][t][i] = __builtin_fmaf(part[u][t][i], by, acc[u][t][i]);
+                }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads that wrote nothing but zeros are still on their way to LDS
@@ -628,16 +642,17 @@ template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
 
 // What a product of more than 32 rows runs on: the least expected time, as rounds of tiles over the 256 compute units (PAIR: two workgroups a unit) times what a block of channels was
 // measured to take there, in us, with weights that come from memory, at 4096 outputs of 4096 channels and 33 to 2048 rows (mostly within a tenth for 22016 outputs and 11008 channels).
-// bf16 results, in this order: 256 rows of 4096 channels, 4096 outputs 21, 14, 18, 21, 28, 38 and 61 us; 1024 rows 67, 50, 36, 32, 29, 38 and 61; 2048 rows 126, 110, 78, 61, 56, 46
-// and 62; 300 rows of 11008 channels 58, 57, 44, 47, 66, 90 and 143; 512 rows of 4096, 22016 outputs 208, 148, 117, 96, 83, 84 and 65
-enum { BY_FEW, BY_64, BY_128, BY_128_PAIR, BY_SQUARE, BY_SQUARE_PAIR, BY_MANY };
+// bf16 results: 256 rows of 4096 channels, 4096 outputs 22, 14, 16, 18, 19, 28, 38 and 62 us in this order; 400 rows, 6144 outputs 43, 36, 29, 32, 26, 28, 38 and 60; 1024 rows, 4096 outputs 63,
+// 50, 44, 36, 40, 29, 38 and 61; 2048 rows 117, 104, 87, 72, 69, 55, 46 and 62; 300 rows of 11008 channels 56, 56, 38, 44, 44, 64, 89 and 143; 512 rows of 4096, 22016 outputs 198, 136, 116,
+// 106, 95, 82, 83 and 65.  fp32 results: 700 rows of 11008, 4096 outputs 117, 104, 90, 106, 83 and, in pairs, 101
+enum { BY_FEW, BY_64, BY_96, BY_128, BY_96_PAIR, BY_SQUARE, BY_SQUARE_PAIR, BY_MANY };
 static int linear_choice(const F8LinearParams &p, bool exact) {
     constexpr float never = 1e9f;                                     // 128 x 128 in bf16 takes alone what it takes in pairs, up to 256 of them
     static constexpr struct {
         int n, m, slots;
         float one, full, exact_one, exact_full, round;   // a block: of a round of up to 256 workgroups, of a full one; in bf16; once a round
-    } ways[] = {{32, 32, 512, 0.15f, 0.26f, 0.15f, 0.27f, 1.0f}, {64, 64, 256, 0.32f, 0.32f, 0.40f, 0.40f, 1.0f}, {128, 64, 256, 0.46f, 0.46f, 0.62f, 0.62f, 1.0f},
-                {128, 64, 512, 0.50f, 0.85f, 0.68f, 1.15f, 1.5f}, {128, 128, 256, 0.73f, 0.73f, never, never, 1.5f}, {128, 128, 512, 1.00f, 1.30f, 1.12f, 1.95f, 1.5f},
+    } ways[] = {{32, 32, 512, 0.15f, 0.26f, 0.15f, 0.27f, 1.0f}, {64, 64, 256, 0.32f, 0.32f, 0.40f, 0.40f, 1.0f}, {96, 64, 256, 0.38f, 0.38f, 0.53f, 0.53f, 1.0f},
+                {128, 64, 256, 0.46f, 0.46f, 0.62f, 0.62f, 1.0f}, {96, 64, 512, 0.44f, 0.67f, 0.62f, 0.93f, 1.5f}, {128, 128, 256, 0.73f, 0.73f, never, never, 1.5f}, {128, 128, 512, 1.00f, 1.30f, 1.12f, 1.95f, 1.5f},
                 {256, 256, 256, 1.65f, 1.65f, never, never, 6.0f}};
     const float blocks = (float) ((p.k + 127) / 128);
     int best = BY_SQUARE_PAIR;
@@ -744,8 +759,9 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
         switch (linear_choice(p, EXACT)) {
         case BY_FEW: return few.template operator()<DT>();
         case BY_64: return tile_launch<DT, EXACT, 64, 64, 2, 2, 2, 3>(p, st);
+        case BY_96: return tile_launch<DT, EXACT, 96, 64, 2, 2, 2, 3>(p, st);
         case BY_128: return tile_launch<DT, EXACT, 128, 64, 2, 2, 2, 3>(p, st);
-        case BY_128_PAIR: return tile_launch<DT, EXACT, 128, 64, 1, 2, 2, 3>(p, st);
+        case BY_96_PAIR: return tile_launch<DT, EXACT, 96, 64, 1, 2, 2, 3>(p, st);
         case BY_SQUARE_PAIR: return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 2>(p, st);
         case BY_SQUARE: if constexpr (!EXACT) return tile_launch<DT, EXACT, 128, 128, 1, 2, 2, 3>(p, st); break;
         case BY_MANY: if constexpr (!EXACT) return many_launch<DT>(p, st); break;

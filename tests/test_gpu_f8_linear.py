@@ -40,9 +40,9 @@ def test_product(dtype, m, n, k):
 
 
 # one and more of every kernel, whole and ragged at each edge, one block of channels and several, an odd number of workgroups for the XCDs
-WAYS = [(0, 40, 500, 900), (0, 64, 2048, 128), (0, 100, 300, 2056), (1, 200, 4090, 1500), (1, 130, 4096, 4096), (1, 200, 3000, 1000), (2, 400, 4096, 1025), (2, 512, 4000, 700), (3, 64, 40000, 520), (3, 50, 33000, 1000),
-        (4, 128, 20000, 520), (4, 1000, 4096, 640), (4, 333, 10007, 130), (5, 600, 10000, 300), (5, 1999, 4090, 1100), (6, 4000, 4096, 4104), (6, 4090, 4090, 1030), (6, 8170, 8150, 640),
-        (6, 8161, 4085, 777)]
+WAYS = [(0, 40, 500, 900), (0, 64, 2048, 128), (0, 100, 300, 2056), (1, 200, 4090, 1500), (1, 130, 4096, 4096), (1, 200, 3000, 1000), (2, 300, 4090, 2056), (2, 200, 6100, 1500), (2, 40, 20000, 300),
+        (3, 400, 4096, 1025), (3, 512, 4000, 700), (4, 64, 40000, 520), (4, 333, 6000, 130), (4, 700, 4096, 640), (4, 128, 20000, 520), (5, 1000, 4096, 640), (5, 333, 10007, 130),
+        (6, 600, 10000, 300), (6, 1999, 4090, 1100), (7, 4000, 4096, 4104), (7, 4090, 4090, 1030), (7, 8170, 8150, 640), (7, 8161, 4085, 777)]
 
 
 @pytest.mark.parametrize("dtype", DT)

@@ -27,7 +27,7 @@ struct F8LinearParams {
     int m, n, k;
     int tiles_m, tiles_n;
     Div31 by_group, by_last;         // tiles in HIGH rows of them; rows of tiles in the last such group
-    bool vec, wide;                  // four results are one aligned store; eight, in rows up to 2^22 bytes apart
+    bool wide;                       // rows of results start at whole words
     bool quads;                      // scales of a row's blocks lie side by side, four of them at least
 };
 
@@ -83,9 +83,9 @@ template <int DT> __device__ __forceinline__ void store4(const F8LinearParams &p
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += n + j < p.n ? p.bias[n + j] : 0.0f;
     char *at = p.out + m * p.os + (long long) n * element_bytes<DT>;
-    if (p.vec && n + 4 <= p.n) {
-        if constexpr (DT == DT_F32) *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
-        else *reinterpret_cast<uint2 *>(at) = make_uint2(pack_h16<DT>(v[0], v[1]), pack_h16<DT>(v[2], v[3]));
+    if (n + 4 <= p.n) {
+        if constexpr (DT == DT_F32) *reinterpret_cast<any_f32x4 *>(at) = v;
+        else *reinterpret_cast<any_u32x2 *>(at) = any_u32x2{pack_h16<DT>(v[0], v[1]), pack_h16<DT>(v[2], v[3])};
         return;
     }
 #pragma unroll
@@ -387,29 +387,30 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
 #pragma unroll
                     for (int t = 0; t < TM; ++t) acc[u][t][i] += bias;
                 }
-        if (p.wide) {
-            // two tiles' halves exchanged between groups of lanes: eight consecutive outputs a lane
-            const int n_wide = n0 + wn * 128 + (l >> 4) % 2 * 16 + (l >> 5) * 8;
+        // two tiles' halves exchanged between groups of lanes: eight consecutive outputs a lane
+        const int n_wide = n0 + wn * 128 + (l >> 4) % 2 * 16 + (l >> 5) * 8;
 #pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const unsigned off = row + t * 16 < rows ? (unsigned) ((row + t * 16) * p.os) + n_wide * 2 : OOB;
+        for (int t = 0; t < TM; ++t) {
+            const bool live = row + t * 16 < rows;
+            const unsigned off = (unsigned) ((row + t * 16) * p.os) + n_wide * 2;
 #pragma unroll
-                for (int u = 0; u < TN; u += 2) {
-                    unsigned x[2], y[2];
+            for (int u = 0; u < TN; u += 2) {
+                unsigned x[2], y[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[i] = pack_h16<DT>(acc[u][t][2 * i], acc[u][t][2 * i + 1]);
-                        y[i] = pack_h16<DT>(acc[u + 1][t][2 * i], acc[u + 1][t][2 * i + 1]);
-                        const auto z = __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false);
-                        x[i] = z[0];
-                        y[i] = z[1];
-                    }
-                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, n_wide + u * 16 + 8 <= p.n ? off + u * 32 : OOB, 0, 0);
+                for (int i = 0; i < 2; ++i) {
+                    x[i] = pack_h16<DT>(acc[u][t][2 * i], acc[u][t][2 * i + 1]);
+                    y[i] = pack_h16<DT>(acc[u + 1][t][2 * i], acc[u + 1][t][2 * i + 1]);
+                    const auto z = __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false);
+                    x[i] = z[0];
+                    y[i] = z[1];
                 }
+                const bool there = live && n_wide + u * 16 + 8 <= p.n;
+                if (p.wide) __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, ro, there ? off + u * 32 : OOB, 0, 0);
+                else if (there) *reinterpret_cast<any_u32x4 *>(p.out + m0 * p.os + off + u * 32) = any_u32x4{x[0], x[1], y[0], y[1]};
             }
-            stored = true;
         }
-        const int from = p.wide ? p.n & ~7 : 0;   // one at a time: all of them, or the last ones of a row
+        stored = p.wide;
+        const int from = p.n & ~7;   // the last ones of a row, one at a time
         if (from < p.n && n0 + BN > from) {
 #pragma unroll
             for (int t = 0; t < TM; ++t) {
@@ -741,8 +742,7 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
     p.w_scale = w_scale;
     p.bias = bias;
     p.out = static_cast<char *>(out);
-    p.vec = !misaligned(out, 4 * (uintptr_t) size) && p.os % (4 * size) == 0;
-    p.wide = !misaligned(out, 16) && p.os % 16 == 0;
+    p.wide = !misaligned(out, 4) && p.os % 4 == 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     // up to 32 rows: 16 outputs a workgroup, or 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and
     // 27.6 us; 4096 of 4096, 16 rows: 5.6 and 7.1)

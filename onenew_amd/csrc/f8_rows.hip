@@ -27,7 +27,7 @@ struct NormParams {
 
 // WAVES wavefronts a row (one: four rows a workgroup), NI groups of eight channels a lane, so that a row stays in registers between its sum and its result; a row longer than that (LONG) is read twice.
 // One row's time is its chain of loads, sum and store: 4096 channels take four wavefronts 3 us with the launch
-template <int DT, bool F8, int WAVES, int NI, bool LONG, bool VEC>
+template <int DT, bool F8, int WAVES, int NI, bool LONG>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel(const NormParams p) {
     constexpr int SIZE = element_bytes<DT>, STEP = 512 * WAVES;
     __shared__ float part[WAVES];
@@ -38,10 +38,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
     const int first = (WAVES == 1 ? 0 : wave) * 512 + lane * 8;
 
     auto load = [&](int at, float (&h)[8]) __attribute__((always_inline)) {
-        load8<DT, VEC>(x + (long long) at * SIZE, p.n - at, h);
+        load8<DT>(x + (long long) at * SIZE, p.n - at, h);
         if (res) {
             float r[8];
-            load8<DT, VEC>(res + (long long) at * SIZE, p.n - at, r);
+            load8<DT>(res + (long long) at * SIZE, p.n - at, r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[j] += r[j];
         }
@@ -89,9 +89,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
 
     auto finish = [&](int at, const float (&v)[8]) __attribute__((always_inline)) {
         const int left = p.n - at;
-        if (p.sum && left > 0) store8<DT, VEC>(p.sum + row * p.us + (long long) at * SIZE, left, v);
+        if (p.sum && left > 0) store8<DT>(p.sum + row * p.us + (long long) at * SIZE, left, v);
         float y[8], w[8];
-        if (p.weight) load8<DT_F32, VEC>(reinterpret_cast<const char *>(p.weight + at), left, w);
+        if (p.weight) load8<DT_F32>(reinterpret_cast<const char *>(p.weight + at), left, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = v[j] * by * root * (p.weight ? w[j] : 1.0f);
         if constexpr (F8) {
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
                 if (lane % 16 == 0) p.scale[row * p.ss[0] + at / F8_BLOCK * p.ss[1]] = s;
             }
         } else {
-            if (left > 0) store8<DT, VEC>(p.out + row * p.os + (long long) at * SIZE, left, y);
+            if (left > 0) store8<DT>(p.out + row * p.os + (long long) at * SIZE, left, y);
         }
     };
     if constexpr (LONG) {
@@ -128,7 +128,7 @@ struct RowsParams {
 };
 
 // sixteen lanes a block of 128, four blocks a wavefront
-template <int DT, bool GATED, bool VEC>
+template <int DT, bool GATED>
 __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsParams p) {
     constexpr int SIZE = element_bytes<DT>;
     const unsigned item = (unsigned) f8_group() * 16 + threadIdx.x / 16;
@@ -136,10 +136,10 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsParams p) {
     const long long row = div31(item, p.by_blocks);
     const int block = (int) (item - (unsigned) row * p.blocks), at = block * F8_BLOCK + (threadIdx.x & 15) * 8, left = p.n - at;
     float y[8];
-    load8<DT, VEC>(p.x + row * p.xs + (long long) at * SIZE, left, y);
+    load8<DT>(p.x + row * p.xs + (long long) at * SIZE, left, y);
     if constexpr (GATED) {
         float u[8];
-        load8<DT, VEC>(p.x + row * p.xs + ((long long) p.n + at) * SIZE, left, u);
+        load8<DT>(p.x + row * p.xs + ((long long) p.n + at) * SIZE, left, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             // e^-|g|, so that neither side leaves fp32's range; off by |g| 2^-24 of itself (an exponent in two parts changed one e4m3 of 25 million)
@@ -164,7 +164,7 @@ struct WeightsParams {
 };
 
 // a workgroup a block of 128 x 128: sixteen lanes have 128 channels of eight of its rows
-template <int DT, bool VEC>
+template <int DT>
 __global__ __launch_bounds__(256) void f8_weights_kernel(const WeightsParams p) {
     __shared__ float part[4];
     const unsigned group = (unsigned) f8_group();
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void f8_weights_kernel(const WeightsParams p) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const long long row = first + 16 * i;
-        load8<DT, VEC>(p.x + row * p.xs + (long long) at * element_bytes<DT>, row < p.rows ? left : 0, y[i]);
+        load8<DT>(p.x + row * p.xs + (long long) at * element_bytes<DT>, row < p.rows ? left : 0, y[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, block_top(y[i]));
@@ -221,11 +221,11 @@ static int f8_result(const char *what, void *q, long long q_stride, float *scale
     return ONHIP_OK;
 }
 
-template <int DT, bool F8, bool VEC>
+template <int DT, bool F8>
 static int norm_launch(const NormParams &p, hipStream_t stream) {
     const unsigned rows = (unsigned) p.rows;
     auto go = [&]<int WAVES, int NI, bool LONG>() {
-        hipLaunchKernelGGL((rms_norm_kernel<DT, F8, WAVES, NI, LONG, VEC>), f8_grid(WAVES == 1 ? (rows + 3) / 4 : rows), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, p);
+        hipLaunchKernelGGL((rms_norm_kernel<DT, F8, WAVES, NI, LONG>), f8_grid(WAVES == 1 ? (rows + 3) / 4 : rows), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, p);
     };
     if (p.n <= 512) go.template operator()<1, 1, false>();
     else if (p.n <= 2048) go.template operator()<4, 1, false>();
@@ -284,11 +284,8 @@ int onhip_rms_norm(const onhip_norm_desc_t *d, const void *x, const void *residu
     p.rows = d->rows;
     p.n = d->channels;
     p.eps = d->eps;
-    const bool vec = !misaligned(x, 16) && p.xs % 16 == 0 && !misaligned(residual, 16) && p.rs % 16 == 0 && !misaligned(weight, 16) && !misaligned(sum, 16) && p.us % 16 == 0 &&
-                     (d->f8 || (!misaligned(out, 16) && p.os % 16 == 0));
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    auto by_vec = [&]<int DT, bool F8>() { return vec ? norm_launch<DT, F8, true>(p, st) : norm_launch<DT, F8, false>(p, st); };
-    auto by_kind = [&]<int DT>() { return d->f8 ? by_vec.template operator()<DT, true>() : by_vec.template operator()<DT, false>(); };
+    auto by_kind = [&]<int DT>() { return d->f8 ? norm_launch<DT, true>(p, st) : norm_launch<DT, false>(p, st); };
     return dt == DT_F32 ? by_kind.template operator()<DT_F32>() : dt == DT_BF16 ? by_kind.template operator()<DT_BF16>() : by_kind.template operator()<DT_F16>();
 }
 
@@ -311,7 +308,6 @@ int onhip_f8_from_rows(const onhip_f8_rows_desc_t *d, const void *x, void *q, fl
     if (!apart(of_q, of_x) || !apart(of_scale, of_x) || !apart(of_q, of_scale)) return set_error(ONHIP_ERR_ARG, "%s: results lie over the operand or over each other", what);
     const long long items = (long long) scale_rows * blocks, groups = weights ? items : (items + 15) / 16;
     if (items >= (1LL << 31) - 16) return set_error(ONHIP_ERR_ARG, "%s: too many rows", what);
-    const bool vec = !misaligned(x, 16) && xs % 16 == 0 && (!gated || (long long) d->channels * size % 16 == 0);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const dim3 grid = f8_grid(groups);
     const char *from = static_cast<const char *>(x);
@@ -319,15 +315,13 @@ int onhip_f8_from_rows(const onhip_f8_rows_desc_t *d, const void *x, void *q, fl
     if (weights) {
         const WeightsParams p = {from, to, scale, xs, os, {ss[0], ss[1]}, d->rows, d->channels, blocks, scale_rows};
         auto go = [&]<int DT>() {
-            if (vec) hipLaunchKernelGGL((f8_weights_kernel<DT, true>), grid, dim3(256), 0, st, p);
-            else hipLaunchKernelGGL((f8_weights_kernel<DT, false>), grid, dim3(256), 0, st, p);
+            hipLaunchKernelGGL((f8_weights_kernel<DT>), grid, dim3(256), 0, st, p);
         };
         dt == DT_F32 ? go.template operator()<DT_F32>() : dt == DT_BF16 ? go.template operator()<DT_BF16>() : go.template operator()<DT_F16>();
     } else {
         const RowsParams p = {from, to, scale, xs, os, {ss[0], ss[1]}, d->channels, blocks, (unsigned) items, make_div31((unsigned) blocks)};
         auto go = [&]<int DT, bool GATED>() {
-            if (vec) hipLaunchKernelGGL((f8_rows_kernel<DT, GATED, true>), grid, dim3(256), 0, st, p);
-            else hipLaunchKernelGGL((f8_rows_kernel<DT, GATED, false>), grid, dim3(256), 0, st, p);
+            hipLaunchKernelGGL((f8_rows_kernel<DT, GATED>), grid, dim3(256), 0, st, p);
         };
         auto by_form = [&]<int DT>() { gated ? go.template operator()<DT, true>() : go.template operator()<DT, false>(); };
         dt == DT_F32 ? by_form.template operator()<DT_F32>() : dt == DT_BF16 ? by_form.template operator()<DT_BF16>() : by_form.template operator()<DT_F16>();

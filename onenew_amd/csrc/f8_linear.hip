@@ -225,7 +225,7 @@ __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams
 // ---- many rows -----------------------------------------------------------------------------------------------------
 // A workgroup a compute unit walks over tiles of 256 weights x 256 rows, eight wavefronts of 128 x 64: 2048 cycles of matrix instructions a block of channels, whose tiles come in during the
 // block before, across the ends of tiles.  A matrix instruction has four multiply-adds beside it, which a SIMD with two wavefronts issues in its time but for a seventh (37 cycles for 32).
-// 8192 rows of 4096 channels, 22016 outputs: 680 us, 2.17 PFLOP/s; 8192 of 8192, 8192 outputs 452 us, 2.43 PFLOP/s.  (Instructions alone reach 4.3 to 4.9 in a loop; the clock falls to some 2 GHz.)
+// 8192 rows of 4096 channels, 22016 outputs: 681 to 690 us, 2.15 PFLOP/s; 8192 of 8192, 8192 outputs 452 us, 2.43 PFLOP/s.  (Instructions alone reach 4.3 to 4.9 in a loop; the clock falls to some 2 GHz.)
 // Measured and not kept: a block's last products held back over the barrier, loads a block and a half ahead with two barriers a block (8192^3 486 us), lines asked for ahead of time, stores past the
 // caches (650 us with operands in the last-level cache, 701 with operands from memory).
 __device__ __forceinline__ f32x4 f8_mma(i32x8 a, i32x8 b) {

@@ -268,11 +268,11 @@ int onhip_rms_norm(const onhip_norm_desc_t *d, const void *x, const void *residu
                of_out = {static_cast<const char *>(out), p.os, d->f8 ? (long long) d->channels : row, d->rows},
                of_scale = scale_span(d->f8 ? out_scale : nullptr, p.ss, d->rows, (int) blocks);
     if (!apart(of_out, of_sum) || !apart(of_out, of_scale) || !apart(of_sum, of_scale)) return set_error(ONHIP_ERR_ARG, "%s: one memory for two results", what);
-    // a lane writes an element when it has read what it needs of the operands' there: results of the operands' type may take their places
+    // a lane writes an element when it has read x and the residual there: results of their type may take their places, but not the weight's, which is read behind the sum's store and by every row
     auto fits = [&](const Span &result, bool like) {
-        for (const Span &from : {of_x, of_r, of_w})
+        for (const Span &from : {of_x, of_r})
             if (!apart(result, from) && !(like && same(result, from))) return false;
-        return true;
+        return apart(result, of_w);
     };
     if (!fits(of_out, !d->f8) || !fits(of_sum, true) || !fits(of_scale, false)) return set_error(ONHIP_ERR_ARG, "%s: a result lies over an operand", what);
     p.x = static_cast<const char *>(x);

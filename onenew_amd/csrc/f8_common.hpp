@@ -80,11 +80,11 @@ template <int DT> __device__ __forceinline__ void store8(char *at, int left, con
         }
 }
 
-// the largest magnitude of a block whose values sixteen lanes have, eight each; NaN is passed over
+// the largest magnitude of a block whose values sixteen lanes have, eight each; NaN is passed over, and a block of nothing else has 0
 __device__ __forceinline__ float block_top(const float (&y)[8]) {
-    float top = fabsf(y[0]);
+    float top = 0.0f;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, fabsf(y[j]));
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(y[j]));
     top = fmaxf(top, lane_moved<DPP_XOR1>(top));
     top = fmaxf(top, lane_moved<DPP_XOR2>(top));
     top = fmaxf(top, lane_moved<DPP_MIRROR8>(top));

@@ -138,16 +138,29 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsParams p) {
     float y[8];
     load8<DT>(p.x + row * p.xs + (long long) at * SIZE, left, y);
     if constexpr (GATED) {
-        float u[8];
+        constexpr float LOG2E = 1.44269504088896340736f;
+        float u[8], z[8], lowest = 0.0f;
         load8<DT>(p.x + row * p.xs + ((long long) p.n + at) * SIZE, left, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            // e^-|g|, so that neither side leaves fp32's range; off by |g| 2^-24 of itself (an exponent in two parts changed one e4m3 of 25 million)
-            const float g = y[j], e = __builtin_amdgcn_exp2f(fabsf(g) * -1.44269504088896340736f), d = 1.0f + e;
+            // e^-|g|, so that neither side leaves fp32's range; off by 1.25 |g| 2^-24 of itself, the exponent's rounding and its constant's (an exponent in two parts changed one e4m3 of 25 million)
+            const float g = y[j], e = __builtin_amdgcn_exp2f(fabsf(g) * -LOG2E), d = 1.0f + e;
             float inv = __builtin_amdgcn_rcpf(d);
             inv = __builtin_fmaf(__builtin_fmaf(-d, inv, 1.0f), inv, inv);
-            y[j] = (g < 0.0f ? g * e : g) * inv * u[j];
+            z[j] = (g < 0.0f ? g * e : g) * inv * u[j];
+            lowest = fminf(lowest, g);
         }
+        if (lowest < -87.0f) {
+            // The instruction gives zero for a subnormal e, from g = -87.34 on, where g e u need not be small: g e^g u with e^g in three parts, the last two the square root of what is
+            // below 2^-120 (1 + e^g is 1 there).  Below -1000 it is zero for every u
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float g = fmaxf(y[j], -1000.0f), a = g * LOG2E, high = fmaxf(a, -120.0f), low = __builtin_amdgcn_exp2f(0.5f * (a - high));
+                if (y[j] < -87.0f && y[j] > -INFINITY) z[j] = g * __builtin_amdgcn_exp2f(high) * u[j] * low * low;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = z[j];
     }
     const float s = f8_scale(block_top(y));
     if (left > 0) f8_store(p.out + row * p.os + at, left, f8_pack(y, s));

@@ -86,6 +86,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
         total = squares(by);
     }
     const float root = rsqrtf(total / (float) p.n + p.eps * by * by);
+    // the small one of a value's two factors behind the other: a small value of a row that is scaled down, times 2^-80 at first, would lose bits as a subnormal number
+    const float once = by < 1.0f ? root : by, then = by < 1.0f ? by : root;
 
     auto finish = [&](int at, const float (&v)[8]) __attribute__((always_inline)) {
         const int left = p.n - at;
@@ -93,7 +95,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
         float y[8], w[8];
         if (p.weight) load8<DT_F32>(reinterpret_cast<const char *>(p.weight + at), left, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = v[j] * by * root * (p.weight ? w[j] : 1.0f);
+        for (int j = 0; j < 8; ++j) y[j] = v[j] * once * then * (p.weight ? w[j] : 1.0f);
         if constexpr (F8) {
             const float s = f8_scale(block_top(y));
             if (left > 0) {

@@ -270,7 +270,7 @@ class F8LinearDesc(C.Structure):
     """onhip_f8_linear_desc_t"""
     _fields_ = [("rows", C.c_int32), ("outputs", C.c_int32), ("channels", C.c_int32), ("compute", C.c_int32),
                 ("a_stride", C.c_longlong), ("w_stride", C.c_longlong), ("out_stride", C.c_longlong),
-                ("a_scale_strides", C.c_longlong * 2), ("w_scale_strides", C.c_longlong * 2)]
+                ("a_scale_strides", C.c_longlong * 2), ("w_scale_strides", C.c_longlong * 2), ("exact", C.c_int32)]
 
 
 def check_layout():

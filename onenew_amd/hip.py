@@ -1152,7 +1152,7 @@ def f8_from_weights(w, out=None, scale_out=None):
     return _f8_rows("f8_from_weights", abi.F8_WEIGHTS, w, out, scale_out)
 
 
-def _linear_f8_plan(a, a_scale, w, w_scale, bias, dtype, out):
+def _linear_f8_plan(a, a_scale, w, w_scale, bias, dtype, out, exact):
     import torch
     what = "linear_f8"
     compute = _f8_compute(what, dtype)
@@ -1165,19 +1165,21 @@ def _linear_f8_plan(a, a_scale, w, w_scale, bias, dtype, out):
     _need(what, torch.float32, (_f8_blocks(outputs), _f8_blocks(n)), w_scale=w_scale)
     _need(what, torch.float32, (outputs,), flat=True, bias=bias)
     _rows_of(what, dtype, (rows, outputs), out=out)
-    d = abi.F8LinearDesc(rows, outputs, n, compute, a.stride(0), w.stride(0), outputs if out is None else out.stride(0), a_scale.stride(), w_scale.stride())
+    d = abi.F8LinearDesc(rows, outputs, n, compute, a.stride(0), w.stride(0), outputs if out is None else out.stride(0), a_scale.stride(), w_scale.stride(), int(exact))
     return C.byref(d), (rows, outputs), rows == 0 or outputs == 0
 
 
-def linear_f8(a, a_scale, w, w_scale, bias=None, dtype=None, out=None):
+def linear_f8(a, a_scale, w, w_scale, bias=None, dtype=None, out=None, exact=False):
     """a [rows, channels] times w [outputs, channels], both e4m3 rows with fp32 scales ([rows, blocks of 128 channels] and [blocks of 128 outputs, blocks of 128
-    channels], any strides), plus bias [outputs] (float32): [rows, outputs] in `dtype` (float32, float16 or bfloat16, which it is unless given)"""
+    channels], any strides), plus bias [outputs] (float32): [rows, outputs] in `dtype` (float32, float16 or bfloat16, which it is unless given).  Sums are those of 32 bits
+    up to 32 rows and for float32; more rows in 16 bits add eight products at a time with 13 bits, in about half the time, unless `exact`"""
     import torch
+    exact = bool(exact)
     dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
     key = (_device(), a.dtype, a.get_device(), a.shape, a.stride(), a_scale.dtype, a_scale.get_device(), a_scale.shape, a_scale.stride(),
-           w.dtype, w.get_device(), w.shape, w.stride(), w_scale.dtype, w_scale.get_device(), w_scale.shape, w_scale.stride(), _flat(bias), dtype, _meta(out))
+           w.dtype, w.get_device(), w.shape, w.stride(), w_scale.dtype, w_scale.get_device(), w_scale.shape, w_scale.stride(), _flat(bias), dtype, _meta(out), exact)
     last = _last.get("linear f8")
-    d, shape, empty = last[1] if last is not None and last[0] == key else _plan("linear f8", key, _linear_f8_plan, a, a_scale, w, w_scale, bias, dtype, out)
+    d, shape, empty = last[1] if last is not None and last[0] == key else _plan("linear f8", key, _linear_f8_plan, a, a_scale, w, w_scale, bias, dtype, out, exact)
     if out is None:
         out = a.new_empty(shape, dtype=dtype)
     if not empty:

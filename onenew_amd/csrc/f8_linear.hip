@@ -102,8 +102,9 @@ template <int DT> __device__ __forceinline__ void store4(const F8LinearParams &p
 // A workgroup has 16 NT outputs of AM rows, its wavefronts a run of the blocks of channels each.  A wavefront has a place for a block in LDS of its own,
 // which nobody else waits for, and takes the next one when it has read the last; whole lines come in (a load of matrix operands straight into registers takes sixteen rows at once, a line each:
 // 10 bytes a cycle and compute unit were measured so).  The wavefronts' sums meet in LDS, in one order.  Deeper rings cost wavefronts a unit and were level or behind.
-// Bound by the weights' bytes: 32 rows of 4096 channels, 22016 outputs 18.3 us (92 MB at 5.0 TB/s; a large copy reaches 4.9 to 5.4), 5 rows of 4000, 32003 fp32 outputs 26.5 us (129 MB, 4.9 TB/s);
-// one row of 4096, 6144 outputs 6.4 us, of which half are the launch and a wavefront's first loads.
+// Bound by the weights' bytes.  On the device, with weights from memory and from the last-level cache: 32 rows of 4096 channels, 22016 outputs 23.9 and 17.0 us (92 MB at 3.8 and 5.4 TB/s; a large
+// copy reaches 4.9 to 5.4), 5 rows of 4000, 32003 fp32 outputs 28.4 and 21.5 us (129 MB, 4.5 and 6.0 TB/s); one row of 4096, 6144 outputs 7.5 and 4.9 us, where the launch and a wavefront's first
+// loads count.
 template <int DT, int AM, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void f8_few_kernel(const F8LinearParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(512) void f8_many_kernel(const F8LinearParams p) {
 // ---- some rows -----------------------------------------------------------------------------------------------------
 // A workgroup has BN weights x BM rows, its wavefronts WN x WM parts of them in each of KG groups, and a group a run of the blocks of channels, in a ring of DEPTH blocks: tiles
 // enough for the compute units, and wavefronts enough for a unit, where there are few rows.  The groups' sums meet in LDS, in one order.
-// EXACT: matrix instructions in bf16, which sum in fp32.
+// EXACT: matrix instructions in bf16, which sum in fp32: for fp32 results, and for 16-bit ones where they are asked for.
 // Bound by what goes into LDS: a block of 96 x 64 is 20 KB for 192 cycles of matrix instructions, and takes some 800.  300 rows of 11008 channels, 4096 outputs 38 us with weights from memory (0.7 PFLOP/s,
 // 215 tiles on 256 units), 26 to 30 from the last-level cache.  Measured and not kept: operands of the next block read ahead into registers, lines asked for ahead of time (2 to 15% behind).
 template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
@@ -645,9 +646,9 @@ template <int DT, bool EXACT, int BN, int BM, int KG, int WN, int WM, int DEPTH>
 
 // What a product of more than 32 rows runs on: the least expected time, as rounds of tiles over the 256 compute units (PAIR: two workgroups a unit) times what a block of channels was
 // measured to take there, in us, with weights that come from memory, at 4096 outputs of 4096 channels and 33 to 2048 rows (mostly within a tenth for 22016 outputs and 11008 channels).
-// bf16 results: 256 rows of 4096 channels, 4096 outputs 22, 14, 16, 18, 19, 28, 38 and 62 us in this order; 400 rows, 6144 outputs 43, 36, 29, 32, 26, 28, 38 and 60; 1024 rows, 4096 outputs 63,
+// Sums of 13 bits, bf16 results: 256 rows of 4096 channels, 4096 outputs 22, 14, 16, 18, 19, 28, 38 and 62 us in this order; 400 rows, 6144 outputs 43, 36, 29, 32, 26, 28, 38 and 60; 1024 rows, 4096 outputs 63,
 // 50, 44, 36, 40, 29, 38 and 61; 2048 rows 117, 104, 87, 72, 69, 55, 46 and 62; 300 rows of 11008 channels 56, 56, 38, 44, 44, 64, 89 and 143; 512 rows of 4096, 22016 outputs 198, 136, 116,
-// 106, 95, 82, 83 and 65.  fp32 results: 700 rows of 11008, 4096 outputs 117, 104, 90, 106, 83 and, in pairs, 101
+// 106, 95, 82, 83 and 65.  Exact sums, fp32 results: 700 rows of 11008, 4096 outputs 117, 104, 90, 106, 83 and, in pairs, 101
 enum { BY_FEW, BY_64, BY_96, BY_128, BY_96_PAIR, BY_SQUARE, BY_SQUARE_PAIR, BY_MANY };
 static int linear_choice(const F8LinearParams &p, bool exact) {
     constexpr float never = 1e9f;                                     // 128 x 128 in bf16 takes alone what it takes in pairs, up to 256 of them
@@ -748,7 +749,7 @@ int onhip_linear_f8(const onhip_f8_linear_desc_t *d, const void *a, const float 
     p.wide = !misaligned(out, 4) && p.os % 4 == 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     // up to 32 rows: 16 outputs a workgroup, or 32 and half as many wavefronts where that leaves four workgroups a compute unit (32003 outputs of 4000 channels, 5 rows: 28.8 and
-    // 27.6 us; 4096 of 4096, 16 rows: 5.6 and 7.1)
+    // 27.6 us; 4096 of 4096, 16 rows: 5.6 and 7.1; weights from the last-level cache.  Widths between those were not timed)
     auto few = [&]<int DT>() {
         const bool wide = p.n > 16384;
         if (p.m <= 8) return wide ? few_launch<DT, 8, 2, 4>(p, st) : few_launch<DT, 8, 1, 8>(p, st);

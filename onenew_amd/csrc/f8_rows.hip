@@ -3,7 +3,7 @@
 //
 //   norm:   h = x + r,  sum = round(h),  y = h / sqrt(mean(h^2) + eps) * w
 //   gated:  y = g / (1 + e^-g) * u, g and u the two halves of a row
-// in fp32; y goes out in x's type or as e4m3 and scales.
+// in fp32; y goes out in x's type or as e4m3 and scales.  What leaves fp32's range on the way and not in the result has a way of its own: squares of a row, the exponential of a low gate.
 //
 // A lane has eight consecutive channels (16 bytes of a 16-bit type in, 8 bytes of e4m3 out), sixteen lanes a block of 128: its largest magnitude goes from
 // lane to lane in the vector pipe.  Every operand is read once and every result written once (rows of the norm past 16384 channels are read twice).
